@@ -68,8 +68,7 @@
 
 #include <math.h>
 
-#include <mutex>
-
+#include "gemm_common.cuh"
 #include "host_common.h"
 #include "norm_rope_math.cuh"
 #include "ptx_sm100.cuh"
@@ -78,8 +77,6 @@ namespace hdit {
 namespace {
 
 constexpr int kTileK = 64;  // one 128-byte swizzle row of 16-bit elements
-constexpr uint32_t kSpinLimit = 8u * 1000u * 1000u;
-constexpr int kMaxSmem = 232448;  // 227 KiB opt-in limit per CTA
 // Relative time per 128 x 128 of output for each work-unit shape, from measurement; used only to choose a shape. 256 x 256
 // pair : 128 x 256 : 128 x 128, us per wave: 10.6 : 11.8 : 6.8 per (2 : 2 : 1) blocks at K = 1536, 20.8 : 25 : 15.5 at 12464
 // rows and K = 3072, 30 : 31 : 15.2 at 1280 rows, where the clock is not held down. Pairs of 256, 192 and 128 columns, us per
@@ -184,100 +181,6 @@ __device__ __forceinline__ void tile_coords(const GemmItem& p, int tile, int& m_
   const int rows = min(p.group_m, p.m_tiles - m0);
   n_t = r / rows;
   m_t = m0 + (r - n_t * rows);
-}
-
-__device__ __forceinline__ void tma_load_2d(void* smem_dst, const void* tmap, uint64_t* bar, int c0, int c1) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-      :
-      : "r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(smem_u32(bar)), "r"(c0), "r"(c1)
-      : "memory");
-}
-
-// ---- CTA-pair helpers ------------------------------------------------------------------------------------
-// Tiled load into this CTA's shared memory that completes on a barrier of either CTA of the pair
-// (`bar_cluster_addr` is a shared::cluster address).
-__device__ __forceinline__ void tma_load_2d_pair(void* smem_dst, const void* tmap, uint32_t bar_cluster_addr, int c0,
-                                                 int c1) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], "
-      "[%2];"
-      :
-      : "r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar_cluster_addr), "r"(c0), "r"(c1)
-      : "memory");
-}
-__device__ __forceinline__ uint32_t cluster_ctarank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync_all() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// shared::cluster address of `p` (an address in this CTA's shared memory) as seen in CTA `rank` of the cluster
-__device__ __forceinline__ uint32_t map_to_cta(const void* p, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
-  return r;
-}
-// What the arrival orders is tensor-memory traffic (tcgen05.fence on both sides), not generic-proxy data, so the
-// default semantics suffice; a cluster-scope acquire on the waiting side cost ~500 cycles per wait when measured.
-__device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
-}
-__device__ __forceinline__ void tmem_alloc_pair(uint32_t* smem_slot, uint32_t ncols) {
-  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(smem_slot)),
-               "r"(ncols)
-               : "memory");
-}
-__device__ __forceinline__ void tmem_relinquish_pair() {
-  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {
-  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
-}
-// D[tmem of both CTAs] (+)= A[smem of each CTA] * B[smem halves of both CTAs]; issued by the even CTA only
-__device__ __forceinline__ void umma_ss_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                             uint32_t accumulate) {
-  asm volatile(
-      "{\n\t"
-      ".reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t"
-      "}"
-      :
-      : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-// Arrive on the barrier at `bar`'s offset in both CTAs of the pair once every MMA issued so far is done.
-__device__ __forceinline__ void tc_commit_pair(uint64_t* bar) {
-  asm volatile(
-      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
-          smem_u32(bar)),
-      "h"(static_cast<uint16_t>(3))
-      : "memory");
-}
-
-template <bool FP16>
-__device__ __forceinline__ float to_f(uint16_t v) {
-  if constexpr (FP16) return __half2float(__ushort_as_half(v));
-  else return __bfloat162float(__ushort_as_bfloat16(v));
-}
-template <bool FP16>
-__device__ __forceinline__ uint16_t from_f(float f) {
-  if constexpr (FP16) return __half_as_ushort(__float2half_rn(f));
-  else return __bfloat16_as_ushort(__float2bfloat16_rn(f));
-}
-template <bool FP16>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  return static_cast<uint32_t>(from_f<FP16>(lo)) | (static_cast<uint32_t>(from_f<FP16>(hi)) << 16);
-}
-
-__device__ __forceinline__ float gelu_tanh_f(float x) {
-  const float u = 0.7978845608028654f * fmaf(0.044715f * x, x * x, x);
-  float t;
-  asm("tanh.approx.f32 %0, %1;" : "=f"(t) : "f"(u));
-  return 0.5f * x * (1.0f + t);
 }
 
 // {mean, 1 / deviation} of this thread's row over the head whose accumulator columns start at `taddr`, from the values
@@ -731,23 +634,6 @@ __global__ void __launch_bounds__(GemmCfg<BM, BN, PAIR>::kThreads, 1)
 }
 
 // ------------------------------------------------------------------ host side
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* ptr = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(ptr);
-  });
-  return fn;
-}
-
 // Descriptor over a (rows, K) matrix with K contiguous; box = 64 elements x box_rows rows.
 int encode_matrix(CUtensorMap* map, const void* ptr, long long rows, long long k, long long ld, int box_rows,
                   int dtype) {
@@ -765,18 +651,6 @@ int encode_matrix(CUtensorMap* map, const void* ptr, long long rows, long long k
     return set_error(HDIT_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d (rows=%lld k=%lld ld=%lld)",
                      static_cast<int>(r), rows, k, ld);
   return HDIT_OK;
-}
-
-int sm_count() {
-  static int counts[64] = {0};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
-  if (counts[dev] == 0) {
-    int n = 0;
-    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
-    counts[dev] = n;
-  }
-  return counts[dev];
 }
 
 template <int BM, int BN, bool PAIR, bool FP16>
