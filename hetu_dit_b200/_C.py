@@ -232,6 +232,40 @@ class LnItem(ctypes.Structure):
     ]
 
 
+class Int8LinearArgs(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("epilogue", ctypes.c_int32),
+        ("m", ctypes.c_int64),
+        ("n", ctypes.c_int64),
+        ("k", ctypes.c_int64),
+        ("a", ctypes.c_void_p),
+        ("lda", ctypes.c_int64),
+        ("a_scale", ctypes.c_void_p),
+        ("x", ctypes.c_void_p),
+        ("x_rows_per_batch", ctypes.c_int64),
+        ("x_batch_stride", ctypes.c_int64),
+        ("x_row_stride", ctypes.c_int64),
+        ("w", ctypes.c_void_p),
+        ("ldw", ctypes.c_int64),
+        ("w_scale", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("ldo", ctypes.c_int64),
+        ("residual", ctypes.c_void_p),
+        ("ldr", ctypes.c_int64),
+        ("gate", ctypes.c_void_p),
+        ("gate_batch_stride", ctypes.c_int64),
+        ("rows_per_batch", ctypes.c_int64),
+        ("stream", ctypes.c_void_p),
+        ("tile", ctypes.c_int32),
+        ("max_ctas", ctypes.c_int32),
+    ]
+
+
+INT8_MAX_K = 131072
+ACT_NONE, ACT_SILU = 0, 1
+
 _lib = None
 _lock = threading.Lock()
 
@@ -274,6 +308,21 @@ def _declare(lib):
     lib.hdit_linear_fused.argtypes = [ctypes.POINTER(GemmArgs)]
     lib.hdit_linear_group.restype = ctypes.c_int
     lib.hdit_linear_group.argtypes = [ctypes.POINTER(LinearGroupArgs)]
+    lib.hdit_quantize_rows.restype = ctypes.c_int
+    lib.hdit_quantize_rows.argtypes = [ctypes.c_int32] + [ctypes.c_void_p] * 3 + [ctypes.c_int64] * 6 + [ctypes.c_void_p]
+    lib.hdit_ln_modulate_int8.restype = ctypes.c_int
+    lib.hdit_ln_modulate_int8.argtypes = [ctypes.c_int32] + [ctypes.c_void_p] * 5 + [ctypes.c_int64] * 7 + [
+        ctypes.c_float, ctypes.c_void_p]
+    lib.hdit_int8_linear.restype = ctypes.c_int
+    lib.hdit_int8_linear.argtypes = [ctypes.POINTER(Int8LinearArgs)]
+    lib.hdit_group_norm_scratch.restype = ctypes.c_int64
+    lib.hdit_group_norm_scratch.argtypes = [ctypes.c_int64] * 4
+    lib.hdit_group_norm.restype = ctypes.c_int
+    lib.hdit_group_norm.argtypes = [ctypes.c_int32] + [ctypes.c_void_p] * 5 + [ctypes.c_int64] * 8 + [
+        ctypes.c_float, ctypes.c_int32, ctypes.c_void_p]
+    lib.hdit_group_norm_int8.restype = ctypes.c_int
+    lib.hdit_group_norm_int8.argtypes = [ctypes.c_int32] + [ctypes.c_void_p] * 6 + [ctypes.c_int64] * 7 + [
+        ctypes.c_float, ctypes.c_int32, ctypes.c_void_p]
     lib.hdit_heap_alloc.restype = ctypes.c_int
     lib.hdit_heap_alloc.argtypes = [ctypes.c_int64, ctypes.POINTER(ctypes.c_void_p)]
     lib.hdit_heap_free.restype = ctypes.c_int

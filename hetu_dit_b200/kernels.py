@@ -927,3 +927,246 @@ def cfg_euler_step(noise_pred, sample, sigmas, step_index, guidance_scale, cfg=T
                                               _stream_ptr(sample.device)))
     _count()
     return out
+
+
+class Int8Rows:
+    """Rows of 16-bit values held in 8 bits: row r stands for q[r] * scale[r]. q: (..., K) int8, K contiguous, rows on 16-byte
+    boundaries (quantize_rows() lays them out so); scale: (...) fp32, contiguous; dtype: the 16-bit type of what they stand
+    for, and of what a layer computes from them. A linear layer's weight (N, K) has a row per output channel."""
+    __slots__ = ("q", "scale", "dtype")
+
+    def __init__(self, q, scale, dtype=torch.bfloat16):
+        self.q, self.scale, self.dtype = q, scale, dtype
+
+    shape = property(lambda self: self.q.shape)
+    device = property(lambda self: self.q.device)
+    is_cuda = property(lambda self: self.q.is_cuda)
+
+    def dequantize(self):
+        """The values as a tensor of `dtype`."""
+        return (self.q.float() * self.scale[..., None]).to(self.dtype)
+
+
+def _empty_int8_rows(lead, k, device, dtype):
+    pitch = (k + 15) & ~15
+    q = torch.empty((*lead, pitch), dtype=torch.int8, device=device)
+    return Int8Rows(q if pitch == k else q[..., :k], torch.empty(lead, dtype=torch.float32, device=device), dtype)
+
+
+def quantize_rows(x):
+    """Rows of x, (B, S, K) or (rows, K), in 8 bits with a scale each: scale = max|row| / 127, q = row / scale to the nearest
+    integer, ties to even. Any K and strides with contiguous K. A row with an infinity or NaN gets a NaN scale (what is
+    computed from it is NaN), one below 2^-100 throughout counts as zero."""
+    _require_cuda(x)
+    if x.dtype not in _DTYPE_CODE:
+        raise TypeError(f"unsupported dtype {x.dtype}")
+    if x.dim() not in (2, 3) or x.shape[-1] == 0 or (x.stride(-1) != 1 and x.shape[-1] != 1):
+        raise ValueError("expected (B, S, K) or (rows, K) with contiguous K")
+    lead, k = x.shape[:-1], x.shape[-1]
+    out = _empty_int8_rows(lead, k, x.device, x.dtype)
+    rows = out.scale.numel()
+    if rows == 0:
+        return out
+    sb = x.stride(0) if x.dim() == 3 else 0
+    with _on(x.device):
+        _C.check(_C.lib().hdit_quantize_rows(_DTYPE_CODE[x.dtype], x.data_ptr(), out.q.data_ptr(), out.scale.data_ptr(), rows, k,
+                                             lead[-1], sb, x.stride(-2), out.q.stride(-2), _stream_ptr(x.device)))
+    _count()
+    return out
+
+
+def ln_modulate_int8(x, shift, scale, eps=1e-6):
+    """ln_modulate() with its rows in 8 bits, see quantize_rows(); nothing is rounded to 16 bits in between. x (B, S, Dm) with
+    contiguous Dm, a multiple of 8 and at most 8192; shift / scale (B, Dm) views."""
+    _require_cuda(x)
+    if x.dtype not in _DTYPE_CODE or shift.dtype != x.dtype or scale.dtype != x.dtype:
+        raise TypeError("x, shift and scale must be of one 16-bit type")
+    if x.dim() != 3 or x.stride(2) != 1:
+        raise ValueError("expected a (B, S, Dm) tensor with contiguous last dim")
+    B, S, dim = x.shape
+    if shift.shape != (B, dim) or scale.shape != (B, dim) or shift.stride(1) != 1 or scale.stride(1) != 1 or \
+            (B > 1 and shift.stride(0) != scale.stride(0)):
+        raise ValueError("shift / scale must be (B, Dm) views with contiguous last dim and equal batch stride")
+    if shift.device != x.device or scale.device != x.device:
+        raise ValueError("x, shift and scale must be on one device")
+    out = _empty_int8_rows((B, S), dim, x.device, x.dtype)
+    with _on(x.device):
+        _C.check(_C.lib().hdit_ln_modulate_int8(_DTYPE_CODE[x.dtype], x.data_ptr(), shift.data_ptr(), scale.data_ptr(),
+                                                out.q.data_ptr(), out.scale.data_ptr(), B * S, dim, max(S, 1), x.stride(0),
+                                                x.stride(1), out.q.stride(1), shift.stride(0), eps, _stream_ptr(x.device)))
+    if B * S:
+        _count()
+    return out
+
+
+_TAILS = {"bias": _C.GEMM_BIAS, "gelu_tanh": _C.GEMM_BIAS_GELU_TANH, "gate_residual": _C.GEMM_BIAS_GATE_RESIDUAL}
+
+
+def linear_int8(x, weight, bias=None, epilogue="bias", residual=None, gate=None, out=None, tile=0, max_ctas=0):
+    """epilogue(x @ weight.T + bias) over 8-bit integers on the tensor cores (csrc/int8_linear_sm100.cu). x: Int8Rows, or a
+    16-bit tensor whose rows are taken as quantize_rows() gives them; (B, S, K) or (rows, K). weight: Int8Rows (N, K).
+    epilogue "bias", "gelu_tanh" or "gate_residual" = residual + gate[:, None, :] * linear(x), gate (B, N), as in
+    linear_fused(). The sums are exact integers; scales, bias and epilogue run in fp32 and the result is rounded to x's
+    16-bit type once. B, S, K, N need not be multiples of anything. `out` may be a column block of a wider buffer, or
+    `residual` itself."""
+    held = type(x) is Int8Rows
+    rows_of = x.q if held else x
+    _require_cuda(rows_of)
+    dtype, dev = x.dtype, rows_of.device
+    if dtype not in _DTYPE_CODE:
+        raise TypeError(f"unsupported dtype {dtype}")
+    if epilogue not in _TAILS:
+        raise ValueError(f"unknown epilogue {epilogue}")
+    if type(weight) is not Int8Rows:
+        raise TypeError("weight must be Int8Rows, as quantize_rows() makes them")
+    if rows_of.dim() == 2:
+        x3 = Int8Rows(x.q[None], x.scale[None], dtype) if held else x[None]
+        return linear_int8(x3, weight, bias, epilogue, None if residual is None else residual[None], gate,
+                           None if out is None else out[None], tile, max_ctas)[0]
+    w, w_scale = weight.q, weight.scale
+    if rows_of.dim() != 3 or w.dim() != 2:
+        raise ValueError("x must be (B, S, K) or (rows, K), weight (N, K)")
+    (B, S, k), (n, kw) = rows_of.shape, w.shape
+    if k != kw or k == 0 or n == 0 or w.dtype != torch.int8 or w_scale.dtype != torch.float32 or w_scale.shape != (n,) or \
+            not w_scale.is_contiguous() or w.device != dev or w_scale.device != dev:
+        raise ValueError("weight must be (N, K) int8 with N contiguous fp32 scales, on x's device")
+    if (w.stride(1) != 1 and k != 1) or (w.stride(0) % 16 and n != 1) or w.data_ptr() % 16:
+        raise ValueError("weight rows must be contiguous and start on 16-byte boundaries, as quantize_rows() lays them out")
+    if held:
+        if x.q.dtype != torch.int8 or x.scale.dtype != torch.float32 or x.scale.shape != (B, S) or x.scale.device != dev:
+            raise ValueError("x must be int8 with a fp32 scale for each row, on one device")
+        if (x.q.stride(2) != 1 and k != 1) or (x.q.stride(1) % 16 and S != 1) or (x.q.stride(0) % 16 and B != 1) or x.q.data_ptr() % 16:
+            raise ValueError("x's rows must be contiguous and start on 16-byte boundaries, as quantize_rows() lays them out")
+    elif x.stride(2) != 1 and k != 1:
+        raise ValueError("x must have contiguous K")
+    if bias is not None and (bias.numel() != n or not bias.is_contiguous() or bias.dtype != dtype or bias.device != dev):
+        raise ValueError("bias must be N contiguous elements of x's dtype, on its device")
+    gated = epilogue == "gate_residual"
+    if gated:
+        if residual is None or gate is None:
+            raise ValueError("the gate_residual epilogue needs residual and gate")
+        if residual.shape != (B, S, n) or residual.dtype != dtype or residual.device != dev or (residual.stride(2) != 1 and n != 1):
+            raise ValueError("residual does not match (B, S, N), x's dtype or its device")
+        if gate.shape != (B, n) or (gate.stride(1) != 1 and n != 1) or gate.dtype != dtype or gate.device != dev:
+            raise ValueError("gate must be (B, N) of x's dtype, on its device")
+    if out is None:
+        out = torch.empty((B, S, n), dtype=dtype, device=dev)
+    elif out.shape != (B, S, n) or out.dtype != dtype or out.device != dev or (out.stride(2) != 1 and n != 1):
+        raise ValueError("out does not match (B, S, N), x's dtype or its device")
+    if B > 1 and not (_even_rows(out) and (not gated or _even_rows(residual)) and
+                      (not held or (_even_rows(x.q) and x.scale.is_contiguous()))):
+        for b in range(B):  # a slice of the rows of every entry: one launch per entry
+            xb = Int8Rows(x.q[b:b + 1], x.scale[b:b + 1], dtype) if held else x[b:b + 1]
+            linear_int8(xb, weight, bias, epilogue, residual[b:b + 1] if gated else None, gate[b:b + 1] if gated else None,
+                        out[b:b + 1], tile, max_ctas)
+        return out
+    m = B * S
+    if m == 0:
+        return out
+    a = _C.Int8LinearArgs()
+    a.dtype, a.epilogue, a.m, a.n, a.k = _DTYPE_CODE[dtype], _TAILS[epilogue], m, n, k
+    if held:
+        q, scale = x.q, x.scale if x.scale.is_contiguous() else x.scale.contiguous()
+    else:
+        own = _empty_int8_rows((B, S), k, dev, dtype)
+        q, scale = own.q, own.scale
+        a.x, a.x_rows_per_batch, a.x_batch_stride, a.x_row_stride = x.data_ptr(), S, x.stride(0), x.stride(1)
+    a.a, a.a_scale, a.lda = q.data_ptr(), scale.data_ptr(), q.stride(1) if S > 1 or not held else (k + 15) & ~15
+    a.w, a.ldw, a.w_scale = w.data_ptr(), w.stride(0) if n > 1 else (k + 15) & ~15, w_scale.data_ptr()
+    if bias is not None:
+        a.bias = bias.data_ptr()
+    a.out, a.ldo = out.data_ptr(), out.stride(1) if m > 1 else n
+    if gated:
+        a.residual, a.ldr = residual.data_ptr(), residual.stride(1) if m > 1 else n
+        a.gate, a.gate_batch_stride, a.rows_per_batch = gate.data_ptr(), gate.stride(0), S
+    a.tile, a.max_ctas = tile, max_ctas
+    with _on(dev):
+        a.stream = _stream_ptr(dev)
+        _C.check(_C.lib().hdit_int8_linear(ctypes.byref(a)))
+    _count(1 if held else 2)
+    return out
+
+
+def _image_rows(x):
+    """A channels-last image as (batch, rows, channels, batch stride, row stride): (B, S, C), or (B, C, H, W) / (B, C, T, H, W)
+    with the channels contiguous and the pixels evenly strided."""
+    if x.dim() not in (3, 4, 5):
+        raise ValueError("expected (B, S, C), or (B, C, H, W) or (B, C, T, H, W) in channels-last layout")
+    v = x if x.dim() == 3 else x.movedim(1, -1)
+    B, C = v.shape[0], v.shape[-1]
+    rows, stride = 1, None
+    for n, s in zip(reversed(v.shape[1:-1]), reversed(v.stride()[1:-1])):
+        if n != 1 and stride is None:
+            rows, stride = n, s
+        elif n != 1 and s == rows * stride:
+            rows *= n
+        elif n != 1:
+            raise ValueError("pixels must be evenly strided (channels-last layout)")
+    if C != 1 and v.stride(-1) != 1:
+        raise ValueError("channels must be contiguous (channels-last layout)")
+    if x.numel() == 0:
+        rows = 0
+    return B, rows, C, v.stride(0) if B > 1 else 0, C if stride is None else stride
+
+
+_ACTS = {None: _C.ACT_NONE, "silu": _C.ACT_SILU}
+
+
+@functools.lru_cache(maxsize=1024)
+def _group_norm_scratch(batch, rows, channels, groups):
+    return _C.lib().hdit_group_norm_scratch(batch, rows, channels, groups)
+
+
+def _group_norm_args(x, groups, weight, bias, act):
+    _require_cuda(x)
+    if x.dtype not in _DTYPE_CODE:
+        raise TypeError(f"unsupported dtype {x.dtype}")
+    if act not in _ACTS:
+        raise ValueError(f"unknown activation {act}")
+    B, rows, C, sb, sr = _image_rows(x)
+    groups = int(groups)
+    if groups < 1 or C % groups:
+        raise ValueError("channels must be a multiple of groups")
+    for t in (weight, bias):
+        if t is not None and (t.dtype != x.dtype or t.shape != (C,) or not t.is_contiguous() or t.device != x.device):
+            raise ValueError("weight / bias must be C contiguous elements of x's dtype, on its device")
+    return B, rows, C, sb, sr, groups
+
+
+def group_norm(x, groups, weight=None, bias=None, eps=1e-6, act=None, out=None):
+    """GroupNorm over a channels-last image, then `act` (None or "silu"), one rounding. x: (B, C, H, W) or (B, C, T, H, W) in
+    torch's channels_last / channels_last_3d layout (channels contiguous, pixels evenly strided), or (B, S, C); C a multiple of
+    8 and of `groups`, at most 4096. weight, bias: (C,) or None. Returns a tensor of x's shape in the same layout; `out` may be
+    x."""
+    B, rows, C, sb, sr, groups = _group_norm_args(x, groups, weight, bias, act)
+    if out is None:
+        out = torch.empty_like(x) if x.dim() == 3 else \
+            torch.empty((B, *x.shape[2:], C), dtype=x.dtype, device=x.device).movedim(-1, 1)
+    if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
+        raise ValueError("out does not match x")
+    _, _, _, osb, osr = _image_rows(out)
+    scratch = torch.empty(_group_norm_scratch(B, rows, C, groups), dtype=torch.uint8, device=x.device)
+    with _on(x.device):
+        _C.check(_C.lib().hdit_group_norm(_DTYPE_CODE[x.dtype], x.data_ptr(), weight.data_ptr() if weight is not None else None,
+                                          bias.data_ptr() if bias is not None else None, out.data_ptr(), scratch.data_ptr(), B,
+                                          rows, C, groups, sb, sr, osb, osr, eps, _ACTS[act], _stream_ptr(x.device)))
+    if B * rows:
+        _count(2)
+    return out
+
+
+def group_norm_int8(x, groups, weight=None, bias=None, eps=1e-6, act=None):
+    """group_norm() with its rows (all channels of a pixel) in 8 bits, see quantize_rows(); nothing is rounded to 16 bits in
+    between. Returns Int8Rows (B, pixels, C), what linear_int8() takes."""
+    B, rows, C, sb, sr, groups = _group_norm_args(x, groups, weight, bias, act)
+    out = _empty_int8_rows((B, rows), C, x.device, x.dtype)
+    scratch = torch.empty(_group_norm_scratch(B, rows, C, groups), dtype=torch.uint8, device=x.device)
+    with _on(x.device):
+        _C.check(_C.lib().hdit_group_norm_int8(_DTYPE_CODE[x.dtype], x.data_ptr(),
+                                               weight.data_ptr() if weight is not None else None,
+                                               bias.data_ptr() if bias is not None else None, out.q.data_ptr(),
+                                               out.scale.data_ptr(), scratch.data_ptr(), B, rows, C, groups, sb, sr,
+                                               out.q.stride(1), eps, _ACTS[act], _stream_ptr(x.device)))
+    if B * rows:
+        _count(2)
+    return out

@@ -533,6 +533,91 @@ typedef struct hdit_linear_group_args {
 
 HDIT_API int hdit_linear_group(const hdit_linear_group_args* args);
 
+/*
+ * 8-bit rows: a row y of values as signed integers q with one fp32 scale s,
+ *   s = max|y| / 127,   q = y / s to the nearest integer, ties to even (so |q| <= 127 and y = q s up to half a step).
+ * A row whose largest magnitude is below 2^-100 counts as zero (s = 0, q = 0). A row that holds an infinity or NaN gets s = NaN and
+ * q = 0: what is computed from it is NaN. Memory: rows of `dim` bytes, 16-byte aligned, their stride a multiple of 16; bytes
+ * behind a row's end are neither read nor written. (The reference has no 8-bit path.)
+ *
+ * hdit_quantize_rows    : y = x, 16-bit storage. q is exact for these inputs, borders between two integers included. Row r of x
+ *                         starts at (r / rows_per_batch) * x_batch_stride + (r % rows_per_batch) * x_row_stride elements; any
+ *                         strides and row length (16-byte aligned rows are read 16 bytes at a time). The same call lays out a
+ *                         linear layer's weight (n, k), one scale per output channel.
+ * hdit_ln_modulate_int8 : y = LayerNorm(x) * (1 + scale[b]) + shift[b] in fp32, as hdit_ln_modulate but for the rounding to 16
+ *                         bits; dim a multiple of 8, at most 8192; b = r / rows_per_batch.
+ */
+HDIT_API int hdit_quantize_rows(int32_t dtype, const void* x, void* q, float* scale, int64_t rows, int64_t dim,
+                                int64_t rows_per_batch, int64_t x_batch_stride, int64_t x_row_stride, int64_t q_row_stride,
+                                void* stream);
+HDIT_API int hdit_ln_modulate_int8(int32_t dtype, const void* x, const void* shift, const void* scale, void* q, float* q_scale,
+                                   int64_t rows, int64_t dim, int64_t rows_per_batch, int64_t x_batch_stride,
+                                   int64_t x_row_stride, int64_t q_row_stride, int64_t mod_batch_stride, float eps, void* stream);
+
+/*
+ * Linear layer over 8-bit rows: out[r, c] = tail(a_scale[r] * w_scale[c] * sum_k a[r, k] w[c, k] + bias[c]) with the tails of
+ * hdit_linear_fused. The sum is exact (32-bit integers, k at most HDIT_INT8_MAX_K); scales, bias and tail run in fp32 and the
+ * result is rounded to 16 bits once (hdit_linear_fused rounds before the tail, too).
+ * a (m, k) and w (n, k) are 8-bit rows as above, a_scale and w_scale m and n contiguous floats. x != NULL: a and a_scale are
+ * scratch that hdit_quantize_rows fills from these 16-bit rows first (x_rows_per_batch, x_batch_stride, x_row_stride as there).
+ * bias, gate, residual and out are 16-bit of `dtype`, any strides that keep rows of residual and out apart; m, n and k need not
+ * be multiples of anything; rows_per_batch >= 1 (HDIT_GEMM_BIAS_GATE_RESIDUAL only). `out` may alias `residual`.
+ * tile: 0 = the library chooses, 1 = 128 x 128 tiles, 2, 3, 4 = 256 x 128, 256 x 192, 256 x 256 on a CTA pair. max_ctas: 0 = one
+ * persistent CTA per SM.
+ */
+#define HDIT_INT8_MAX_K 131072 /* 127 * 127 * k < 2^31 */
+
+typedef struct hdit_int8_linear_args {
+  int32_t dtype;
+  int32_t epilogue; /* HDIT_GEMM_BIAS, _GELU_TANH, _GATE_RESIDUAL */
+  int64_t m, n, k;
+  const void* a;
+  int64_t lda;
+  const float* a_scale;
+  const void* x;
+  int64_t x_rows_per_batch, x_batch_stride, x_row_stride;
+  const void* w;
+  int64_t ldw;
+  const float* w_scale;
+  const void* bias;
+  void* out;
+  int64_t ldo;
+  const void* residual;
+  int64_t ldr;
+  const void* gate;
+  int64_t gate_batch_stride;
+  int64_t rows_per_batch;
+  void* stream;
+  int32_t tile;
+  int32_t max_ctas;
+} hdit_int8_linear_args;
+
+HDIT_API int hdit_int8_linear(const hdit_int8_linear_args* args);
+
+/*
+ * GroupNorm over channels-last images, then an activation:
+ *   out[b, r, c] = act((x[b, r, c] - mean[b, g]) / sqrt(var[b, g] + eps) * weight[c] + bias[c]),  g = c / (channels / groups)
+ * with mean and biased variance over the rows r (pixels) and channels of group g, fp32 arithmetic, 16-bit storage. x and out are
+ * (batch, rows, channels) with contiguous channels, any batch and row strides (elements); channels a multiple of 8 and of
+ * groups, at most 4096; weight and bias `channels` elements each or NULL (1 and 0). scratch: hdit_group_norm_scratch() bytes,
+ * 8-byte aligned, of which nothing has to be kept before or after the call; calls that may overlap need one each. `out` may be x.
+ * hdit_group_norm_int8 writes each row (all channels of a pixel) as an 8-bit row instead, rows of all images in order.
+ *
+ * The reference takes the norm of its image decoder from diffusers and shards it over ranks
+ * (hetu_dit/model_executor/vae_executor/models/layers/normalization.py:52-188), NCHW.
+ */
+enum { HDIT_ACT_NONE = 0, HDIT_ACT_SILU = 1 };
+
+HDIT_API int64_t hdit_group_norm_scratch(int64_t batch, int64_t rows, int64_t channels, int64_t groups);
+HDIT_API int hdit_group_norm(int32_t dtype, const void* x, const void* weight, const void* bias, void* out, void* scratch,
+                             int64_t batch, int64_t rows, int64_t channels, int64_t groups, int64_t x_batch_stride,
+                             int64_t x_row_stride, int64_t out_batch_stride, int64_t out_row_stride, float eps, int32_t act,
+                             void* stream);
+HDIT_API int hdit_group_norm_int8(int32_t dtype, const void* x, const void* weight, const void* bias, void* q, float* q_scale,
+                                  void* scratch, int64_t batch, int64_t rows, int64_t channels, int64_t groups,
+                                  int64_t x_batch_stride, int64_t x_row_stride, int64_t q_row_stride, float eps, int32_t act,
+                                  void* stream);
+
 #ifdef __cplusplus
 }
 #endif

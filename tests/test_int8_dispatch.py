@@ -1,0 +1,141 @@
+"""CPU tests of what the wrappers of the 8-bit rows and the group norm refuse before a launch, and of what the library
+refuses by itself. Nothing is launched."""
+import ctypes
+
+import pytest
+import torch
+
+from hetu_dit_b200 import _C, kernels
+from tests.test_host_dispatch import OnGpu, gpu_like, lib  # noqa: F401
+
+
+def rows8(*shape, dtype=torch.bfloat16):
+    q = torch.zeros(*shape, dtype=torch.int8)
+    pitch = -(-shape[-1] // 16) * 16
+    q = torch.zeros(*shape[:-1], pitch, dtype=torch.int8)[..., :shape[-1]].as_subclass(OnGpu)
+    return kernels.Int8Rows(q, torch.ones(shape[:-1]).as_subclass(OnGpu), dtype)
+
+
+def test_host_tensors_are_refused(lib):  # noqa: F811
+    x, w = torch.randn(1, 4, 32).bfloat16(), rows8(16, 32)
+    for call in (lambda: kernels.quantize_rows(x), lambda: kernels.ln_modulate_int8(x, x[:, 0], x[:, 0]),
+                 lambda: kernels.linear_int8(x, w), lambda: kernels.group_norm(x, 4), lambda: kernels.group_norm_int8(x, 4)):
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            call()
+    assert lib.calls == []
+
+
+def _linear(**change):
+    a = dict(x=gpu_like(2, 40, 32), weight=rows8(24, 32), bias=gpu_like(24), epilogue="gate_residual", residual=gpu_like(2, 40, 24),
+             gate=gpu_like(2, 24), out=gpu_like(2, 40, 24))
+    a.update(change)
+    return kernels.linear_int8(a.pop("x"), a.pop("weight"), a.pop("bias"), a.pop("epilogue"), **a)
+
+
+BAD_LINEAR = {
+    "type of x": dict(x=gpu_like(2, 40, 32, dtype=torch.float32)),
+    "weight in 16 bits": dict(weight=gpu_like(24, 32)),
+    "inner sizes": dict(x=gpu_like(2, 40, 48)),
+    "epilogue": dict(epilogue="silu"),
+    "bias size": dict(bias=gpu_like(23)),
+    "bias type": dict(bias=gpu_like(24, dtype=torch.float16)),
+    "no residual": dict(residual=None),
+    "no gate": dict(gate=None),
+    "residual shape": dict(residual=gpu_like(2, 40, 25)),
+    "residual type": dict(residual=gpu_like(2, 40, 24, dtype=torch.float16)),
+    "gate shape": dict(gate=gpu_like(1, 24)),
+    "out shape": dict(out=gpu_like(2, 41, 24)),
+    "out type": dict(out=gpu_like(2, 40, 24, dtype=torch.float16)),
+    "x columns": dict(x=gpu_like(2, 40, 64)[..., ::2]),
+    "weight scale type": dict(weight=kernels.Int8Rows(rows8(24, 32).q, torch.ones(24).half().as_subclass(OnGpu))),
+    "weight scale count": dict(weight=kernels.Int8Rows(rows8(24, 32).q, torch.ones(23).as_subclass(OnGpu))),
+    "weight rows": dict(weight=kernels.Int8Rows(torch.zeros(24, 40, dtype=torch.int8).as_subclass(OnGpu)[:, :32],
+                                                torch.ones(24).as_subclass(OnGpu))),
+    "x rows": dict(x=kernels.Int8Rows(torch.zeros(2, 40, 40, dtype=torch.int8).as_subclass(OnGpu)[..., :32],
+                                      torch.ones(2, 40).as_subclass(OnGpu))),
+    "x scale": dict(x=kernels.Int8Rows(rows8(2, 40, 32).q, torch.ones(2, 41).as_subclass(OnGpu))),
+    "dimensions": dict(x=gpu_like(2, 2, 40, 32)),
+    "another device": dict(bias=torch.empty(24, dtype=torch.bfloat16, device="meta")),
+}
+
+
+@pytest.mark.parametrize("what", BAD_LINEAR)
+def test_linear_int8_refuses(lib, what):  # noqa: F811
+    with pytest.raises((ValueError, TypeError)):
+        _linear(**BAD_LINEAR[what])
+    assert lib.calls == []
+
+
+def test_linear_int8_takes_what_it_documents(lib, monkeypatch):  # noqa: F811
+    monkeypatch.setattr(kernels, "_cuda_index", lambda device: 0)
+    _linear()
+    _linear(x=rows8(2, 40, 32))
+    assert [c[0] for c in lib.calls] == ["hdit_int8_linear"] * 2
+    first, second = (c[1][0]._obj for c in lib.calls)
+    assert (first.m, first.n, first.k, first.rows_per_batch) == (80, 24, 32, 40)
+    assert first.x and not second.x
+    assert _linear(x=gpu_like(2, 0, 32), residual=gpu_like(2, 0, 24), out=gpu_like(2, 0, 24)).shape == (2, 0, 24)
+    assert len(lib.calls) == 2
+    # rows that are a slice of every entry's: a launch for each
+    _linear(out=gpu_like(2, 50, 24)[:, 3:43])
+    assert len(lib.calls) == 4
+
+
+def test_rows_and_norms_refuse(lib):  # noqa: F811
+    x = gpu_like(2, 40, 64)
+    for bad in (gpu_like(64), x[..., ::2], x[..., :0]):
+        with pytest.raises(ValueError):
+            kernels.quantize_rows(bad)
+    with pytest.raises(TypeError):
+        kernels.quantize_rows(x.float())
+    for sh, sc in ((gpu_like(1, 64), gpu_like(1, 64)), (gpu_like(2, 64), gpu_like(2, 128)[:, :64]), (gpu_like(2, 128)[:, ::2],) * 2):
+        with pytest.raises(ValueError):
+            kernels.ln_modulate_int8(x, sh, sc)
+    with pytest.raises(TypeError):
+        kernels.ln_modulate_int8(x, gpu_like(2, 64, dtype=torch.float16), gpu_like(2, 64))
+    image = gpu_like(2, 6, 10, 64).permute(0, 3, 1, 2)
+    for bad in (gpu_like(2, 64, 6, 10), image[..., ::2], image[:, ::2], gpu_like(60, 64)):
+        with pytest.raises(ValueError):
+            kernels.group_norm(bad, 8)
+        with pytest.raises(ValueError):
+            kernels.group_norm_int8(bad, 8)
+    for kw in (dict(groups=7), dict(groups=0), dict(groups=8, act="gelu"), dict(groups=8, weight=gpu_like(63)),
+               dict(groups=8, bias=gpu_like(64, dtype=torch.float16)), dict(groups=8, out=gpu_like(2, 64, 6, 10)),
+               dict(groups=8, out=gpu_like(2, 64, 6, 11))):
+        with pytest.raises(ValueError):
+            kernels.group_norm(image, **kw)
+    assert [c for c in lib.calls if c[0] != "hdit_group_norm_scratch"] == []
+
+
+def test_the_library_refuses_by_itself():
+    real = _C.lib()
+    q, s = ctypes.c_void_p(4096), ctypes.c_void_p(4096)  # addresses that nothing reads
+    none = ctypes.c_void_p(0)
+    rows = lambda **k: real.hdit_quantize_rows(*{**dict(dtype=0, x=q, q=q, s=s, rows=4, dim=32, rpb=4, xb=0, xr=32, qr=32, st=none), **k}.values())  # noqa: E731
+    for bad in (dict(dtype=2), dict(rows=-1), dict(dim=0), dict(rpb=0), dict(x=none), dict(q=none), dict(s=none), dict(qr=24), dict(qr=16),
+                dict(q=ctypes.c_void_p(4104)), dict(x=ctypes.c_void_p(4097)), dict(s=ctypes.c_void_p(4098)), dict(dim=1 << 31)):
+        assert rows(**bad) in (_C.HDIT_ERR_BAD_ARG, _C.HDIT_ERR_SHAPE, _C.HDIT_ERR_TOO_LARGE), bad
+    assert rows(rows=0) == 0
+    ln = lambda **k: real.hdit_ln_modulate_int8(*{**dict(dtype=0, x=q, sh=q, sc=q, q=q, s=s, rows=4, dim=32, rpb=4, xb=0, xr=32, qr=32, mb=32, eps=1e-6, st=none), **k}.values())  # noqa: E731
+    for bad in (dict(dim=20), dict(dim=8200, qr=8208), dict(sh=none), dict(sc=ctypes.c_void_p(4097))):
+        assert ln(**bad) in (_C.HDIT_ERR_BAD_ARG, _C.HDIT_ERR_SHAPE), bad
+    gn = lambda **k: real.hdit_group_norm(*{**dict(dtype=0, x=q, w=none, b=none, out=q, scratch=q, batch=1, rows=4, c=64, g=8, xb=0, xr=64, ob=0, orow=64, eps=1e-6, act=0, st=none), **k}.values())  # noqa: E731
+    for bad in (dict(dtype=2), dict(batch=-1), dict(c=60), dict(g=7), dict(g=0), dict(c=4104), dict(act=2), dict(x=none), dict(scratch=none),
+                dict(batch=65536), dict(rows=1 << 31)):
+        assert gn(**bad) in (_C.HDIT_ERR_BAD_ARG, _C.HDIT_ERR_SHAPE, _C.HDIT_ERR_TOO_LARGE), bad
+    assert gn(batch=0) == 0 and gn(rows=0) == 0
+
+    def linear(**change):
+        a = _C.Int8LinearArgs()
+        fields = dict(dtype=0, epilogue=2, m=8, n=24, k=32, a=4096, lda=32, a_scale=4096, w=4096, ldw=32, w_scale=4096, bias=4096, out=4096,
+                      ldo=24, residual=4096, ldr=24, gate=4096, gate_batch_stride=24, rows_per_batch=4)
+        for name, v in {**fields, **change}.items():
+            setattr(a, name, v)
+        return real.hdit_int8_linear(ctypes.byref(a))
+
+    for bad in (dict(dtype=2), dict(epilogue=3), dict(m=-1), dict(n=0), dict(k=0), dict(k=131073), dict(m=1 << 31), dict(a=0), dict(w=0), dict(out=0),
+                dict(a_scale=0), dict(w_scale=0), dict(lda=24), dict(ldw=16), dict(a=4104), dict(w=4104), dict(ldo=20), dict(ldr=20), dict(residual=0),
+                dict(gate=0), dict(rows_per_batch=0), dict(out=4097), dict(a_scale=4098), dict(residual=4097)):
+        assert linear(**bad) in (_C.HDIT_ERR_BAD_ARG, _C.HDIT_ERR_SHAPE, _C.HDIT_ERR_TOO_LARGE), bad
+    assert linear(m=0) == 0
+    assert real.hdit_int8_linear(None) == _C.HDIT_ERR_BAD_ARG
