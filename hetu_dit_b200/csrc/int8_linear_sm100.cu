@@ -7,10 +7,9 @@
 // MMAs of 32 -- so operand bytes per clock are the same and the main loop of a tile takes half the time for the same K; the
 // epilogue has half the time to hide behind it.
 //
-//   epilogue     per 32 x 64 piece of a warp: scales and bias of the warp's columns wait in shared memory since before
-//                the accumulator was ready (a lane would else wait for the same 64 values from global memory one after
-//                the other); the residual's piece is brought in by full 128-byte lines through the staging buffer and the
-//                result leaves through it the same way, in place.
+//   epilogue     per 32 x 64 piece of a warp, a lane to a row: scales, bias and gate of the warp's columns wait in shared
+//                memory (they are fetched while the tile before is worked on), the residual's piece comes into the staging
+//                buffer by TMA one piece ahead, the result takes its place there and leaves by TMA. Two staging buffers.
 //
 // All waits are bounded, see gemm_sm100.cu.
 #include <math.h>
@@ -28,6 +27,7 @@ enum Int8Wait : int {
   Q_MMA_FULL = 212,
   Q_MMA_ACC_EMPTY = 213,
   Q_EPI_ACC_FULL = 214,
+  Q_EPI_RESIDUAL = 215,
 };
 
 // Instruction descriptor for kind::i8: signed operands, both K-major, 32-bit integer accumulators, no saturation.
@@ -58,9 +58,26 @@ __device__ __forceinline__ void umma_i8_pair(uint32_t d_tmem, uint64_t a_desc, u
       : "memory");
 }
 
-struct Int8Params {
+// ---- results leave shared memory by TMA
+__device__ __forceinline__ void tma_store_2d(const void* tmap, const void* smem_src, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];"
+               :
+               : "l"(reinterpret_cast<uint64_t>(tmap)), "r"(smem_u32(smem_src)), "r"(c0), "r"(c1)
+               : "memory");
+}
+__device__ __forceinline__ void tma_store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+// All but the last N stores of this thread have read their shared memory.
+template <int N>
+__device__ __forceinline__ void tma_store_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void tma_store_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
+struct alignas(64) Int8Params {
   CUtensorMap a_map;
   CUtensorMap w_map;
+  CUtensorMap out_map;  // boxes of 64 columns x 32 rows, where tma_out / tma_residual say so
+  CUtensorMap residual_map;
   int M, N, k_blocks;
   int m_tiles, n_tiles, group_m;
   const float* a_scale;
@@ -73,11 +90,11 @@ struct Int8Params {
   const uint16_t* gate;
   long long gate_batch_stride;
   int rows_per_batch;
-  bool vec;  // rows of out and residual are whole 16-byte chunks
+  bool tma_out, tma_residual;  // rows start on 16-byte boundaries
   int32_t* status;
 };
 
-template <int BN, bool PAIR>
+template <int BN, bool PAIR, int EPI>
 struct Int8Cfg {
   // Four warps reach the 128 lanes of an accumulator; a second team takes the other half of the columns
   static constexpr int kPieces = BN / 64;
@@ -90,14 +107,21 @@ struct Int8Cfg {
   static constexpr int kABytes = 128 * kTileKBytes;
   static constexpr int kBBytes = kBRows * kTileKBytes;
   static constexpr int kStageBytes = kABytes + kBBytes;
-  static constexpr int kStagingBytes = kEpiWarps * 4096;  // 32 rows x 64 columns of 16 bits per epilogue warp
-  static constexpr int kColBytes = kEpiWarps * kTeamPieces * 64 * 12;  // scale, bias, gate of a warp's columns, fp32
-  static constexpr int kBarBytes = 256;
-  static constexpr int kStagesFit = (kMaxSmem - 1024 - kBarBytes - kStagingBytes - kColBytes) / kStageBytes;
+  // pieces of 32 rows x 64 columns of 16 bits per epilogue warp: two where a residual comes in beside the result that leaves.
+  // One more costs a stage of the ring, which 256 columns miss more: 4608 x 12288 x 3072 + GELU takes 137 us with 4 stages and
+  // two buffers, 124 with 6 and one.
+  static constexpr int kBufs = EPI == HDIT_GEMM_BIAS_GATE_RESIDUAL ? 2 : 1;
+  static constexpr int kStagingBytes = kEpiWarps * kBufs * 4096;
+  // barriers and the columns' scales, bias and gate: what is left of 227 KB beside six stages of 32 KB and one piece per warp
+  static constexpr int kSmallBytes = 3072;
+  static constexpr int kStagesFit = (kMaxSmem - kSmallBytes - kStagingBytes) / kStageBytes;
   static constexpr int kStages = kStagesFit > 8 ? 8 : kStagesFit;
   static constexpr int kAccCols = BN == 192 ? 256 : BN;
   static constexpr int kTmemCols = 2 * kAccCols;
-  static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kStagingBytes + kColBytes + kBarBytes;
+  static constexpr int kSmemBytes = kSmallBytes + kStages * kStageBytes + kStagingBytes;
+  static constexpr int kTeamCols = kTeamPieces * 64;  // at most one for each of the team's 128 threads
+  static_assert(512 + kColTeams * kTeamCols * 10 <= kSmallBytes, "no room for the columns");
+  static_assert(kStageBytes % 1024 == 0, "TMA tiles start at multiples of the swizzle's 1024 bytes");
   static_assert(kStages >= 3, "ring too short");
   static_assert(kTmemCols == 128 || kTmemCols == 256 || kTmemCols == 512, "TMEM allocation must be a power of two");
 };
@@ -113,20 +137,21 @@ __device__ __forceinline__ void int8_tile_coords(const Int8Params& p, int tile, 
 }
 
 template <int BN, bool PAIR, bool FP16, int EPI>
-__global__ void __launch_bounds__(Int8Cfg<BN, PAIR>::kThreads, 1) int8_linear_kernel(const __grid_constant__ Int8Params p) {
-  using C = Int8Cfg<BN, PAIR>;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* stage_base = smem;
-  uint8_t* staging_base = smem + C::kStages * C::kStageBytes;
-  float* col_base = reinterpret_cast<float*>(staging_base + C::kStagingBytes);
-  uint64_t* full = reinterpret_cast<uint64_t*>(staging_base + C::kStagingBytes + C::kColBytes);
+__global__ void __launch_bounds__(Int8Cfg<BN, PAIR, EPI>::kThreads, 1) int8_linear_kernel(const __grid_constant__ Int8Params p) {
+  using C = Int8Cfg<BN, PAIR, EPI>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem);
   uint64_t* empty = full + 8;
   uint64_t* acc_full = empty + 8;
   uint64_t* acc_empty = acc_full + 2;
   uint64_t* drain_bar = acc_empty + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain_bar + 1);
+  uint64_t* res_bars = drain_bar + 1;  // two for each epilogue warp
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(res_bars + 2 * C::kEpiWarps);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  static_assert((8 + 8 + 2 + 2 + 1 + 2 * C::kEpiWarps + 1) * 8 <= 512, "barriers");
+  uint8_t* col_base = smem + 512;
+  uint8_t* stage_base = smem + C::kSmallBytes;
+  uint8_t* staging_base = stage_base + C::kStages * C::kStageBytes;
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -148,6 +173,7 @@ __global__ void __launch_bounds__(Int8Cfg<BN, PAIR>::kThreads, 1) int8_linear_ke
       mbar_init(&acc_empty[i], PAIR ? 2 * C::kEpiWarps : C::kEpiWarps);
     }
     mbar_init(drain_bar, 1);
+    for (int i = 0; i < 2 * C::kEpiWarps; ++i) mbar_init(&res_bars[i], 1);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -261,87 +287,131 @@ __global__ void __launch_bounds__(Int8Cfg<BN, PAIR>::kThreads, 1) int8_linear_ke
     }
   } else {
     // ------------------------------------------------------------------ epilogue
+    constexpr bool kGated = EPI == HDIT_GEMM_BIAS_GATE_RESIDUAL;
     const int quarter = warp & 3;  // the TMEM lanes this warp may read: [32 * quarter, 32 * quarter + 32)
     const int team = (warp - 2) >> 2;
     const int c0 = team * C::kTeamPieces, c1 = min(C::kPieces, c0 + C::kTeamPieces);
-    uint8_t* staging = staging_base + (warp - 2) * 4096;
-    float* col_scale = col_base + (warp - 2) * (C::kTeamPieces * 64 * 3);
-    float* col_bias = col_scale + C::kTeamPieces * 64;
-    float* col_gate = col_bias + C::kTeamPieces * 64;
-    const int sub_row = lane >> 3, chunk = lane & 7;  // full lines: 4 rows per instruction, 8 lanes per row
-    uint32_t local = 0;
-    for (int tile = unit; tile < total_tiles; tile += n_units, ++local) {
+    uint8_t* const staging = staging_base + (warp - 2) * (C::kBufs * 4096);
+    uint64_t* const res_full = res_bars + (warp - 2) * 2;
+    const int t_col = (threadIdx.x - 64) & 127;  // the column of its team that this thread fetches
+    float* const col_scale = reinterpret_cast<float*>(col_base + team * (C::kTeamCols * 10));
+    float* const col_bias = col_scale + C::kTeamCols;
+    uint16_t* const col_gate = reinterpret_cast<uint16_t*>(col_bias + C::kTeamCols);
+    auto team_sync = [&] { asm volatile("bar.sync %0, 128;" ::"r"(1 + team) : "memory"); };
+
+    // what the tile needs beside its sums; fetched one tile ahead
+    long long row0 = 0;     // first row of the warp
+    int tile_col = 0;       // first column of the team
+    bool one_batch = true;  // all rows of the team have one batch entry: its gate waits in shared memory, else each row reads its own
+    float row_scale = 0.f, f_scale = 0.f;
+    uint16_t f_bias = 0, f_gate = 0;
+    auto fetch = [&](int tile) {
       int m_t, n_t;
       int8_tile_coords(p, tile, m_t, n_t);
-      const uint32_t acc = local & 1, use = local >> 1;
-      const long long row0 = static_cast<long long>(m_t) * C::kTileRows + static_cast<long long>(rank) * 128 + quarter * 32;
-      const long long my_row = row0 + lane;
-      const int tile_col = n_t * BN + c0 * 64;  // first column of this warp
-      // one batch entry for all rows of the warp: its gate waits beside the scales; else each row reads its own
-      long long batch = 0;
-      bool one_batch = true;
-      if constexpr (EPI == HDIT_GEMM_BIAS_GATE_RESIDUAL) {
-        const unsigned first = static_cast<unsigned>(row0 < p.M ? row0 : 0), last = static_cast<unsigned>(row0 + 31 < p.M ? row0 + 31 : p.M - 1);
-        const unsigned b_first = first / static_cast<unsigned>(p.rows_per_batch);
-        one_batch = first > last || b_first == last / static_cast<unsigned>(p.rows_per_batch);
-        batch = one_batch ? b_first : (my_row < p.M ? static_cast<unsigned>(my_row) / static_cast<unsigned>(p.rows_per_batch) : b_first);
+      const long long team_row0 = static_cast<long long>(m_t) * C::kTileRows + static_cast<long long>(rank) * 128;
+      row0 = team_row0 + quarter * 32;
+      tile_col = n_t * BN + c0 * 64;
+      unsigned batch = 0;
+      if constexpr (kGated) {
+        const unsigned first = static_cast<unsigned>(team_row0 < p.M ? team_row0 : 0);
+        const unsigned last = static_cast<unsigned>(team_row0 + 127 < p.M ? team_row0 + 127 : p.M - 1);
+        const unsigned per = static_cast<unsigned>(p.rows_per_batch);
+        batch = first / per;
+        one_batch = first > last || batch == last / per;
       }
-      const float row_scale = my_row < p.M ? p.a_scale[my_row] : 0.f;
-      __syncwarp();  // everyone is done with the previous tile's columns
-      for (int i = lane; i < C::kTeamPieces * 64; i += 32) {
-        const int col = tile_col + i;
+      row_scale = row0 + lane < p.M ? p.a_scale[row0 + lane] : 0.f;
+      const int col = tile_col + t_col;
+      if (t_col < C::kTeamCols) {
         const bool in = col < p.N;
-        col_scale[i] = in ? p.w_scale[col] : 0.f;
-        col_bias[i] = in && p.bias != nullptr ? to_f<FP16>(p.bias[col]) : 0.f;
-        if constexpr (EPI == HDIT_GEMM_BIAS_GATE_RESIDUAL)
-          if (one_batch) col_gate[i] = in ? to_f<FP16>(p.gate[batch * p.gate_batch_stride + col]) : 0.f;
+        f_scale = in ? p.w_scale[col] : 0.f;
+        f_bias = in && p.bias != nullptr ? p.bias[col] : uint16_t(0);
+        if constexpr (kGated) f_gate = in && one_batch ? p.gate[static_cast<long long>(batch) * p.gate_batch_stride + col] : uint16_t(0);
       }
-      __syncwarp();
-      bool waited = false;
-      bool ok = true;
+    };
+    // pieces are numbered through all tiles; piece i has staging buffer i % kBufs
+    uint32_t piece = 0, res_phase = 0, res_pending = 0;
+    auto issue_residual = [&](long long row, int col, uint32_t buf) {
+      if (lane == 0 && row < p.M && col < p.N) {
+        mbar_expect_tx(&res_full[buf], 4096);
+        tma_load_2d(staging + buf * 4096, &p.residual_map, &res_full[buf], col, static_cast<int>(row));
+      }
+      if (row < p.M && col < p.N) res_pending |= 1u << buf;
+    };
+    uint32_t local = 0;
+    bool ok = true;
+    if (unit < total_tiles) {
+      fetch(unit);
+      if constexpr (kGated)
+        if (p.tma_residual) issue_residual(row0, tile_col, 0);
+    }
+    for (int tile = unit; tile < total_tiles; tile += n_units, ++local) {
+      const uint32_t acc = local & 1, use = local >> 1;
+      const long long my_row0 = row0;
+      const int my_col = tile_col;
+      const bool my_one_batch = one_batch;
+      const float my_scale = row_scale;
+      team_sync();  // everyone is done with the previous tile's columns
+      if (t_col < C::kTeamCols) {
+        col_scale[t_col] = f_scale;
+        col_bias[t_col] = to_f<FP16>(f_bias);
+        if constexpr (kGated) col_gate[t_col] = f_gate;
+      }
+      team_sync();
+      if (!ok) continue;  // after a failure: the team's other warps still meet the barriers
+      if (tile + n_units < total_tiles) fetch(tile + n_units);
+      if (!__all_sync(0xffffffffu, mbar_wait_bounded(&acc_full[acc], use & 1, abort_flag, kSpinLimit))) {
+        if (lane == 0) report_failure(p.status, abort_flag, HDIT_ERR_PEER_TIMEOUT, Q_EPI_ACC_FULL, static_cast<int>(local));
+        ok = false;
+        continue;
+      }
+      tc_fence_after();
 #pragma unroll 1
-      for (int c = c0; c < c1; ++c) {
-        const int col0 = n_t * BN + c * 64;
-        const int col = col0 + chunk * 8;
-        const int at = (c - c0) * 64;
-        if constexpr (EPI == HDIT_GEMM_BIAS_GATE_RESIDUAL) {
-          // the residual's 32 x 64 values to the staging buffer (16-byte chunk j of row r sits at chunk j ^ (r & 7))
-          uint4 xv[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const long long row = row0 + i * 4 + sub_row;
-            xv[i] = make_uint4(0, 0, 0, 0);
-            if (row < p.M && col < p.N) {
-              const uint16_t* src = p.residual + row * p.ldr + col;
-              if (p.vec) {
-                xv[i] = *reinterpret_cast<const uint4*>(src);
-              } else {
-                uint16_t* e = reinterpret_cast<uint16_t*>(&xv[i]);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) e[k] = col + k < p.N ? src[k] : uint16_t(0);
-              }
-            }
-          }
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int rl = i * 4 + sub_row;
-            *reinterpret_cast<uint4*>(staging + rl * 128 + ((chunk ^ (rl & 7)) << 4)) = xv[i];
-          }
-          __syncwarp();
-        }
-        if (!waited) {
-          waited = true;
-          if (!__all_sync(0xffffffffu, mbar_wait_bounded(&acc_full[acc], use & 1, abort_flag, kSpinLimit))) {
-            if (lane == 0) report_failure(p.status, abort_flag, HDIT_ERR_PEER_TIMEOUT, Q_EPI_ACC_FULL, static_cast<int>(local));
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-        }
+      for (int c = c0; c < c1; ++c, ++piece) {
+        const uint32_t buf = C::kBufs == 1 ? 0 : piece & 1;
+        uint8_t* const stage = staging + buf * 4096;
+        const int at = (c - c0) * 64, col0 = my_col + at;
+        const bool in = my_row0 < p.M && col0 < p.N;
         const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + acc * C::kAccCols + c * 64;
         uint32_t r[64];
         tmem_ld32(taddr, *reinterpret_cast<uint32_t(*)[32]>(&r[0]));
         tmem_ld32(taddr + 32, *reinterpret_cast<uint32_t(*)[32]>(&r[32]));
+        if constexpr (kGated) {
+          if (p.tma_residual) {
+            // the next piece's residual, into the buffer that the previous piece's result has left
+            if (!p.tma_out) fence_proxy_async_smem();  // it left by plain loads
+            if (lane == 0) tma_store_wait_read<0>();
+            __syncwarp();
+            if (c + 1 < c1) issue_residual(my_row0, col0 + 64, buf ^ 1);
+            else if (tile + n_units < total_tiles) issue_residual(row0, tile_col, buf ^ 1);
+            if (in) {
+              if (!__all_sync(0xffffffffu, mbar_wait_bounded(&res_full[buf], (res_phase >> buf) & 1, abort_flag, kSpinLimit))) {
+                if (lane == 0) report_failure(p.status, abort_flag, HDIT_ERR_PEER_TIMEOUT, Q_EPI_RESIDUAL, static_cast<int>(piece));
+                ok = false;
+                break;
+              }
+              res_phase ^= 1u << buf;
+              res_pending &= ~(1u << buf);
+            }
+          } else {
+            if (lane == 0) tma_store_wait_read<1>();
+            __syncwarp();
+            // 16-byte chunk j of row r sits at chunk j ^ (r & 7), as TMA lays it out
+            for (int i = 0; i < 32 && in; ++i) {
+              const long long row = my_row0 + i;
+              if (row >= p.M) break;
+#pragma unroll
+              for (int h = 0; h < 64; h += 32) {
+                const int k = h + lane;
+                if (col0 + k < p.N)
+                  *reinterpret_cast<uint16_t*>(stage + i * 128 + (((k >> 3) ^ (i & 7)) << 4) + (k & 7) * 2) = p.residual[row * p.ldr + col0 + k];
+              }
+            }
+            __syncwarp();
+          }
+        } else {
+          if (lane == 0) tma_store_wait_read<C::kBufs - 1>();  // the buffer's last result has left
+          __syncwarp();
+        }
         tc_wait_ld();
         if (c == c1 - 1) {
           // the accumulator is in registers: hand it back to the MMA warp
@@ -352,64 +422,91 @@ __global__ void __launch_bounds__(Int8Cfg<BN, PAIR>::kThreads, 1) int8_linear_ke
             else mbar_arrive(&acc_empty[acc]);
           }
         }
-        // row `lane`: scale, bias, tail, one rounding
+        // Row `lane`: scale, bias, tail, one rounding. What eight columns need is read before the eight ones before are
+        // written: the compiler cannot tell that the two do not overlap, and two warps per scheduler hide little of a chain of
+        // reads and writes.
+        uint8_t* const own = stage + lane * 128;
+        float4 s4[2], b4[2];
+        uint4 x4, g8;
+        auto read = [&](int j) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            s4[h] = *reinterpret_cast<const float4*>(col_scale + at + j * 8 + h * 4);
+            b4[h] = *reinterpret_cast<const float4*>(col_bias + at + j * 8 + h * 4);
+          }
+          if constexpr (kGated) {
+            g8 = *reinterpret_cast<const uint4*>(col_gate + at + j * 8);
+            x4 = *reinterpret_cast<const uint4*>(own + ((j ^ (lane & 7)) << 4));
+          }
+        };
+        read(0);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           float v[8];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float4 s4 = *reinterpret_cast<const float4*>(col_scale + at + j * 8 + h * 4);
-            const float4 b4 = *reinterpret_cast<const float4*>(col_bias + at + j * 8 + h * 4);
             const uint32_t* a4 = &r[j * 8 + h * 4];
-            v[h * 4 + 0] = fmaf(static_cast<float>(static_cast<int>(a4[0])) * row_scale, s4.x, b4.x);
-            v[h * 4 + 1] = fmaf(static_cast<float>(static_cast<int>(a4[1])) * row_scale, s4.y, b4.y);
-            v[h * 4 + 2] = fmaf(static_cast<float>(static_cast<int>(a4[2])) * row_scale, s4.z, b4.z);
-            v[h * 4 + 3] = fmaf(static_cast<float>(static_cast<int>(a4[3])) * row_scale, s4.w, b4.w);
+            v[h * 4 + 0] = fmaf(static_cast<float>(static_cast<int>(a4[0])) * my_scale, s4[h].x, b4[h].x);
+            v[h * 4 + 1] = fmaf(static_cast<float>(static_cast<int>(a4[1])) * my_scale, s4[h].y, b4[h].y);
+            v[h * 4 + 2] = fmaf(static_cast<float>(static_cast<int>(a4[2])) * my_scale, s4[h].z, b4[h].z);
+            v[h * 4 + 3] = fmaf(static_cast<float>(static_cast<int>(a4[3])) * my_scale, s4[h].w, b4[h].w);
           }
-          uint4* place = reinterpret_cast<uint4*>(staging + lane * 128 + ((j ^ (lane & 7)) << 4));
           if constexpr (EPI == HDIT_GEMM_BIAS_GELU_TANH) {
 #pragma unroll
             for (int k = 0; k < 8; ++k) v[k] = gelu_tanh_f(v[k]);
-          } else if constexpr (EPI == HDIT_GEMM_BIAS_GATE_RESIDUAL) {
-            const uint4 x4 = *place;
+          } else if constexpr (kGated) {
             const uint16_t* xe = reinterpret_cast<const uint16_t*>(&x4);
-            if (one_batch) {
+            const uint16_t* ge = reinterpret_cast<const uint16_t*>(&g8);
+            float g[8];
 #pragma unroll
-              for (int k = 0; k < 8; ++k) v[k] = fmaf(col_gate[at + j * 8 + k], v[k], to_f<FP16>(xe[k]));
-            } else {
+            for (int k = 0; k < 8; ++k) g[k] = to_f<FP16>(ge[k]);
+            if (!my_one_batch) {
+              const long long row = my_row0 + lane;
+              const uint16_t* gr = p.gate + (row < p.M ? static_cast<unsigned>(row) / static_cast<unsigned>(p.rows_per_batch) : 0u) * p.gate_batch_stride;
 #pragma unroll
               for (int k = 0; k < 8; ++k) {
                 const int gc = col0 + j * 8 + k;
-                const float g = gc < p.N ? to_f<FP16>(p.gate[batch * p.gate_batch_stride + gc]) : 0.f;
-                v[k] = fmaf(g, v[k], to_f<FP16>(xe[k]));
+                g[k] = gc < p.N ? to_f<FP16>(gr[gc]) : 0.f;
               }
             }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = fmaf(g[k], v[k], to_f<FP16>(xe[k]));
           }
-          *place = make_uint4(pack2<FP16>(v[0], v[1]), pack2<FP16>(v[2], v[3]), pack2<FP16>(v[4], v[5]), pack2<FP16>(v[6], v[7]));
+          if (j < 7) read(j + 1);
+          *reinterpret_cast<uint4*>(own + ((j ^ (lane & 7)) << 4)) =
+              make_uint4(pack2<FP16>(v[0], v[1]), pack2<FP16>(v[2], v[3]), pack2<FP16>(v[4], v[5]), pack2<FP16>(v[6], v[7]));
         }
-        __syncwarp();
-        if (col < p.N) {
+        if (p.tma_out) {
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            if (in) tma_store_2d(&p.out_map, stage, col0, static_cast<int>(my_row0));
+            tma_store_commit();
+          }
+        } else {
+          __syncwarp();
+          for (int i = 0; i < 32 && in; ++i) {
+            const long long row = my_row0 + i;
+            if (row >= p.M) break;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int rl = i * 4 + sub_row;
-            const long long row = row0 + rl;
-            if (row >= p.M) continue;
-            const uint4 v = *reinterpret_cast<const uint4*>(staging + rl * 128 + ((chunk ^ (rl & 7)) << 4));
-            uint16_t* dst = p.out + row * p.ldo + col;
-            if (p.vec) {
-              *reinterpret_cast<uint4*>(dst) = v;
-            } else {
-              const uint16_t* e = reinterpret_cast<const uint16_t*>(&v);
-#pragma unroll
-              for (int k = 0; k < 8; ++k)
-                if (col + k < p.N) dst[k] = e[k];
+            for (int h = 0; h < 64; h += 32) {
+              const int k = h + lane;
+              if (col0 + k < p.N)
+                p.out[row * p.ldo + col0 + k] = *reinterpret_cast<const uint16_t*>(stage + i * 128 + (((k >> 3) ^ (i & 7)) << 4) + (k & 7) * 2);
             }
           }
+          __syncwarp();
         }
-        __syncwarp();  // the staging buffer is overwritten by the next piece
       }
-      if (!ok) break;
     }
+    // copies in flight must have left or landed before the CTA's shared memory is given back
+    if (lane == 0) tma_store_wait_all();
+    if constexpr (kGated) {
+      volatile int never = 0;
+      for (uint32_t buf = 0; buf < 2; ++buf)
+        if ((res_pending >> buf) & 1) mbar_wait_bounded(&res_full[buf], (res_phase >> buf) & 1, &never, kSpinLimit);
+    }
+    __syncwarp();
   }
 
   tc_fence_before();
@@ -438,9 +535,25 @@ int encode_bytes(CUtensorMap* map, const void* ptr, long long rows, long long k,
   return HDIT_OK;
 }
 
+// Map of a (rows, n) matrix of 16-bit values for the epilogue's pieces.
+int encode_pieces(CUtensorMap* map, const void* ptr, long long rows, long long n, long long ld, int dtype) {
+  EncodeTiledFn enc = encode_fn();
+  if (enc == nullptr) return set_error(HDIT_ERR_CUDA, "cuTensorMapEncodeTiled entry point unavailable");
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(n), static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * 2};
+  cuuint32_t box[2] = {64, 32};
+  cuuint32_t estr[2] = {1, 1};
+  const CUtensorMapDataType dt = dtype == HDIT_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const CUresult r = enc(map, dt, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return set_error(HDIT_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d (rows=%lld n=%lld ld=%lld)", static_cast<int>(r), rows, n, ld);
+  return HDIT_OK;
+}
+
 template <int BN, bool PAIR, bool FP16, int EPI>
 int launch_int8(Int8Params& p, const hdit_int8_linear_args* a) {
-  using C = Int8Cfg<BN, PAIR>;
+  using C = Int8Cfg<BN, PAIR, EPI>;
   auto kernel = int8_linear_kernel<BN, PAIR, FP16, EPI>;
   static thread_local int last_dev = -1;  // the attribute is per device
   int dev = 0;
@@ -453,6 +566,8 @@ int launch_int8(Int8Params& p, const hdit_int8_linear_args* a) {
   if (rc != HDIT_OK) return rc;
   rc = encode_bytes(&p.w_map, a->w, a->n, a->k, a->ldw, C::kBRows);
   if (rc != HDIT_OK) return rc;
+  if (p.tma_out && (rc = encode_pieces(&p.out_map, a->out, a->m, a->n, a->ldo, a->dtype)) != HDIT_OK) return rc;
+  if (p.tma_residual && (rc = encode_pieces(&p.residual_map, a->residual, a->m, a->n, a->ldr, a->dtype)) != HDIT_OK) return rc;
   const long long ctas = a->max_ctas > 0 ? a->max_ctas : sm_count();
   const long long m_tiles = (a->m + C::kTileRows - 1) / C::kTileRows, n_tiles = (a->n + BN - 1) / BN;
   if (m_tiles * n_tiles > 0x7fffffffLL) return set_error(HDIT_ERR_TOO_LARGE, "more than 2^31 output tiles");
@@ -522,7 +637,8 @@ extern "C" int hdit_int8_linear(const hdit_int8_linear_args* a) {
   p.gate_batch_stride = a->gate_batch_stride;
   p.rows_per_batch = static_cast<int>(a->rows_per_batch > 0 && a->rows_per_batch < a->m ? a->rows_per_batch : a->m);
   auto whole = [&](const void* ptr, long long ld) { return (reinterpret_cast<uintptr_t>(ptr) & 15) == 0 && ld % 8 == 0; };
-  p.vec = a->n % 8 == 0 && whole(a->out, a->ldo) && (!gated || whole(a->residual, a->ldr));
+  p.tma_out = whole(a->out, a->ldo);
+  p.tma_residual = gated && whole(a->residual, a->ldr);
   p.status = device_status_ptr();
   if (p.status == nullptr) return HDIT_ERR_CUDA;
   if (a->x != nullptr) {
