@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(kRowThreads) group_norm_int8_kernel(const __gr
   grid_dependency_release();
   grid_dependency_wait();
   extern __shared__ float smem[];  // a[channels], b[channels], then {mean, 1 / deviation}[groups]
-  __shared__ float red[kRowThreads / 32];
+  __shared__ float red[2][kRowThreads / 32];
   float* fa = smem;
   float* fb = smem + p.channels;
   float2* stat = reinterpret_cast<float2*>(smem + 2 * p.channels);
@@ -257,11 +257,12 @@ __global__ void __launch_bounds__(kRowThreads) group_norm_int8_kernel(const __gr
   const long long r0 = static_cast<long long>(blockIdx.x) * p.strip_rows;
   const long long r1 = r0 + p.strip_rows < p.rows ? r0 + p.strip_rows : p.rows;
   const uint16_t* xb = p.x + blockIdx.y * p.x_batch_stride;
-  for (long long rt = r1 - kTeams; rt > r0 - kTeams; rt -= kTeams) {
+  int turn = 0;
+  for (long long rt = r1 - kTeams; rt > r0 - kTeams; rt -= kTeams, turn ^= 1) {
     const long long r = rt + threadIdx.x / TEAM;
     const bool live = r >= r0;
     float y[NCH][8];
-    uint32_t top = 0;
+    float top = 0.f;
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
       const int c = (k * TEAM + lane) * 8;
@@ -282,25 +283,21 @@ __global__ void __launch_bounds__(kRowThreads) group_norm_int8_kernel(const __gr
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           if constexpr (SILU) y[k][i] = silu(y[k][i]);
-          const uint32_t m = __float_as_uint(y[k][i]) & 0x7FFFFFFFu;
-          top = top > m ? top : m;
+          top = max_magnitude(top, y[k][i]);
         }
       }
     }
-    const Int8Scale s = int8_scale(team.max(top));
+    const Int8Scale s = int8_scale(team.max(__float_as_uint(top) & 0x7FFFFFFFu, turn));
     if (live) {
       const long long row = blockIdx.y * p.rows + r;
 #pragma unroll
       for (int k = 0; k < NCH; ++k) {
         const int c = (k * TEAM + lane) * 8;
         if (c < p.channels) {
-          float t[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) t[i] = s.inv == 0.f ? 0.f : y[k][i] * s.inv;
-          int8_store8(p.q + row * p.out_row_stride, c, p.channels, make_uint2(int8_pack4(t[0], t[1], t[2], t[3]), int8_pack4(t[4], t[5], t[6], t[7])));
+          int8_put8_of(p.q + row * p.out_row_stride, c, s, y[k]);
         }
       }
-      if (lane == 0) p.q_scale[row] = s.scale;
+      if (lane == 0) p.q_scale[row] = int8_step(s);
     }
   }
 }

@@ -21,196 +21,230 @@ struct RowsParams {
   const uint16_t* scale;
   int8_t* q;
   float* q_scale;
-  long long rows, rows_per_batch, x_batch_stride, x_row_stride, q_row_stride, mod_batch_stride;
+  long long batches, rows_per_batch, x_batch_stride, x_row_stride, q_row_stride, mod_batch_stride;
   int dim;
   float eps;
-  bool vec;  // 16-byte loads of x (and of shift, scale) are aligned
+  bool mod_vec;  // shift and scale of a batch entry start on 16-byte boundaries
 };
 
-// TEAM threads hold a row of at most TEAM * NCH * 8 elements. Rows are taken in the same order by all teams of a CTA, so
-// that a team without a row still meets the others' barriers.
-template <bool FP16, int TEAM, int NCH, bool LN>
-__global__ void __launch_bounds__(kRowThreads) int8_rows_kernel(const __grid_constant__ RowsParams p) {
+// CTAs that are to fit an SM beside one another
+constexpr int rows_ctas(int nch, bool ln) { return ln ? (nch <= 2 ? 4 : nch <= 4 ? 3 : 2) : nch <= 4 ? 4 : 2; }
+
+// TEAM threads hold a row of at most TEAM * NCH * 8 elements as the 16-bit values that were read, and have the next row on its
+// way while they work on one. What a row costs beside its elements (reductions, divisions, addresses) is paid by every warp of
+// the team, so a thread has up to 32 elements: with eight a thread 8192 x 1536 with the norm took 28 us, with a warp to a row, 128
+// registers and no row ahead 20, in this form 11. Modulation vectors wait in shared memory as fp32 (1 + scale, shift); a CTA stays with
+// one batch entry at a time.
+template <bool FP16, int TEAM, int NCH, bool LN, bool VEC>
+__global__ void __launch_bounds__(kRowThreads, rows_ctas(NCH, LN)) int8_rows_kernel(const __grid_constant__ RowsParams p) {
   grid_dependency_release();
   grid_dependency_wait();
-  __shared__ float red[kRowThreads / 32];
+  // 1 + scale, then shift: first the lower four columns of every chunk, then the upper four, so that the lanes' 16 bytes lie
+  // side by side
+  extern __shared__ float4 mods[];
+  __shared__ float red[3][kRowThreads / 32];
   const Team<TEAM> team{red};
   constexpr int kTeams = kRowThreads / TEAM;
-  const int lane = threadIdx.x % TEAM;
-  const long long step = static_cast<long long>(gridDim.x) * kTeams;
-  for (long long row0 = static_cast<long long>(blockIdx.x) * kTeams; row0 < p.rows; row0 += step) {
-    const long long row = row0 + threadIdx.x / TEAM;
-    const bool live = row < p.rows;
-    const long long b = live ? row / p.rows_per_batch : 0;
-    const uint16_t* xr = p.x + (live ? b * p.x_batch_stride + (row - b * p.rows_per_batch) * p.x_row_stride : 0);
-    uint4 raw[NCH];
-#pragma unroll
-    for (int c = 0; c < NCH; ++c) {
-      const int col = (c * TEAM + lane) * 8;
-      raw[c] = live && col < p.dim ? int8_load8(xr, col, p.dim, p.vec) : make_uint4(0, 0, 0, 0);
-    }
-    if constexpr (!LN) {
-      // magnitudes of two 16-bit values at a time, as integers
-      uint32_t top2 = 0;
+  const int col0 = static_cast<int>(threadIdx.x % TEAM) * 8;
+  const long long first = static_cast<long long>(blockIdx.x) * kTeams + threadIdx.x / TEAM, step = static_cast<long long>(gridDim.x) * kTeams;
+  const float inv_dim = 1.f / static_cast<float>(p.dim);
+  const int chunks = p.dim / 8;
+  for (long long b = blockIdx.y; b < p.batches; b += gridDim.y) {
+    const uint16_t* xr = p.x + b * p.x_batch_stride + first * p.x_row_stride;
+    const long long row0 = b * p.rows_per_batch;
+    uint4 next[NCH];
+    auto fetch = [&] {
 #pragma unroll
       for (int c = 0; c < NCH; ++c) {
-        const uint32_t* u = reinterpret_cast<const uint32_t*>(&raw[c]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) top2 = __vmaxu2(top2, u[i] & 0x7FFF7FFFu);
+        next[c] = make_uint4(0, 0, 0, 0);
+        if (col0 + c * TEAM * 8 < p.dim) next[c] = int8_load8(xr, col0 + c * TEAM * 8, p.dim, VEC);
       }
-      const uint32_t top16 = team.max((top2 & 0xFFFFu) > (top2 >> 16) ? top2 & 0xFFFFu : top2 >> 16);
-      const Int8Scale s = int8_scale(__float_as_uint(int8_unpack2<FP16>(top16).x));
-      if (live) {
+    };
+    if (first < p.rows_per_batch) fetch();
+    if constexpr (LN) {
+      __syncthreads();
+      for (int k = threadIdx.x; k < chunks; k += kRowThreads) {
+        const uint4 g4 = int8_load8(p.scale + b * p.mod_batch_stride, k * 8, p.dim, p.mod_vec), a4 = int8_load8(p.shift + b * p.mod_batch_stride, k * 8, p.dim, p.mod_vec);
+        const uint32_t* g = reinterpret_cast<const uint32_t*>(&g4);
+        const uint32_t* a = reinterpret_cast<const uint32_t*>(&a4);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float2 g0 = int8_unpack2<FP16>(g[2 * h]), g1 = int8_unpack2<FP16>(g[2 * h + 1]);
+          const float2 a0 = int8_unpack2<FP16>(a[2 * h]), a1 = int8_unpack2<FP16>(a[2 * h + 1]);
+          mods[h * chunks + k] = make_float4(1.f + g0.x, 1.f + g0.y, 1.f + g1.x, 1.f + g1.y);
+          mods[(2 + h) * chunks + k] = make_float4(a0.x, a0.y, a1.x, a1.y);
+        }
+      }
+      __syncthreads();
+    }
+    int turn = 0;
+    for (long long r = first; r < p.rows_per_batch; r += step, turn ^= 1) {
+      uint4 raw[NCH];
+#pragma unroll
+      for (int c = 0; c < NCH; ++c) raw[c] = next[c];
+      xr += step * p.x_row_stride;
+      if (r + step < p.rows_per_batch) fetch();
+      int8_t* const qr = p.q + (row0 + r) * p.q_row_stride;
+      Int8Scale s;
+      if constexpr (!LN) {
+        // magnitudes of two 16-bit values at a time, as integers
+        uint32_t top2 = 0;
 #pragma unroll
         for (int c = 0; c < NCH; ++c) {
-          const int col = (c * TEAM + lane) * 8;
+          const uint32_t* u = reinterpret_cast<const uint32_t*>(&raw[c]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) top2 = __vmaxu2(top2, u[i] & 0x7FFF7FFFu);
+        }
+        const uint32_t top16 = team.max((top2 & 0xFFFFu) > (top2 >> 16) ? top2 & 0xFFFFu : top2 >> 16, turn);
+        s = int8_scale(__float_as_uint(int8_unpack2<FP16>(top16).x));
+        const float inv17 = 17.f * s.inv;
+#pragma unroll
+        for (int c = 0; c < NCH; ++c) {
+          if (col0 + c * TEAM * 8 >= p.dim) continue;
           const uint32_t* u = reinterpret_cast<const uint32_t*>(&raw[c]);
           float t[8];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float2 v = int8_unpack2<FP16>(u[i]);
-            t[2 * i] = int8_steps_of_16bit(v.x, s.inv);
-            t[2 * i + 1] = int8_steps_of_16bit(v.y, s.inv);
+            t[2 * i] = int8_steps_of_16bit(v.x, s.inv, inv17);
+            t[2 * i + 1] = int8_steps_of_16bit(v.y, s.inv, inv17);
           }
-          if (s.inv == 0.f) {  // infinities and NaN times 0
-#pragma unroll
-            for (int i = 0; i < 8; ++i) t[i] = 0.f;
-          }
-          if (col < p.dim)
-            int8_store8(p.q + row * p.q_row_stride, col, p.dim, make_uint2(int8_pack4(t[0], t[1], t[2], t[3]), int8_pack4(t[4], t[5], t[6], t[7])));
+          int8_put8(qr, col0 + c * TEAM * 8, s, t);
         }
-        if (lane == 0) p.q_scale[row] = s.scale;
-      }
-    } else {
-      float sum = 0.f;
+      } else {
+        float y[NCH][8];  // x, its distance from the mean, the result
+        float sum = 0.f;
 #pragma unroll
-      for (int c = 0; c < NCH; ++c) {
-        const uint32_t* u = reinterpret_cast<const uint32_t*>(&raw[c]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 v = int8_unpack2<FP16>(u[i]);
-          sum += v.x + v.y;
-        }
-      }
-      const float mean = team.sum(sum) / static_cast<float>(p.dim);
-      float sq = 0.f;
-#pragma unroll
-      for (int c = 0; c < NCH; ++c) {
-        const uint32_t* u = reinterpret_cast<const uint32_t*>(&raw[c]);
-        if ((c * TEAM + lane) * 8 < p.dim) {  // dim is a multiple of 8
+        for (int c = 0; c < NCH; ++c) {
+          const uint32_t* u = reinterpret_cast<const uint32_t*>(&raw[c]);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float2 v = int8_unpack2<FP16>(u[i]);
-            sq = fmaf(v.x - mean, v.x - mean, sq);
-            sq = fmaf(v.y - mean, v.y - mean, sq);
+            y[c][2 * i] = v.x;
+            y[c][2 * i + 1] = v.y;
+            sum += v.x + v.y;
           }
         }
-      }
-      const float rstd = rsqrtf(team.sum(sq) / static_cast<float>(p.dim) + p.eps);
-      float y[NCH][8];
-      uint32_t top = 0;
+        const float mean = team.sum(sum, 0) * inv_dim;
+        float sq = 0.f;
 #pragma unroll
-      for (int c = 0; c < NCH; ++c) {
-        const int col = (c * TEAM + lane) * 8;
-        const uint32_t* u = reinterpret_cast<const uint32_t*>(&raw[c]);
-        if (col < p.dim) {
-          const uint4 sh4 = int8_load8(p.shift + b * p.mod_batch_stride, col, p.dim, p.vec);
-          const uint4 sc4 = int8_load8(p.scale + b * p.mod_batch_stride, col, p.dim, p.vec);
-          const uint32_t* sh = reinterpret_cast<const uint32_t*>(&sh4);
-          const uint32_t* sc = reinterpret_cast<const uint32_t*>(&sc4);
+        for (int c = 0; c < NCH; ++c)
+          if (col0 + c * TEAM * 8 < p.dim) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 v = int8_unpack2<FP16>(u[i]), h = int8_unpack2<FP16>(sh[i]), g = int8_unpack2<FP16>(sc[i]);
-            y[c][2 * i] = fmaf((v.x - mean) * rstd, 1.f + g.x, h.x);
-            y[c][2 * i + 1] = fmaf((v.y - mean) * rstd, 1.f + g.y, h.y);
+            for (int i = 0; i < 8; ++i) {
+              y[c][i] -= mean;
+              sq = fmaf(y[c][i], y[c][i], sq);
+            }
           }
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const uint32_t m = __float_as_uint(y[c][i]) & 0x7FFFFFFFu;
-            top = top > m ? top : m;
-          }
-        }
-      }
-      const Int8Scale s = int8_scale(team.max(top));
-      if (live) {
+        const float rstd = rsqrtf(team.sum(sq, 1) * inv_dim + p.eps);
+        float top = 0.f;
 #pragma unroll
         for (int c = 0; c < NCH; ++c) {
-          const int col = (c * TEAM + lane) * 8;
-          if (col < p.dim) {
-            float t[8];
+          const int col = col0 + c * TEAM * 8;
+          if (col >= p.dim) continue;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) t[i] = s.inv == 0.f ? 0.f : y[c][i] * s.inv;
-            int8_store8(p.q + row * p.q_row_stride, col, p.dim, make_uint2(int8_pack4(t[0], t[1], t[2], t[3]), int8_pack4(t[4], t[5], t[6], t[7])));
+          for (int h = 0; h < 2; ++h) {
+            const float4 g = mods[h * chunks + (col >> 3)], a = mods[(2 + h) * chunks + (col >> 3)];
+            float* v = &y[c][4 * h];
+            v[0] = fmaf(v[0] * rstd, g.x, a.x);
+            v[1] = fmaf(v[1] * rstd, g.y, a.y);
+            v[2] = fmaf(v[2] * rstd, g.z, a.z);
+            v[3] = fmaf(v[3] * rstd, g.w, a.w);
           }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) top = max_magnitude(top, y[c][i]);
         }
-        if (lane == 0) p.q_scale[row] = s.scale;
+        s = int8_scale(team.max(__float_as_uint(top) & 0x7FFFFFFFu, 2));
+#pragma unroll
+        for (int c = 0; c < NCH; ++c)
+          if (col0 + c * TEAM * 8 < p.dim) int8_put8_of(qr, col0 + c * TEAM * 8, s, y[c]);
       }
+      if (col0 == 0) p.q_scale[row0 + r] = int8_step(s);
     }
   }
 }
 
-// Rows longer than the registers of a CTA hold: read twice, the second time from the caches.
+// Rows of any length and alignment: read twice, the second time from the caches.
 template <bool FP16>
-__global__ void __launch_bounds__(kRowThreads) int8_long_rows_kernel(const __grid_constant__ RowsParams p) {
+__global__ void __launch_bounds__(kRowThreads) int8_any_rows_kernel(const __grid_constant__ RowsParams p) {
   grid_dependency_release();
   grid_dependency_wait();
-  __shared__ float red[kRowThreads / 32];
+  __shared__ float red[2][kRowThreads / 32];
   const Team<kRowThreads> team{red};
-  for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
-    const long long b = row / p.rows_per_batch;
-    const uint16_t* xr = p.x + b * p.x_batch_stride + (row - b * p.rows_per_batch) * p.x_row_stride;
-    uint32_t top2 = 0;
-    for (int col = threadIdx.x * 8; col < p.dim; col += kRowThreads * 8) {
-      const uint4 raw = int8_load8(xr, col, p.dim, p.vec);
-      const uint32_t* u = reinterpret_cast<const uint32_t*>(&raw);
+  int turn = 0;
+  for (long long b = blockIdx.y; b < p.batches; b += gridDim.y)
+    for (long long r = blockIdx.x; r < p.rows_per_batch; r += gridDim.x, turn ^= 1) {
+      const uint16_t* xr = p.x + b * p.x_batch_stride + r * p.x_row_stride;
+      const long long row = b * p.rows_per_batch + r;
+      int8_t* const qr = p.q + row * p.q_row_stride;
+      uint32_t top = 0;
+      for (int c = threadIdx.x; c < p.dim; c += kRowThreads) top = max(top, xr[c] & 0x7FFFu);
+      const Int8Scale s = int8_scale(__float_as_uint(int8_unpack2<FP16>(team.max(top, turn)).x));
+      const float inv17 = 17.f * s.inv;
+      for (int c = threadIdx.x * 4; c < p.dim; c += kRowThreads * 4) {
+        float t[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) top2 = __vmaxu2(top2, u[i] & 0x7FFF7FFFu);
-    }
-    const uint32_t top16 = team.max((top2 & 0xFFFFu) > (top2 >> 16) ? top2 & 0xFFFFu : top2 >> 16);
-    const Int8Scale s = int8_scale(__float_as_uint(int8_unpack2<FP16>(top16).x));
-    for (int col = threadIdx.x * 8; col < p.dim; col += kRowThreads * 8) {
-      const uint4 raw = int8_load8(xr, col, p.dim, p.vec);
-      const uint32_t* u = reinterpret_cast<const uint32_t*>(&raw);
-      float t[8];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 v = int8_unpack2<FP16>(u[i]);
-        t[2 * i] = s.inv == 0.f ? 0.f : int8_steps_of_16bit(v.x, s.inv);
-        t[2 * i + 1] = s.inv == 0.f ? 0.f : int8_steps_of_16bit(v.y, s.inv);
+        for (int i = 0; i < 4; ++i) t[i] = c + i < p.dim && s.inv != 0.f ? int8_steps_of_16bit(int8_unpack2<FP16>(xr[c + i]).x, s.inv, inv17) : 0.f;
+        const uint32_t v = int8_pack4(t[0], t[1], t[2], t[3]);
+        if (c + 4 <= p.dim) {
+          *reinterpret_cast<uint32_t*>(qr + c) = v;
+        } else {
+          for (int i = 0; c + i < p.dim; ++i) qr[c + i] = static_cast<int8_t>((v >> (8 * i)) & 0xFFu);
+        }
       }
-      int8_store8(p.q + row * p.q_row_stride, col, p.dim, make_uint2(int8_pack4(t[0], t[1], t[2], t[3]), int8_pack4(t[4], t[5], t[6], t[7])));
+      if (threadIdx.x == 0) p.q_scale[row] = int8_step(s);
     }
-    if (threadIdx.x == 0) p.q_scale[row] = s.scale;
-  }
 }
 
-template <bool FP16, int TEAM, int NCH, bool LN>
+// CTAs for `ctas` beside one another on every SM over all batch entries, no more than there are rows for.
+dim3 rows_grid(const RowsParams& p, long long teams, long long ctas) {
+  const long long y = p.batches < 65535 ? p.batches : 65535;
+  long long x = (148 * ctas + y - 1) / y;
+  const long long most = (p.rows_per_batch + teams - 1) / teams;
+  return dim3(static_cast<unsigned>(x < most ? x : most), static_cast<unsigned>(y));
+}
+
+template <bool FP16, int TEAM, int NCH, bool LN, bool VEC>
 cudaError_t launch_rows(const RowsParams& p, cudaStream_t st) {
-  constexpr int kTeams = kRowThreads / TEAM;
-  long long blocks = (p.rows + kTeams - 1) / kTeams;
-  if (blocks > 148LL * 8) blocks = 148LL * 8;
-  return launch_overlapped(int8_rows_kernel<FP16, TEAM, NCH, LN>, dim3(static_cast<unsigned>(blocks)), dim3(kRowThreads), 0, st, 1, p);
+  auto kernel = int8_rows_kernel<FP16, TEAM, NCH, LN, VEC>;
+  const size_t smem = LN ? static_cast<size_t>(p.dim) * 2 * sizeof(float) : 0;
+  if (smem > 47 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (e != cudaSuccess) return e;
+  }
+  return launch_overlapped(kernel, rows_grid(p, kRowThreads / TEAM, rows_ctas(NCH, LN)), dim3(kRowThreads), smem, st, 1, p);
 }
 
-template <bool FP16, bool LN>
-cudaError_t launch_any(const RowsParams& p, cudaStream_t st) {
+template <bool FP16>
+cudaError_t launch_plain(const RowsParams& p, bool vec, cudaStream_t st) {
   const int chunks = (p.dim + 7) / 8;
-  if (chunks <= 32) return launch_rows<FP16, 32, 1, LN>(p, st);
-  if (chunks <= 64) return launch_rows<FP16, 32, 2, LN>(p, st);
-  if (chunks <= 128) return launch_rows<FP16, 32, 4, LN>(p, st);
-  if (chunks <= 192) return launch_rows<FP16, 32, 6, LN>(p, st);
-  if (chunks <= 256) return launch_rows<FP16, 128, 2, LN>(p, st);
-  if (chunks <= 384) return launch_rows<FP16, 128, 3, LN>(p, st);
-  if (chunks <= 512) return launch_rows<FP16, 256, 2, LN>(p, st);
-  if (chunks <= 768) return launch_rows<FP16, 256, 3, LN>(p, st);
-  if (chunks <= 1024) return launch_rows<FP16, 256, 4, LN>(p, st);
-  if constexpr (!LN) {
-    if (chunks <= 1536) return launch_rows<FP16, 256, 6, false>(p, st);
-    if (chunks <= 2048) return launch_rows<FP16, 256, 8, false>(p, st);
-    const long long blocks = p.rows < 148LL * 8 ? p.rows : 148LL * 8;
-    return launch_overlapped(int8_long_rows_kernel<FP16>, dim3(static_cast<unsigned>(blocks)), dim3(kRowThreads), 0, st, 1, p);
-  }
-  return cudaErrorInvalidValue;
+  if (!vec || chunks > 2048) return launch_overlapped(int8_any_rows_kernel<FP16>, rows_grid(p, 1, 8), dim3(kRowThreads), 0, st, 1, p);
+  if (chunks <= 32) return launch_rows<FP16, 32, 1, false, true>(p, st);
+  if (chunks <= 64) return launch_rows<FP16, 32, 2, false, true>(p, st);
+  if (chunks <= 96) return launch_rows<FP16, 32, 3, false, true>(p, st);
+  if (chunks <= 128) return launch_rows<FP16, 32, 4, false, true>(p, st);
+  if (chunks <= 192) return launch_rows<FP16, 64, 3, false, true>(p, st);
+  if (chunks <= 256) return launch_rows<FP16, 64, 4, false, true>(p, st);
+  if (chunks <= 384) return launch_rows<FP16, 128, 3, false, true>(p, st);
+  if (chunks <= 512) return launch_rows<FP16, 128, 4, false, true>(p, st);
+  if (chunks <= 768) return launch_rows<FP16, 256, 3, false, true>(p, st);
+  if (chunks <= 1024) return launch_rows<FP16, 256, 4, false, true>(p, st);
+  return launch_rows<FP16, 256, 8, false, true>(p, st);
+}
+
+// Unaligned rows: the teams, and so the sums, of aligned ones.
+template <bool FP16, bool VEC>
+cudaError_t launch_ln(const RowsParams& p, cudaStream_t st) {
+  const int chunks = p.dim / 8;
+  if (VEC && chunks <= 32) return launch_rows<FP16, 32, 1, true, true>(p, st);
+  if (VEC && chunks <= 64) return launch_rows<FP16, 32, 2, true, true>(p, st);
+  if (VEC && chunks <= 128) return launch_rows<FP16, 32, 4, true, true>(p, st);
+  if (VEC && chunks <= 192) return launch_rows<FP16, 32, 6, true, true>(p, st);
+  if (chunks <= 256) return launch_rows<FP16, 32, 8, true, VEC>(p, st);
+  if (VEC && chunks <= 384) return launch_rows<FP16, 64, 6, true, true>(p, st);
+  if (chunks <= 512) return launch_rows<FP16, 64, 8, true, VEC>(p, st);
+  if (VEC && chunks <= 768) return launch_rows<FP16, 128, 6, true, true>(p, st);
+  return launch_rows<FP16, 128, 8, true, VEC>(p, st);
 }
 
 bool misaligned(const void* p, int64_t stride) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0 || stride % 8 != 0; }
@@ -237,10 +271,13 @@ extern "C" int hdit_quantize_rows(int32_t dtype, const void* x, void* q, float* 
   using namespace hdit;
   const int rc = check_rows(dtype, x, q, scale, rows, dim, rows_per_batch, q_row_stride);
   if (rc != HDIT_OK || rows == 0) return rc;
-  RowsParams p{static_cast<const uint16_t*>(x), nullptr, nullptr, static_cast<int8_t*>(q), scale, rows, rows_per_batch, x_batch_stride,
-               x_row_stride, q_row_stride, 0, static_cast<int>(dim), 0.f, !misaligned(x, x_row_stride) && x_batch_stride % 8 == 0};
+  const bool flat = rows <= rows_per_batch || x_batch_stride == rows_per_batch * x_row_stride;  // one stride for all rows
+  if (!flat && rows % rows_per_batch != 0) return set_error(HDIT_ERR_SHAPE, "rows must be a multiple of rows_per_batch");
+  RowsParams p{static_cast<const uint16_t*>(x), nullptr, nullptr, static_cast<int8_t*>(q), scale, flat ? 1 : rows / rows_per_batch,
+               flat ? rows : rows_per_batch, x_batch_stride, x_row_stride, q_row_stride, 0, static_cast<int>(dim), 0.f, false};
+  const bool vec = dim % 8 == 0 && !misaligned(x, x_row_stride) && (flat || x_batch_stride % 8 == 0);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  HDIT_CUDA_OK((dtype == HDIT_FP16 ? launch_any<true, false>(p, st) : launch_any<false, false>(p, st)));
+  HDIT_CUDA_OK(dtype == HDIT_FP16 ? launch_plain<true>(p, vec, st) : launch_plain<false>(p, vec, st));
   return HDIT_OK;
 }
 
@@ -255,11 +292,14 @@ extern "C" int hdit_ln_modulate_int8(int32_t dtype, const void* x, const void* s
   if (shift == nullptr || scale == nullptr) return set_error(HDIT_ERR_BAD_ARG, "null shift / scale");
   if (((reinterpret_cast<uintptr_t>(shift) | reinterpret_cast<uintptr_t>(scale)) & 1) != 0)
     return set_error(HDIT_ERR_SHAPE, "shift / scale not aligned to their elements");
-  const bool vec = !misaligned(x, x_row_stride) && x_batch_stride % 8 == 0 && !misaligned(shift, mod_batch_stride) && !misaligned(scale, mod_batch_stride);
+  if (rows > rows_per_batch && rows % rows_per_batch != 0) return set_error(HDIT_ERR_SHAPE, "rows must be a multiple of rows_per_batch");
+  const bool one = rows <= rows_per_batch;
   RowsParams p{static_cast<const uint16_t*>(x), static_cast<const uint16_t*>(shift), static_cast<const uint16_t*>(scale),
-               static_cast<int8_t*>(q), q_scale, rows, rows_per_batch, x_batch_stride, x_row_stride, q_row_stride, mod_batch_stride,
-               static_cast<int>(dim), eps, vec};
+               static_cast<int8_t*>(q), q_scale, one ? 1 : rows / rows_per_batch, one ? rows : rows_per_batch, x_batch_stride, x_row_stride,
+               q_row_stride, mod_batch_stride, static_cast<int>(dim), eps, !misaligned(shift, mod_batch_stride) && !misaligned(scale, mod_batch_stride)};
+  const bool vec = !misaligned(x, x_row_stride) && (one || x_batch_stride % 8 == 0);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  HDIT_CUDA_OK((dtype == HDIT_FP16 ? launch_any<true, true>(p, st) : launch_any<false, true>(p, st)));
+  HDIT_CUDA_OK((dtype == HDIT_FP16 ? (vec ? launch_ln<true, true>(p, st) : launch_ln<true, false>(p, st))
+                                   : (vec ? launch_ln<false, true>(p, st) : launch_ln<false, false>(p, st))));
   return HDIT_OK;
 }

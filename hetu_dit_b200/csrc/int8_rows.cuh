@@ -16,31 +16,39 @@ constexpr uint32_t kInt8RowTiny = 0x0D800000u;  // 2^-100
 constexpr uint32_t kInt8RowInf = 0x7F800000u;
 
 struct Int8Scale {
-  float scale, inv;  // value of one step, steps per unit
+  uint32_t top_bits;  // of max|y|; as unsigned integers magnitudes order like their values, and NaN is above all
+  float inv;          // steps per unit; 0: the row is all zeros
 };
 
-// From the bits of max|y| (as unsigned integers magnitudes order like their values, and NaN is above all).
 __device__ __forceinline__ Int8Scale int8_scale(uint32_t top_bits) {
-  if (top_bits >= kInt8RowInf) return {__uint_as_float(0x7FC00000u), 0.f};
-  if (top_bits < kInt8RowTiny) return {0.f, 0.f};
-  const float top = __uint_as_float(top_bits);
-  return {__fdiv_rn(top, 127.f), __fdiv_rn(127.f, top)};
+  return {top_bits, top_bits >= kInt8RowInf || top_bits < kInt8RowTiny ? 0.f : __fdiv_rn(127.f, __uint_as_float(top_bits))};
 }
+// The row's scale, for the one thread that writes it.
+__device__ __forceinline__ float int8_step(const Int8Scale& s) {
+  if (s.top_bits >= kInt8RowInf) return __uint_as_float(0x7FC00000u);
+  return s.inv == 0.f ? 0.f : __fdiv_rn(__uint_as_float(s.top_bits), 127.f);
+}
+
+constexpr float kInt8Round = 1.5f * 8388608.f;
 
 // Adding 1.5 * 2^23 rounds to the nearest integer, ties to even, and leaves it in the low bits as two's complement; the
 // low bytes of four of them are packed.
 __device__ __forceinline__ uint32_t int8_pack4(float a, float b, float c, float d) {
-  const uint32_t ua = __float_as_uint(__fadd_rn(a, 12582912.f)), ub = __float_as_uint(__fadd_rn(b, 12582912.f));
-  const uint32_t uc = __float_as_uint(__fadd_rn(c, 12582912.f)), ud = __float_as_uint(__fadd_rn(d, 12582912.f));
+  const uint32_t ua = __float_as_uint(__fadd_rn(a, kInt8Round)), ub = __float_as_uint(__fadd_rn(b, kInt8Round));
+  const uint32_t uc = __float_as_uint(__fadd_rn(c, kInt8Round)), ud = __float_as_uint(__fadd_rn(d, kInt8Round));
   return __byte_perm(__byte_perm(ua, ub, 0x0040), __byte_perm(uc, ud, 0x0040), 0x5410);
 }
 
 // v / s for a 16-bit v, exact at the borders between two integers. 254 v - (2 n + 1) max is a whole number of units in the
 // last place of v (v <= max), so 127 v / max is n + 1/2 or at least 2^-19 of its size away from it (v has at most 11 bits);
-// v * inv is within 2^-22.9 of the quotient. Rounding to 20 bits moves it by 2^-20 at most: that restores n + 1/2 (8 bits)
-// exactly and brings nothing else onto it or across.
-__device__ __forceinline__ float int8_steps_of_16bit(float v, float inv) {
-  return __uint_as_float((__float_as_uint(__fmul_rn(v, inv)) + 8u) & ~15u);
+// v * inv is within 2^-24 of the quotient. The sum below is v * inv rounded to 20 bits (Dekker's splitting: both terms are
+// multiples of 16 units of the quotient's last place, the second one rounds the exact difference), which moves it by 2^-20 at
+// most: that restores n + 1/2 (8 bits) exactly and brings nothing else onto it or across. inv17 = 17 * inv. Three operations of
+// the FMA pipe; on the bits, (bits + 8) & ~15 behind the product, two of them would be the integer pipe's, which the packing
+// needs.
+__device__ __forceinline__ float int8_steps_of_16bit(float v, float inv, float inv17) {
+  const float p = __fmul_rn(v, inv17);
+  return __fadd_rn(p, __fmaf_rn(v, inv, -p));
 }
 
 template <bool FP16>
@@ -59,29 +67,22 @@ __device__ __forceinline__ uint4 int8_load8(const uint16_t* row, int c, int dim,
   return make_uint4(e[0] | (e[1] << 16), e[2] | (e[3] << 16), e[4] | (e[5] << 16), e[6] | (e[7] << 16));
 }
 
-// Eight bytes to column c (a multiple of 8) of a row of dim that starts on a 16-byte boundary.
-__device__ __forceinline__ void int8_store8(int8_t* row, int c, int dim, uint2 v) {
-  if (c + 8 <= dim) {
-    *reinterpret_cast<uint2*>(row + c) = v;
-  } else {
-    for (int i = 0; i < 8 && c + i < dim; ++i) row[c + i] = static_cast<int8_t>((i < 4 ? v.x >> (8 * i) : v.y >> (8 * (i - 4))) & 0xFFu);
-  }
-}
-
 constexpr int kRowThreads = 256;  // of a CTA that works on rows
 
-// TEAM threads of a CTA that share a row; all teams of the CTA make the same calls.
+// TEAM threads of a CTA that share a row. A reduction over several warps has one barrier, of the team: each has places of its
+// own, and the barriers of the others stand between its reads and its next row's writes (where there are no others, the rows'
+// parity picks the places).
 template <int TEAM>
 struct Team {
   static constexpr int kWarps = TEAM / 32;
-  float* red;  // one float per warp of the CTA
-  __device__ __forceinline__ uint32_t max(uint32_t v) const {
+  float (*red)[kRowThreads / 32];
+  __device__ __forceinline__ void sync() const { asm volatile("bar.sync %0, %1;" ::"r"(1 + threadIdx.x / TEAM), "n"(TEAM) : "memory"); }
+  __device__ __forceinline__ uint32_t max(uint32_t v, int slot) const {
     v = __reduce_max_sync(0xffffffffu, v);
     if constexpr (kWarps > 1) {
-      uint32_t* r = reinterpret_cast<uint32_t*>(red);
-      __syncthreads();
+      uint32_t* r = reinterpret_cast<uint32_t*>(red[slot]);
       if ((threadIdx.x & 31) == 0) r[threadIdx.x >> 5] = v;
-      __syncthreads();
+      sync();
       v = 0;
       const int w0 = threadIdx.x / TEAM * kWarps;
 #pragma unroll
@@ -89,21 +90,46 @@ struct Team {
     }
     return v;
   }
-  __device__ __forceinline__ float sum(float v) const {
+  __device__ __forceinline__ float sum(float v, int slot) const {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     if constexpr (kWarps > 1) {
-      __syncthreads();
-      if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-      __syncthreads();
+      if ((threadIdx.x & 31) == 0) red[slot][threadIdx.x >> 5] = v;
+      sync();
       v = 0.f;
       const int w0 = threadIdx.x / TEAM * kWarps;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) v += red[w0 + w];
+      for (int w = 0; w < kWarps; ++w) v += red[slot][w0 + w];
     }
     return v;
   }
 };
+
+// Eight values in units of the row's step to column c of the row, which is on an 8-byte boundary; zeros where the row has no
+// step (an infinity times 0 is none).
+__device__ __forceinline__ void int8_put8(int8_t* row, int c, const Int8Scale& s, const float (&t)[8]) {
+  uint2 v = make_uint2(int8_pack4(t[0], t[1], t[2], t[3]), int8_pack4(t[4], t[5], t[6], t[7]));
+  if (s.inv == 0.f) v = make_uint2(0, 0);
+  *reinterpret_cast<uint2*>(row + c) = v;
+}
+
+// The same for eight values: product with inv and rounding to an integer in one operation.
+__device__ __forceinline__ void int8_put8_of(int8_t* row, int c, const Int8Scale& s, const float (&y)[8]) {
+  uint32_t u[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) u[i] = __float_as_uint(__fmaf_rn(y[i], s.inv, kInt8Round));
+  uint2 v = make_uint2(__byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410),
+                       __byte_perm(__byte_perm(u[4], u[5], 0x0040), __byte_perm(u[6], u[7], 0x0040), 0x5410));
+  if (s.inv == 0.f) v = make_uint2(0, 0);
+  *reinterpret_cast<uint2*>(row + c) = v;
+}
+
+// Larger of two magnitudes, NaN if one is: the compiler's fmaxf() drops a NaN.
+__device__ __forceinline__ float max_magnitude(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
+  return r;
+}
 
 }  // namespace
 }  // namespace hdit
