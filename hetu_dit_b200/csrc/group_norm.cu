@@ -3,22 +3,25 @@
 //   y[b, r, c] = (x[b, r, c] - mean[b, g]) / sqrt(var[b, g] + eps) * weight[c] + bias[c],   g = c / (channels / groups)
 // over rows r (pixels) and the channels of a group; biased variance.
 //
-// Two launches. The first one reads x once: a CTA takes a strip of rows of one image, each thread eight fixed channels, and
-// leaves {mean, sum of squared distances from it} per group and strip. Sums are taken relative to the strip's first row, so
-// that a mean far from zero costs no digits. The second one joins the strips (Chan's formula) and reads x again, each strip
-// from its end to its start: what the first launch read last is still in L2.
+// Two launches of one CTA per SM. The first one reads x once: a CTA takes a strip of rows of one image, each thread eight fixed
+// channels, and leaves {mean, sum of squared distances from it} per group and strip. Sums are taken relative to a value of the
+// strip's first row, so that a mean far from zero costs no digits. The second one joins the strips (Chan's formula) and reads x
+// again, each strip from its end to its start: what the first launch read last is still in L2. Every CTA joins the strips of
+// its image by itself; with four strips per SM, read eight at a time by a thread, that alone took 3 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include "host_common.h"
 #include "int8_rows.cuh"
+#include "ptx_sm100.cuh"
 
 namespace hdit {
 namespace {
 
 constexpr int kMaxChannels = 4096;
-constexpr int kGnThreads = 256;  // 512 for more than 2048 channels: a thread has eight of them
+constexpr int kGnThreads = 512;  // what a CTA does beside its rows costs every warp some hundred instructions
+constexpr int kAhead = 6;        // rows of a thread in flight
 
 struct GnParams {
   const uint16_t* x;
@@ -48,78 +51,107 @@ __device__ __forceinline__ float sub_sum(float v, int n_sub) {
   return v;
 }
 
-template <bool FP16>
-__global__ void __launch_bounds__(512) group_norm_stats_kernel(const __grid_constant__ GnParams p) {
+// Walks `count` rows of a thread, `step` elements apart: use(values of the row's eight channels, index). Groups of kAhead rows
+// are on their way while the group before is used.
+template <bool VEC, typename F>
+__device__ __forceinline__ void walk_rows(const uint16_t* x, int c, int channels, int count, long long step, F use) {
+  uint4 next[kAhead];
+  const int full = count / kAhead;
+  auto fetch = [&](int n) {
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      if (k < n) next[k] = int8_load8(x + k * step, c, channels, VEC);
+    x += kAhead * step;
+  };
+  fetch(full > 0 ? kAhead : count);
+  int at = 0;
+  for (int f = 0; f < full; ++f) {
+    uint4 raw[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) raw[k] = next[k];
+    if (f + 1 < full) fetch(kAhead);
+    else fetch(count - full * kAhead);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) use(raw[k], at + k);
+    at += kAhead;
+  }
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k)
+    if (at + k < count) use(next[k], at + k);
+}
+
+template <bool FP16, bool VEC>
+__global__ void __launch_bounds__(kGnThreads, 1) group_norm_stats_kernel(const __grid_constant__ GnParams p) {
   grid_dependency_release();
   grid_dependency_wait();
   extern __shared__ float smem[];  // [lanes][channels] sums, then the same of squares
   const int chunks = p.channels / 8;
-  const int lanes = static_cast<int>(blockDim.x) / chunks;  // rows at a time
-  const int chunk = threadIdx.x % chunks, lane = threadIdx.x / chunks;
+  const int lanes = kGnThreads / chunks;  // rows at a time
+  const int lane = threadIdx.x / chunks, c = (threadIdx.x - lane * chunks) * 8;
   const long long r0 = static_cast<long long>(blockIdx.x) * p.strip_rows;
-  const long long r1 = r0 + p.strip_rows < p.rows ? r0 + p.strip_rows : p.rows;
-  const uint16_t* xb = p.x + blockIdx.y * p.x_batch_stride;
-  const int c = chunk * 8;
-  float s[8], ss[8], pivot[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) s[i] = ss[i] = 0.f;
+  const int rows = static_cast<int>(r0 + p.strip_rows < p.rows ? p.strip_rows : p.rows - r0);
+  const uint16_t* xs = p.x + blockIdx.y * p.x_batch_stride + r0 * p.x_row_stride;
   if (lane < lanes) {
-    const uint4 first = int8_load8(xb + r0 * p.x_row_stride, c, p.channels, p.vec);
+    float s[8], ss[8], pivot[8];
+    const uint4 first = int8_load8(xs, c, p.channels, VEC);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float2 v = int8_unpack2<FP16>(reinterpret_cast<const uint32_t*>(&first)[i]);
       pivot[2 * i] = v.x;
       pivot[2 * i + 1] = v.y;
+      s[2 * i] = s[2 * i + 1] = ss[2 * i] = ss[2 * i + 1] = 0.f;
     }
-    constexpr int kAhead = 4;  // rows in flight
-    for (long long r = r0 + lane; r < r1; r += static_cast<long long>(kAhead) * lanes) {
-      uint4 raw[kAhead];
+    const int count = rows > lane ? (rows - lane + lanes - 1) / lanes : 0;
+    walk_rows<VEC>(xs + lane * p.x_row_stride, c, p.channels, count, lanes * p.x_row_stride, [&](const uint4& raw, int) {
+      const uint32_t* u = reinterpret_cast<const uint32_t*>(&raw);
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k)
-        raw[k] = r + static_cast<long long>(k) * lanes < r1 ? int8_load8(xb + (r + static_cast<long long>(k) * lanes) * p.x_row_stride, c, p.channels, p.vec) : first;
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-        const uint32_t* u = reinterpret_cast<const uint32_t*>(&raw[k]);
-        if (r + static_cast<long long>(k) * lanes < r1) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 v = int8_unpack2<FP16>(u[i]);
-            const float d0 = v.x - pivot[2 * i], d1 = v.y - pivot[2 * i + 1];
-            s[2 * i] += d0;
-            ss[2 * i] = fmaf(d0, d0, ss[2 * i]);
-            s[2 * i + 1] += d1;
-            ss[2 * i + 1] = fmaf(d1, d1, ss[2 * i + 1]);
-          }
-        }
+      for (int i = 0; i < 4; ++i) {
+        const float2 v = int8_unpack2<FP16>(u[i]);
+        const float d0 = v.x - pivot[2 * i], d1 = v.y - pivot[2 * i + 1];
+        s[2 * i] += d0;
+        ss[2 * i] = fmaf(d0, d0, ss[2 * i]);
+        s[2 * i + 1] += d1;
+        ss[2 * i + 1] = fmaf(d1, d1, ss[2 * i + 1]);
       }
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      smem[lane * p.channels + c + i] = s[i];
-      smem[(lanes + lane) * p.channels + c + i] = ss[i];
-    }
+    });
+    float4* to = reinterpret_cast<float4*>(smem + lane * p.channels + c);
+    to[0] = make_float4(s[0], s[1], s[2], s[3]);
+    to[1] = make_float4(s[4], s[5], s[6], s[7]);
+    to = reinterpret_cast<float4*>(smem + (lanes + lane) * p.channels + c);
+    to[0] = make_float4(ss[0], ss[1], ss[2], ss[3]);
+    to[1] = make_float4(ss[4], ss[5], ss[6], ss[7]);
   }
   __syncthreads();
-  // per channel: mean and sum of squared distances from it, in the first lane's places
-  const float n = static_cast<float>(r1 - r0);
-  for (int ch = threadIdx.x; ch < p.channels; ch += blockDim.x) {
+  // Over the lanes: `parts` neighbouring lanes of a warp to a channel. Then per channel, in the first lane's places: the mean,
+  // and the sum of squared distances from it.
+  int parts = 1;
+  while (parts < 32 && parts < lanes && parts * 2 * p.channels <= kGnThreads) parts *= 2;
+  const float inv_rows = 1.f / static_cast<float>(rows);
+  for (int ch0 = 0; ch0 < p.channels; ch0 += kGnThreads / parts) {
+    const int ch = ch0 + static_cast<int>(threadIdx.x) / parts, part = static_cast<int>(threadIdx.x) % parts;
     float a = 0.f, q = 0.f;
-    for (int l = 0; l < lanes; ++l) {
-      a += smem[l * p.channels + ch];
-      q += smem[(lanes + l) * p.channels + ch];
+    if (ch < p.channels)
+      for (int l = part; l < lanes; l += parts) {
+        a += smem[l * p.channels + ch];
+        q += smem[(lanes + l) * p.channels + ch];
+      }
+    a = sub_sum(a, parts);
+    q = sub_sum(q, parts);
+    if (ch < p.channels && part == 0) {  // no other thread reads this channel's first lane
+      const float m2 = q - a * a * inv_rows;
+      smem[ch] = int8_unpack2<FP16>(xs[ch]).x + a * inv_rows;
+      smem[lanes * p.channels + ch] = m2 > 0.f ? m2 : m2 - m2;  // keeps NaN
     }
-    uint16_t first = xb[r0 * p.x_row_stride + ch];
-    smem[ch] = int8_unpack2<FP16>(first).x + a / n;
-    smem[lanes * p.channels + ch] = fmaxf(q - a * a / n, 0.f) + (q - q);  // keeps NaN
   }
   __syncthreads();
   const int per = p.channels / p.groups;
+  const float n = static_cast<float>(rows), inv_per = 1.f / static_cast<float>(per);
   float2* out = p.partial + (static_cast<long long>(blockIdx.y) * p.strips + blockIdx.x) * p.groups;
   for_groups(p.groups, [&](int g, int sub, int n_sub) {
     const bool live = g < p.groups;
     float mean = 0.f, m2 = 0.f;
     for (int k = sub; live && k < per; k += n_sub) mean += smem[g * per + k];
-    mean = sub_sum(mean, n_sub) / static_cast<float>(per);
+    mean = sub_sum(mean, n_sub) * inv_per;
     for (int k = sub; live && k < per; k += n_sub) {
       const float d = smem[g * per + k] - mean;
       m2 += smem[lanes * p.channels + g * per + k] + n * d * d;
@@ -140,7 +172,8 @@ __device__ __forceinline__ void group_norm_join(const GnParams& p, int b, float2
     const bool live = g < p.groups;
     const float base = live ? in[g].x : 0.f;
     float a = 0.f, q = 0.f;
-    for (int k = sub; live && k < p.strips; k += n_sub) {
+#pragma unroll 4
+    for (int k = sub; k < (live ? p.strips : 0); k += n_sub) {
       const float2 v = in[static_cast<long long>(k) * p.groups + g];
       const float d = v.x - base, n = k == p.strips - 1 ? n_last : n_full;
       a = fmaf(n, d, a);
@@ -154,18 +187,33 @@ __device__ __forceinline__ void group_norm_join(const GnParams& p, int b, float2
   });
 }
 
-// y = x * a + b with a = weight / deviation and b = bias - mean * a. Against (x - mean) * a + bias that costs half a unit of
-// 2^-24 of mean * a: a 16-bit x resolves the deviation only while |mean| is below some 2^11 deviations, where this is
-// under 2^-13 of the result's deviation.
+// y = x * a + b with a = weight / deviation and b = bias - mean * a, for all channels of image blockIdx.y into shared memory:
+// `factors` holds a, then b, each first for the lower four channels of every chunk of eight, then for the upper four, so that
+// threads' 16 bytes lie side by side; behind them stand the groups' statistics.
+// Against (x - mean) * a + bias this form costs half a unit of 2^-24 of mean * a: a 16-bit x resolves the deviation only while
+// |mean| is below some 2^11 deviations, where that is under 2^-13 of the result's deviation.
 template <bool FP16>
-__device__ __forceinline__ float2 group_norm_factors(const GnParams& p, const float2* stat, int c) {
-  const float2 st = stat[c / (p.channels / p.groups)];
-  const uint32_t w = p.weight != nullptr ? p.weight[c] : (FP16 ? 0x3C00u : 0x3F80u), bi = p.bias != nullptr ? p.bias[c] : 0u;
-  const float a = st.y * int8_unpack2<FP16>(w).x;
-  return make_float2(a, fmaf(-st.x, a, int8_unpack2<FP16>(bi).x));
+__device__ __forceinline__ void group_norm_factors(const GnParams& p, float4* factors) {
+  const int chunks = p.channels / 8, per = p.channels / p.groups;
+  float2* stat = reinterpret_cast<float2*>(factors + 4 * chunks);
+  group_norm_join(p, blockIdx.y, stat);
+  __syncthreads();
+  for (int c = threadIdx.x; c < p.channels; c += blockDim.x) {
+    const float2 st = stat[c / per];
+    const float a = st.y * (p.weight != nullptr ? int8_unpack2<FP16>(p.weight[c]).x : 1.f);
+    float* to = reinterpret_cast<float*>(factors) + (c >> 3) * 4 + ((c >> 2) & 1) * chunks * 4 + (c & 3);
+    to[0] = a;
+    to[8 * chunks] = fmaf(-st.x, a, p.bias != nullptr ? int8_unpack2<FP16>(p.bias[c]).x : 0.f);
+  }
+  __syncthreads();
 }
 
-__device__ __forceinline__ float silu(float y) { return __fdividef(y, 1.f + __expf(-y)); }
+// y / (1 + exp(-y)): two operations of the special-function unit, each within 2^-22 of its result
+__device__ __forceinline__ float silu(float y) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + ex2_approx(-1.4426950408889634f * y)));
+  return y * r;
+}
 
 template <bool FP16>
 __device__ __forceinline__ uint32_t gn_pack(float lo, float hi) {
@@ -178,139 +226,125 @@ __device__ __forceinline__ uint32_t gn_pack(float lo, float hi) {
   }
 }
 
-template <bool FP16, bool SILU>
-__global__ void __launch_bounds__(512) group_norm_apply_kernel(const __grid_constant__ GnParams p) {
+template <bool FP16, bool SILU, bool VEC>
+__global__ void __launch_bounds__(kGnThreads, 1) group_norm_apply_kernel(const __grid_constant__ GnParams p) {
   grid_dependency_release();
   grid_dependency_wait();
-  extern __shared__ float smem[];
-  float2* stat = reinterpret_cast<float2*>(smem);
-  group_norm_join(p, blockIdx.y, stat);
-  __syncthreads();
+  extern __shared__ float4 factors[];
   const int chunks = p.channels / 8;
-  const int lanes = static_cast<int>(blockDim.x) / chunks;
-  const int chunk = threadIdx.x % chunks, lane = threadIdx.x / chunks;
+  const int lanes = kGnThreads / chunks;
+  const int lane = threadIdx.x / chunks, chunk = threadIdx.x - lane * chunks, c = chunk * 8;
+  const long long r0 = static_cast<long long>(blockIdx.x) * p.strip_rows;
+  const int rows = static_cast<int>(r0 + p.strip_rows < p.rows ? p.strip_rows : p.rows - r0);
+  group_norm_factors<FP16>(p, factors);
   if (lane >= lanes) return;
-  const int c = chunk * 8;
   float a[8], b[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float2 f = group_norm_factors<FP16>(p, stat, c + i);
-    a[i] = f.x;
-    b[i] = f.y;
+  for (int h = 0; h < 2; ++h) {
+    *reinterpret_cast<float4*>(a + 4 * h) = factors[h * chunks + chunk];
+    *reinterpret_cast<float4*>(b + 4 * h) = factors[(2 + h) * chunks + chunk];
   }
-  const long long r0 = static_cast<long long>(blockIdx.x) * p.strip_rows;
-  const long long r1 = r0 + p.strip_rows < p.rows ? r0 + p.strip_rows : p.rows;
-  const uint16_t* xb = p.x + blockIdx.y * p.x_batch_stride;
-  uint16_t* ob = p.out + blockIdx.y * p.out_batch_stride;
-  constexpr int kAhead = 4;
-  for (long long r = r1 - 1 - lane; r >= r0; r -= static_cast<long long>(kAhead) * lanes) {
-    uint4 raw[kAhead];
+  // from the strip's end to its start
+  const int count = rows > lane ? (rows - lane + lanes - 1) / lanes : 0;
+  const long long out_step = lanes * p.out_row_stride;
+  uint16_t* out = p.out + blockIdx.y * p.out_batch_stride + (r0 + rows - 1 - lane) * p.out_row_stride + c;
+  walk_rows<VEC>(p.x + blockIdx.y * p.x_batch_stride + (r0 + rows - 1 - lane) * p.x_row_stride, c, p.channels, count, -lanes * p.x_row_stride,
+                 [&](const uint4& raw, int i) {
+                   uint4 y = raw;
+                   uint32_t* u = reinterpret_cast<uint32_t*>(&y);
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      const long long rk = r - static_cast<long long>(k) * lanes;
-      raw[k] = rk >= r0 ? int8_load8(xb + rk * p.x_row_stride, c, p.channels, p.vec) : make_uint4(0, 0, 0, 0);
-    }
+                   for (int k = 0; k < 4; ++k) {
+                     const float2 v = int8_unpack2<FP16>(u[k]);
+                     float y0 = fmaf(v.x, a[2 * k], b[2 * k]), y1 = fmaf(v.y, a[2 * k + 1], b[2 * k + 1]);
+                     if constexpr (SILU) y0 = silu(y0), y1 = silu(y1);
+                     u[k] = gn_pack<FP16>(y0, y1);
+                   }
+                   uint16_t* dst = out - i * out_step;
+                   if constexpr (VEC) {
+                     *reinterpret_cast<uint4*>(dst) = y;
+                   } else {
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      const long long rk = r - static_cast<long long>(k) * lanes;
-      if (rk < r0) break;
-      uint32_t* u = reinterpret_cast<uint32_t*>(&raw[k]);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 v = int8_unpack2<FP16>(u[i]);
-        float y0 = fmaf(v.x, a[2 * i], b[2 * i]), y1 = fmaf(v.y, a[2 * i + 1], b[2 * i + 1]);
-        if constexpr (SILU) y0 = silu(y0), y1 = silu(y1);
-        u[i] = gn_pack<FP16>(y0, y1);
-      }
-      uint16_t* dst = ob + rk * p.out_row_stride + c;
-      if (p.vec) {
-        *reinterpret_cast<uint4*>(dst) = raw[k];
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) dst[i] = static_cast<uint16_t>(u[i / 2] >> (16 * (i & 1)));
-      }
-    }
-  }
+                     for (int k = 0; k < 8; ++k) dst[k] = static_cast<uint16_t>(u[k / 2] >> (16 * (k & 1)));
+                   }
+                 });
 }
 
-// The rows in 8 bits: TEAM threads hold a row of at most TEAM * NCH * 8 channels; factors of all channels in shared memory.
-template <bool FP16, bool SILU, int TEAM, int NCH>
-__global__ void __launch_bounds__(kRowThreads) group_norm_int8_kernel(const __grid_constant__ GnParams p) {
+// The rows in 8 bits: TEAM threads hold a row of at most TEAM * NCH * 8 channels and have the next one on its way; factors of
+// all channels in shared memory.
+template <bool FP16, bool SILU, int TEAM, int NCH, bool VEC>
+__global__ void __launch_bounds__(kGnThreads, 1) group_norm_int8_kernel(const __grid_constant__ GnParams p) {
   grid_dependency_release();
   grid_dependency_wait();
-  extern __shared__ float smem[];  // a[channels], b[channels], then {mean, 1 / deviation}[groups]
-  __shared__ float red[2][kRowThreads / 32];
-  float* fa = smem;
-  float* fb = smem + p.channels;
-  float2* stat = reinterpret_cast<float2*>(smem + 2 * p.channels);
-  group_norm_join(p, blockIdx.y, stat);
-  __syncthreads();
-  for (int c = threadIdx.x; c < p.channels; c += kRowThreads) {
-    const float2 f = group_norm_factors<FP16>(p, stat, c);
-    fa[c] = f.x;
-    fb[c] = f.y;
-  }
-  __syncthreads();
-  const Team<TEAM> team{red};
-  constexpr int kTeams = kRowThreads / TEAM;
-  const int lane = threadIdx.x % TEAM;
-  const long long r0 = static_cast<long long>(blockIdx.x) * p.strip_rows;
-  const long long r1 = r0 + p.strip_rows < p.rows ? r0 + p.strip_rows : p.rows;
-  const uint16_t* xb = p.x + blockIdx.y * p.x_batch_stride;
+  extern __shared__ float4 factors[];
+  __shared__ float red[2][kGnThreads / 32];
+  const int chunks = p.channels / 8;
+  const Team<TEAM, kGnThreads> team{red};
+  constexpr int kTeams = kGnThreads / TEAM;
+  const int c0 = static_cast<int>(threadIdx.x % TEAM) * 8, first = static_cast<int>(threadIdx.x) / TEAM;
+  const long long s0 = static_cast<long long>(blockIdx.x) * p.strip_rows;
+  const int rows = static_cast<int>(s0 + p.strip_rows < p.rows ? p.strip_rows : p.rows - s0);
+  const uint16_t* x = p.x + blockIdx.y * p.x_batch_stride + (s0 + rows - 1 - first) * p.x_row_stride;  // from the strip's end to its start
+  uint4 next[NCH];
+  auto fetch = [&] {
+#pragma unroll
+    for (int k = 0; k < NCH; ++k) {
+      next[k] = make_uint4(0, 0, 0, 0);
+      if (c0 + k * TEAM * 8 < p.channels) next[k] = int8_load8(x, c0 + k * TEAM * 8, p.channels, VEC);
+    }
+  };
+  if (first < rows) fetch();
+  group_norm_factors<FP16>(p, factors);
   int turn = 0;
-  for (long long rt = r1 - kTeams; rt > r0 - kTeams; rt -= kTeams, turn ^= 1) {
-    const long long r = rt + threadIdx.x / TEAM;
-    const bool live = r >= r0;
+  for (int r = first; r < rows; r += kTeams, turn ^= 1) {
+    uint4 raw[NCH];
+#pragma unroll
+    for (int k = 0; k < NCH; ++k) raw[k] = next[k];
+    x -= kTeams * p.x_row_stride;
+    if (r + kTeams < rows) fetch();
     float y[NCH][8];
     float top = 0.f;
 #pragma unroll
     for (int k = 0; k < NCH; ++k) {
-      const int c = (k * TEAM + lane) * 8;
-      if (live && c < p.channels) {
-        const uint4 raw = int8_load8(xb + r * p.x_row_stride, c, p.channels, p.vec);
-        const uint32_t* u = reinterpret_cast<const uint32_t*>(&raw);
-        const float4* a4 = reinterpret_cast<const float4*>(fa + c);
-        const float4* b4 = reinterpret_cast<const float4*>(fb + c);
+      const int c = c0 + k * TEAM * 8;
+      if (c >= p.channels) continue;
+      const uint32_t* u = reinterpret_cast<const uint32_t*>(&raw[k]);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float4 av = a4[h], bv = b4[h];
-          const float2 v0 = int8_unpack2<FP16>(u[2 * h]), v1 = int8_unpack2<FP16>(u[2 * h + 1]);
-          y[k][4 * h] = fmaf(v0.x, av.x, bv.x);
-          y[k][4 * h + 1] = fmaf(v0.y, av.y, bv.y);
-          y[k][4 * h + 2] = fmaf(v1.x, av.z, bv.z);
-          y[k][4 * h + 3] = fmaf(v1.y, av.w, bv.w);
-        }
+      for (int h = 0; h < 2; ++h) {
+        const float4 av = factors[h * chunks + (c >> 3)], bv = factors[(2 + h) * chunks + (c >> 3)];
+        const float2 v0 = int8_unpack2<FP16>(u[2 * h]), v1 = int8_unpack2<FP16>(u[2 * h + 1]);
+        y[k][4 * h] = fmaf(v0.x, av.x, bv.x);
+        y[k][4 * h + 1] = fmaf(v0.y, av.y, bv.y);
+        y[k][4 * h + 2] = fmaf(v1.x, av.z, bv.z);
+        y[k][4 * h + 3] = fmaf(v1.y, av.w, bv.w);
+      }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if constexpr (SILU) y[k][i] = silu(y[k][i]);
-          top = max_magnitude(top, y[k][i]);
-        }
+      for (int i = 0; i < 8; ++i) {
+        if constexpr (SILU) y[k][i] = silu(y[k][i]);
+        top = max_magnitude(top, y[k][i]);
       }
     }
     const Int8Scale s = int8_scale(team.max(__float_as_uint(top) & 0x7FFFFFFFu, turn));
-    if (live) {
-      const long long row = blockIdx.y * p.rows + r;
+    const long long row = blockIdx.y * p.rows + s0 + rows - 1 - r;
 #pragma unroll
-      for (int k = 0; k < NCH; ++k) {
-        const int c = (k * TEAM + lane) * 8;
-        if (c < p.channels) {
-          int8_put8_of(p.q + row * p.out_row_stride, c, s, y[k]);
-        }
-      }
-      if (lane == 0) p.q_scale[row] = int8_step(s);
-    }
+    for (int k = 0; k < NCH; ++k)
+      if (c0 + k * TEAM * 8 < p.channels) int8_put8_of(p.q + row * p.out_row_stride, c0 + k * TEAM * 8, s, y[k]);
+    if (c0 == 0) p.q_scale[row] = int8_step(s);
   }
 }
 
-int gn_threads(int channels) { return channels > 2048 ? 512 : kGnThreads; }
-
-// Strips per image: four CTAs per SM over all images, at least sixteen rows of every thread's channels each.
+// Strips per image: one CTA per SM over all images, at least two rows of every thread's channels each.
 int strips_of(long long batch, long long rows, int channels) {
-  const long long lanes = gn_threads(channels) / (channels / 8);
-  long long n = (148 * 4 + batch - 1) / batch;
-  const long long most = (rows + lanes * 16 - 1) / (lanes * 16);
+  const long long lanes = kGnThreads / (channels / 8);
+  long long n = 148 / batch;
+  const long long most = (rows + lanes * 2 - 1) / (lanes * 2);
   if (n > most) n = most;
   return static_cast<int>(n < 1 ? 1 : n);
+}
+
+void set_strips(GnParams& p, long long batch) {
+  p.strips = strips_of(batch, p.rows, p.channels);
+  p.strip_rows = (p.rows + p.strips - 1) / p.strips;
+  p.strips = static_cast<int>((p.rows + p.strip_rows - 1) / p.strip_rows);
 }
 
 int check_gn(int dtype, const void* x, const void* out, const void* partial, int64_t batch, int64_t rows, int64_t channels, int64_t groups,
@@ -329,26 +363,43 @@ int check_gn(int dtype, const void* x, const void* out, const void* partial, int
 
 bool off16(const void* p, int64_t a, int64_t b) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0 || a % 8 != 0 || b % 8 != 0; }
 
-cudaError_t launch_stats(const GnParams& p, bool fp16, long long batch, cudaStream_t st) {
-  const int threads = gn_threads(p.channels);
-  const size_t smem = static_cast<size_t>(threads / (p.channels / 8)) * p.channels * 2 * sizeof(float);
-  return launch_overlapped(fp16 ? group_norm_stats_kernel<true> : group_norm_stats_kernel<false>,
-                           dim3(static_cast<unsigned>(p.strips), static_cast<unsigned>(batch)), dim3(static_cast<unsigned>(threads)), smem, st, 1, p);
-}
-
-template <bool FP16, bool SILU>
-cudaError_t launch_int8(const GnParams& p, long long batch, cudaStream_t st) {
-  const size_t smem = static_cast<size_t>(p.channels) * 2 * sizeof(float) + static_cast<size_t>(p.groups) * sizeof(float2);
-  auto kernel = p.channels <= 256    ? group_norm_int8_kernel<FP16, SILU, 32, 1>
-                : p.channels <= 512  ? group_norm_int8_kernel<FP16, SILU, 32, 2>
-                : p.channels <= 1024 ? group_norm_int8_kernel<FP16, SILU, 32, 4>
-                : p.channels <= 2048 ? group_norm_int8_kernel<FP16, SILU, 128, 2>
-                                     : group_norm_int8_kernel<FP16, SILU, 128, 4>;
-  // above 47 KB only where almost every channel is a group of its own
+template <typename K>
+cudaError_t launch_strips(K kernel, const GnParams& p, long long batch, size_t smem, cudaStream_t st) {
+  // static shared memory counts, too
   const cudaError_t e = smem > 47 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) : cudaSuccess;
   if (e != cudaSuccess) return e;
-  return launch_overlapped(kernel, dim3(static_cast<unsigned>(p.strips), static_cast<unsigned>(batch)), dim3(kRowThreads), smem, st, 1, p);
+  return launch_overlapped(kernel, dim3(static_cast<unsigned>(p.strips), static_cast<unsigned>(batch)), dim3(kGnThreads), smem, st, 1, p);
 }
+
+size_t factor_bytes(const GnParams& p) { return static_cast<size_t>(p.channels) * 2 * sizeof(float) + static_cast<size_t>(p.groups) * sizeof(float2); }
+
+template <bool FP16, bool VEC>
+cudaError_t launch_stats(const GnParams& p, long long batch, cudaStream_t st) {
+  const size_t smem = static_cast<size_t>(kGnThreads / (p.channels / 8)) * p.channels * 2 * sizeof(float);
+  return launch_strips(group_norm_stats_kernel<FP16, VEC>, p, batch, smem, st);
+}
+
+template <bool FP16, bool VEC>
+cudaError_t launch_apply(const GnParams& p, long long batch, cudaStream_t st) {
+  return p.act == HDIT_ACT_SILU ? launch_strips(group_norm_apply_kernel<FP16, true, VEC>, p, batch, factor_bytes(p), st)
+                                : launch_strips(group_norm_apply_kernel<FP16, false, VEC>, p, batch, factor_bytes(p), st);
+}
+
+template <bool FP16, bool SILU, bool VEC>
+cudaError_t launch_int8_act(const GnParams& p, long long batch, cudaStream_t st) {
+  auto kernel = p.channels <= 256    ? group_norm_int8_kernel<FP16, SILU, 32, 1, VEC>
+                : p.channels <= 512  ? group_norm_int8_kernel<FP16, SILU, 32, 2, VEC>
+                : p.channels <= 1024 ? group_norm_int8_kernel<FP16, SILU, 32, 4, VEC>
+                                     : group_norm_int8_kernel<FP16, SILU, 128, 4, VEC>;
+  return launch_strips(kernel, p, batch, factor_bytes(p), st);
+}
+
+template <bool FP16, bool VEC>
+cudaError_t launch_int8(const GnParams& p, long long batch, cudaStream_t st) {
+  return p.act == HDIT_ACT_SILU ? launch_int8_act<FP16, true, VEC>(p, batch, st) : launch_int8_act<FP16, false, VEC>(p, batch, st);
+}
+
+#define HDIT_GN_OF(f, fp16, vec) ((fp16) ? ((vec) ? f<true, true> : f<true, false>) : ((vec) ? f<false, true> : f<false, false>))
 
 }  // namespace
 }  // namespace hdit
@@ -369,16 +420,11 @@ extern "C" int hdit_group_norm(int32_t dtype, const void* x, const void* weight,
              nullptr, nullptr, static_cast<float2*>(scratch), rows, x_batch_stride, x_row_stride, out_batch_stride, out_row_stride, 0, 0,
              static_cast<int>(channels), static_cast<int>(groups), act, eps,
              !off16(x, x_batch_stride, x_row_stride) && !off16(out, out_batch_stride, out_row_stride)};
-  p.strips = strips_of(batch, rows, p.channels);
-  p.strip_rows = (rows + p.strips - 1) / p.strips;
-  p.strips = static_cast<int>((rows + p.strip_rows - 1) / p.strip_rows);
+  set_strips(p, batch);
   const bool fp16 = dtype == HDIT_FP16;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  HDIT_CUDA_OK(launch_stats(p, fp16, batch, st));
-  auto kernel = act == HDIT_ACT_SILU ? (fp16 ? group_norm_apply_kernel<true, true> : group_norm_apply_kernel<false, true>)
-                                     : (fp16 ? group_norm_apply_kernel<true, false> : group_norm_apply_kernel<false, false>);
-  HDIT_CUDA_OK(launch_overlapped(kernel, dim3(static_cast<unsigned>(p.strips), static_cast<unsigned>(batch)),
-                                 dim3(static_cast<unsigned>(gn_threads(p.channels))), static_cast<size_t>(p.groups) * sizeof(float2), st, 1, p));
+  HDIT_CUDA_OK((HDIT_GN_OF(launch_stats, fp16, p.vec)(p, batch, st)));
+  HDIT_CUDA_OK((HDIT_GN_OF(launch_apply, fp16, p.vec)(p, batch, st)));
   return HDIT_OK;
 }
 
@@ -395,14 +441,10 @@ extern "C" int hdit_group_norm_int8(int32_t dtype, const void* x, const void* we
   GnParams p{static_cast<const uint16_t*>(x), static_cast<const uint16_t*>(weight), static_cast<const uint16_t*>(bias), nullptr,
              static_cast<int8_t*>(q), q_scale, static_cast<float2*>(scratch), rows, x_batch_stride, x_row_stride, 0, q_row_stride, 0, 0,
              static_cast<int>(channels), static_cast<int>(groups), act, eps, !off16(x, x_batch_stride, x_row_stride)};
-  p.strips = strips_of(batch, rows, p.channels);
-  p.strip_rows = (rows + p.strips - 1) / p.strips;
-  p.strips = static_cast<int>((rows + p.strip_rows - 1) / p.strip_rows);
+  set_strips(p, batch);
   const bool fp16 = dtype == HDIT_FP16;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  HDIT_CUDA_OK(launch_stats(p, fp16, batch, st));
-  const bool sl = act == HDIT_ACT_SILU;
-  HDIT_CUDA_OK((fp16 ? (sl ? launch_int8<true, true>(p, batch, st) : launch_int8<true, false>(p, batch, st))
-                     : (sl ? launch_int8<false, true>(p, batch, st) : launch_int8<false, false>(p, batch, st))));
+  HDIT_CUDA_OK((HDIT_GN_OF(launch_stats, fp16, p.vec)(p, batch, st)));
+  HDIT_CUDA_OK((HDIT_GN_OF(launch_int8, fp16, p.vec)(p, batch, st)));
   return HDIT_OK;
 }

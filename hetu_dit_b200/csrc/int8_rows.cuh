@@ -72,10 +72,10 @@ constexpr int kRowThreads = 256;  // of a CTA that works on rows
 // TEAM threads of a CTA that share a row. A reduction over several warps has one barrier, of the team: each has places of its
 // own, and the barriers of the others stand between its reads and its next row's writes (where there are no others, the rows'
 // parity picks the places).
-template <int TEAM>
+template <int TEAM, int THREADS = kRowThreads>
 struct Team {
   static constexpr int kWarps = TEAM / 32;
-  float (*red)[kRowThreads / 32];
+  float (*red)[THREADS / 32];
   __device__ __forceinline__ void sync() const { asm volatile("bar.sync %0, %1;" ::"r"(1 + threadIdx.x / TEAM), "n"(TEAM) : "memory"); }
   __device__ __forceinline__ uint32_t max(uint32_t v, int slot) const {
     v = __reduce_max_sync(0xffffffffu, v);
