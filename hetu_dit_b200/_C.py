@@ -263,6 +263,30 @@ class Int8LinearArgs(ctypes.Structure):
     ]
 
 
+class GroupNormArgs(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("act", ctypes.c_int32),
+        ("x", ctypes.c_void_p),
+        ("weight", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("out_scale", ctypes.c_void_p),
+        ("scratch", ctypes.c_void_p),
+        ("batch", ctypes.c_int64),
+        ("rows", ctypes.c_int64),
+        ("channels", ctypes.c_int64),
+        ("groups", ctypes.c_int64),
+        ("x_batch_stride", ctypes.c_int64),
+        ("x_row_stride", ctypes.c_int64),
+        ("out_batch_stride", ctypes.c_int64),
+        ("out_row_stride", ctypes.c_int64),
+        ("stream", ctypes.c_void_p),
+        ("eps", ctypes.c_float),
+        ("reserved0", ctypes.c_int32),
+    ]
+
+
 INT8_MAX_K = 131072
 ACT_NONE, ACT_SILU = 0, 1
 
@@ -318,11 +342,9 @@ def _declare(lib):
     lib.hdit_group_norm_scratch.restype = ctypes.c_int64
     lib.hdit_group_norm_scratch.argtypes = [ctypes.c_int64] * 4
     lib.hdit_group_norm.restype = ctypes.c_int
-    lib.hdit_group_norm.argtypes = [ctypes.c_int32] + [ctypes.c_void_p] * 5 + [ctypes.c_int64] * 8 + [
-        ctypes.c_float, ctypes.c_int32, ctypes.c_void_p]
+    lib.hdit_group_norm.argtypes = [ctypes.POINTER(GroupNormArgs)]
     lib.hdit_group_norm_int8.restype = ctypes.c_int
-    lib.hdit_group_norm_int8.argtypes = [ctypes.c_int32] + [ctypes.c_void_p] * 6 + [ctypes.c_int64] * 7 + [
-        ctypes.c_float, ctypes.c_int32, ctypes.c_void_p]
+    lib.hdit_group_norm_int8.argtypes = [ctypes.POINTER(GroupNormArgs)]
     lib.hdit_heap_alloc.restype = ctypes.c_int
     lib.hdit_heap_alloc.argtypes = [ctypes.c_int64, ctypes.POINTER(ctypes.c_void_p)]
     lib.hdit_heap_free.restype = ctypes.c_int

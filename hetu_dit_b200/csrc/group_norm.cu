@@ -347,17 +347,17 @@ void set_strips(GnParams& p, long long batch) {
   p.strips = static_cast<int>((p.rows + p.strip_rows - 1) / p.strip_rows);
 }
 
-int check_gn(int dtype, const void* x, const void* out, const void* partial, int64_t batch, int64_t rows, int64_t channels, int64_t groups,
-             int act) {
-  if (dtype != HDIT_BF16 && dtype != HDIT_FP16) return set_error(HDIT_ERR_BAD_ARG, "dtype must be bf16 or fp16");
-  if (batch < 0 || rows < 0 || channels <= 0 || groups <= 0) return set_error(HDIT_ERR_BAD_ARG, "bad sizes");
-  if (act != HDIT_ACT_NONE && act != HDIT_ACT_SILU) return set_error(HDIT_ERR_BAD_ARG, "unknown activation %d", act);
-  if (channels % 8 != 0 || channels > kMaxChannels || channels % groups != 0)
+int check_gn(const hdit_group_norm_args* a) {
+  if (a == nullptr) return set_error(HDIT_ERR_BAD_ARG, "null args");
+  if (a->dtype != HDIT_BF16 && a->dtype != HDIT_FP16) return set_error(HDIT_ERR_BAD_ARG, "dtype must be bf16 or fp16");
+  if (a->batch < 0 || a->rows < 0 || a->channels <= 0 || a->groups <= 0) return set_error(HDIT_ERR_BAD_ARG, "bad sizes");
+  if (a->act != HDIT_ACT_NONE && a->act != HDIT_ACT_SILU) return set_error(HDIT_ERR_BAD_ARG, "unknown activation %d", a->act);
+  if (a->channels % 8 != 0 || a->channels > kMaxChannels || a->channels % a->groups != 0)
     return set_error(HDIT_ERR_SHAPE, "channels must be a multiple of 8 and of groups, at most %d", kMaxChannels);
-  if (batch > 65535 || rows > 0x7fffffffLL) return set_error(HDIT_ERR_TOO_LARGE, "at most 65535 images of 2^31 - 1 rows");
-  if (batch == 0 || rows == 0) return HDIT_OK;
-  if (x == nullptr || out == nullptr || partial == nullptr) return set_error(HDIT_ERR_BAD_ARG, "null x / out / scratch");
-  if ((reinterpret_cast<uintptr_t>(partial) & 7) != 0) return set_error(HDIT_ERR_SHAPE, "scratch not 8-byte aligned");
+  if (a->batch > 65535 || a->rows > 0x7fffffffLL) return set_error(HDIT_ERR_TOO_LARGE, "at most 65535 images of 2^31 - 1 rows");
+  if (a->batch == 0 || a->rows == 0) return HDIT_OK;
+  if (a->x == nullptr || a->out == nullptr || a->scratch == nullptr) return set_error(HDIT_ERR_BAD_ARG, "null x / out / scratch");
+  if ((reinterpret_cast<uintptr_t>(a->scratch) & 7) != 0) return set_error(HDIT_ERR_SHAPE, "scratch not 8-byte aligned");
   return HDIT_OK;
 }
 
@@ -369,6 +369,29 @@ cudaError_t launch_strips(K kernel, const GnParams& p, long long batch, size_t s
   const cudaError_t e = smem > 47 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) : cudaSuccess;
   if (e != cudaSuccess) return e;
   return launch_overlapped(kernel, dim3(static_cast<unsigned>(p.strips), static_cast<unsigned>(batch)), dim3(kGnThreads), smem, st, 1, p);
+}
+
+GnParams params_of(const hdit_group_norm_args* a, bool out_vec) {
+  GnParams p{};
+  p.x = static_cast<const uint16_t*>(a->x);
+  p.weight = static_cast<const uint16_t*>(a->weight);
+  p.bias = static_cast<const uint16_t*>(a->bias);
+  p.out = static_cast<uint16_t*>(a->out);
+  p.q = static_cast<int8_t*>(a->out);
+  p.q_scale = a->out_scale;
+  p.partial = static_cast<float2*>(a->scratch);
+  p.rows = a->rows;
+  p.x_batch_stride = a->x_batch_stride;
+  p.x_row_stride = a->x_row_stride;
+  p.out_batch_stride = a->out_batch_stride;
+  p.out_row_stride = a->out_row_stride;
+  p.channels = static_cast<int>(a->channels);
+  p.groups = static_cast<int>(a->groups);
+  p.act = a->act;
+  p.eps = a->eps;
+  p.vec = out_vec && !off16(a->x, a->x_batch_stride, a->x_row_stride);
+  set_strips(p, a->batch);
+  return p;
 }
 
 size_t factor_bytes(const GnParams& p) { return static_cast<size_t>(p.channels) * 2 * sizeof(float) + static_cast<size_t>(p.groups) * sizeof(float2); }
@@ -410,41 +433,30 @@ extern "C" int64_t hdit_group_norm_scratch(int64_t batch, int64_t rows, int64_t 
   return batch * strips_of(batch, rows, static_cast<int>(channels)) * groups * static_cast<int64_t>(sizeof(float2));
 }
 
-extern "C" int hdit_group_norm(int32_t dtype, const void* x, const void* weight, const void* bias, void* out, void* scratch, int64_t batch,
-                               int64_t rows, int64_t channels, int64_t groups, int64_t x_batch_stride, int64_t x_row_stride,
-                               int64_t out_batch_stride, int64_t out_row_stride, float eps, int32_t act, void* stream) {
+extern "C" int hdit_group_norm(const hdit_group_norm_args* a) {
   using namespace hdit;
-  const int rc = check_gn(dtype, x, out, scratch, batch, rows, channels, groups, act);
-  if (rc != HDIT_OK || batch == 0 || rows == 0) return rc;
-  GnParams p{static_cast<const uint16_t*>(x), static_cast<const uint16_t*>(weight), static_cast<const uint16_t*>(bias), static_cast<uint16_t*>(out),
-             nullptr, nullptr, static_cast<float2*>(scratch), rows, x_batch_stride, x_row_stride, out_batch_stride, out_row_stride, 0, 0,
-             static_cast<int>(channels), static_cast<int>(groups), act, eps,
-             !off16(x, x_batch_stride, x_row_stride) && !off16(out, out_batch_stride, out_row_stride)};
-  set_strips(p, batch);
-  const bool fp16 = dtype == HDIT_FP16;
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  HDIT_CUDA_OK((HDIT_GN_OF(launch_stats, fp16, p.vec)(p, batch, st)));
-  HDIT_CUDA_OK((HDIT_GN_OF(launch_apply, fp16, p.vec)(p, batch, st)));
+  const int rc = check_gn(a);
+  if (rc != HDIT_OK || a->batch == 0 || a->rows == 0) return rc;
+  const GnParams p = params_of(a, !off16(a->out, a->out_batch_stride, a->out_row_stride));
+  const bool fp16 = a->dtype == HDIT_FP16;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(a->stream);
+  HDIT_CUDA_OK((HDIT_GN_OF(launch_stats, fp16, p.vec)(p, a->batch, st)));
+  HDIT_CUDA_OK((HDIT_GN_OF(launch_apply, fp16, p.vec)(p, a->batch, st)));
   return HDIT_OK;
 }
 
-extern "C" int hdit_group_norm_int8(int32_t dtype, const void* x, const void* weight, const void* bias, void* q, float* q_scale, void* scratch,
-                                    int64_t batch, int64_t rows, int64_t channels, int64_t groups, int64_t x_batch_stride, int64_t x_row_stride,
-                                    int64_t q_row_stride, float eps, int32_t act, void* stream) {
+extern "C" int hdit_group_norm_int8(const hdit_group_norm_args* a) {
   using namespace hdit;
-  const int rc = check_gn(dtype, x, q, scratch, batch, rows, channels, groups, act);
+  const int rc = check_gn(a);
   if (rc != HDIT_OK) return rc;
-  if ((reinterpret_cast<uintptr_t>(q) & 15) != 0 || q_row_stride % 16 != 0 || q_row_stride < channels)
+  if ((reinterpret_cast<uintptr_t>(a->out) & 15) != 0 || a->out_row_stride % 16 != 0 || a->out_row_stride < a->channels)
     return set_error(HDIT_ERR_SHAPE, "8-bit rows need a 16-byte aligned pointer and a row stride that is a multiple of 16 and covers a row");
-  if (batch == 0 || rows == 0) return HDIT_OK;
-  if (q_scale == nullptr) return set_error(HDIT_ERR_BAD_ARG, "null scale");
-  GnParams p{static_cast<const uint16_t*>(x), static_cast<const uint16_t*>(weight), static_cast<const uint16_t*>(bias), nullptr,
-             static_cast<int8_t*>(q), q_scale, static_cast<float2*>(scratch), rows, x_batch_stride, x_row_stride, 0, q_row_stride, 0, 0,
-             static_cast<int>(channels), static_cast<int>(groups), act, eps, !off16(x, x_batch_stride, x_row_stride)};
-  set_strips(p, batch);
-  const bool fp16 = dtype == HDIT_FP16;
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  HDIT_CUDA_OK((HDIT_GN_OF(launch_stats, fp16, p.vec)(p, batch, st)));
-  HDIT_CUDA_OK((HDIT_GN_OF(launch_int8, fp16, p.vec)(p, batch, st)));
+  if (a->batch == 0 || a->rows == 0) return HDIT_OK;
+  if (a->out_scale == nullptr) return set_error(HDIT_ERR_BAD_ARG, "null scale");
+  const GnParams p = params_of(a, true);
+  const bool fp16 = a->dtype == HDIT_FP16;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(a->stream);
+  HDIT_CUDA_OK((HDIT_GN_OF(launch_stats, fp16, p.vec)(p, a->batch, st)));
+  HDIT_CUDA_OK((HDIT_GN_OF(launch_int8, fp16, p.vec)(p, a->batch, st)));
   return HDIT_OK;
 }

@@ -947,10 +947,11 @@ class Int8Rows:
         return (self.q.float() * self.scale[..., None]).to(self.dtype)
 
 
-def _empty_int8_rows(lead, k, device, dtype):
+def _empty_int8_rows(x, lead, k):
+    """Int8Rows for rows of x's type on its device, rows on 16-byte boundaries."""
     pitch = (k + 15) & ~15
-    q = torch.empty((*lead, pitch), dtype=torch.int8, device=device)
-    return Int8Rows(q if pitch == k else q[..., :k], torch.empty(lead, dtype=torch.float32, device=device), dtype)
+    q = x.new_empty((*lead, pitch), dtype=torch.int8)
+    return Int8Rows(q if pitch == k else q[..., :k], x.new_empty(lead, dtype=torch.float32), x.dtype)
 
 
 def quantize_rows(x):
@@ -958,19 +959,27 @@ def quantize_rows(x):
     integer, ties to even. Any K and strides with contiguous K. A row with an infinity or NaN gets a NaN scale (what is
     computed from it is NaN), one below 2^-100 throughout counts as zero."""
     _require_cuda(x)
-    if x.dtype not in _DTYPE_CODE:
-        raise TypeError(f"unsupported dtype {x.dtype}")
-    if x.dim() not in (2, 3) or x.shape[-1] == 0 or (x.stride(-1) != 1 and x.shape[-1] != 1):
+    dtype = x.dtype
+    if dtype not in _DTYPE_CODE:
+        raise TypeError(f"unsupported dtype {dtype}")
+    shape, strides = x.shape, x.stride()
+    if len(shape) == 3:
+        (B, S, k), (sb, ss, sk) = shape, strides
+        lead = (B, S)
+    elif len(shape) == 2:
+        (S, k), (ss, sk), B, sb = shape, strides, 1, 0
+        lead = (S,)
+    else:
+        raise ValueError("expected (B, S, K) or (rows, K)")
+    if k == 0 or (sk != 1 and k != 1):
         raise ValueError("expected (B, S, K) or (rows, K) with contiguous K")
-    lead, k = x.shape[:-1], x.shape[-1]
-    out = _empty_int8_rows(lead, k, x.device, x.dtype)
-    rows = out.scale.numel()
-    if rows == 0:
+    out = _empty_int8_rows(x, lead, k)
+    if B * S == 0:
         return out
-    sb = x.stride(0) if x.dim() == 3 else 0
-    with _on(x.device):
-        _C.check(_C.lib().hdit_quantize_rows(_DTYPE_CODE[x.dtype], x.data_ptr(), out.q.data_ptr(), out.scale.data_ptr(), rows, k,
-                                             lead[-1], sb, x.stride(-2), out.q.stride(-2), _stream_ptr(x.device)))
+    dev = x.device
+    with _on(dev):
+        _C.check(_C.lib().hdit_quantize_rows(_DTYPE_CODE[dtype], x.data_ptr(), out.q.data_ptr(), out.scale.data_ptr(), B * S, k, S,
+                                             sb, ss, (k + 15) & ~15, _stream_ptr(dev)))
     _count()
     return out
 
@@ -979,23 +988,27 @@ def ln_modulate_int8(x, shift, scale, eps=1e-6):
     """ln_modulate() with its rows in 8 bits, see quantize_rows(); nothing is rounded to 16 bits in between. x (B, S, Dm) with
     contiguous Dm, a multiple of 8 and at most 8192; shift / scale (B, Dm) views."""
     _require_cuda(x)
-    if x.dtype not in _DTYPE_CODE or shift.dtype != x.dtype or scale.dtype != x.dtype:
+    dtype, dev, shape = x.dtype, x.device, x.shape
+    if dtype not in _DTYPE_CODE or shift.dtype != dtype or scale.dtype != dtype:
         raise TypeError("x, shift and scale must be of one 16-bit type")
-    if x.dim() != 3 or x.stride(2) != 1:
+    if len(shape) != 3:
         raise ValueError("expected a (B, S, Dm) tensor with contiguous last dim")
-    B, S, dim = x.shape
-    if shift.shape != (B, dim) or scale.shape != (B, dim) or shift.stride(1) != 1 or scale.stride(1) != 1 or \
-            (B > 1 and shift.stride(0) != scale.stride(0)):
+    (B, S, dim), (sb, ss, sk) = shape, x.stride()
+    if sk != 1:
+        raise ValueError("expected a (B, S, Dm) tensor with contiguous last dim")
+    mod = shift.stride()
+    if shift.shape != (B, dim) or scale.shape != (B, dim) or mod[1] != 1 or (mod != scale.stride() and (B > 1 or scale.stride(1) != 1)):
         raise ValueError("shift / scale must be (B, Dm) views with contiguous last dim and equal batch stride")
-    if shift.device != x.device or scale.device != x.device:
+    if shift.device != dev or scale.device != dev:
         raise ValueError("x, shift and scale must be on one device")
-    out = _empty_int8_rows((B, S), dim, x.device, x.dtype)
-    with _on(x.device):
-        _C.check(_C.lib().hdit_ln_modulate_int8(_DTYPE_CODE[x.dtype], x.data_ptr(), shift.data_ptr(), scale.data_ptr(),
-                                                out.q.data_ptr(), out.scale.data_ptr(), B * S, dim, max(S, 1), x.stride(0),
-                                                x.stride(1), out.q.stride(1), shift.stride(0), eps, _stream_ptr(x.device)))
-    if B * S:
-        _count()
+    out = _empty_int8_rows(x, (B, S), dim)
+    if B * S == 0:
+        return out
+    with _on(dev):
+        _C.check(_C.lib().hdit_ln_modulate_int8(_DTYPE_CODE[dtype], x.data_ptr(), shift.data_ptr(), scale.data_ptr(),
+                                                out.q.data_ptr(), out.scale.data_ptr(), B * S, dim, S, sb, ss, (dim + 15) & ~15,
+                                                mod[0], eps, _stream_ptr(dev)))
+    _count()
     return out
 
 
@@ -1010,38 +1023,41 @@ def linear_int8(x, weight, bias=None, epilogue="bias", residual=None, gate=None,
     16-bit type once. B, S, K, N need not be multiples of anything. `out` may be a column block of a wider buffer, or
     `residual` itself."""
     held = type(x) is Int8Rows
-    rows_of = x.q if held else x
-    _require_cuda(rows_of)
-    dtype, dev = x.dtype, rows_of.device
+    xr = x.q if held else x
+    _require_cuda(xr)
+    dtype, dev, shape = x.dtype, xr.device, xr.shape
     if dtype not in _DTYPE_CODE:
         raise TypeError(f"unsupported dtype {dtype}")
-    if epilogue not in _TAILS:
+    tail = _TAILS.get(epilogue)
+    if tail is None:
         raise ValueError(f"unknown epilogue {epilogue}")
     if type(weight) is not Int8Rows:
         raise TypeError("weight must be Int8Rows, as quantize_rows() makes them")
-    if rows_of.dim() == 2:
+    if len(shape) == 2:
         x3 = Int8Rows(x.q[None], x.scale[None], dtype) if held else x[None]
         return linear_int8(x3, weight, bias, epilogue, None if residual is None else residual[None], gate,
                            None if out is None else out[None], tile, max_ctas)[0]
     w, w_scale = weight.q, weight.scale
-    if rows_of.dim() != 3 or w.dim() != 2:
+    if len(shape) != 3 or w.dim() != 2:
         raise ValueError("x must be (B, S, K) or (rows, K), weight (N, K)")
-    (B, S, k), (n, kw) = rows_of.shape, w.shape
-    if k != kw or k == 0 or n == 0 or w.dtype != torch.int8 or w_scale.dtype != torch.float32 or w_scale.shape != (n,) or \
-            not w_scale.is_contiguous() or w.device != dev or w_scale.device != dev:
+    (B, S, k), (n, kw), (sb, ss, sk), (wn, wk) = shape, w.shape, xr.stride(), w.stride()
+    m, pitch, w_ptr = B * S, (k + 15) & ~15, w.data_ptr()
+    if k != kw or k == 0 or n == 0 or w.dtype != torch.int8 or w.device != dev or w_scale.dtype != torch.float32 or \
+            w_scale.device != dev or w_scale.shape != (n,) or not w_scale.is_contiguous():
         raise ValueError("weight must be (N, K) int8 with N contiguous fp32 scales, on x's device")
-    if (w.stride(1) != 1 and k != 1) or (w.stride(0) % 16 and n != 1) or w.data_ptr() % 16:
+    if (wk != 1 and k != 1) or (wn % 16 and n != 1) or w_ptr % 16:
         raise ValueError("weight rows must be contiguous and start on 16-byte boundaries, as quantize_rows() lays them out")
-    if held:
-        if x.q.dtype != torch.int8 or x.scale.dtype != torch.float32 or x.scale.shape != (B, S) or x.scale.device != dev:
-            raise ValueError("x must be int8 with a fp32 scale for each row, on one device")
-        if (x.q.stride(2) != 1 and k != 1) or (x.q.stride(1) % 16 and S != 1) or (x.q.stride(0) % 16 and B != 1) or x.q.data_ptr() % 16:
-            raise ValueError("x's rows must be contiguous and start on 16-byte boundaries, as quantize_rows() lays them out")
-    elif x.stride(2) != 1 and k != 1:
+    if sk != 1 and k != 1:
         raise ValueError("x must have contiguous K")
+    if held:
+        scale = x.scale
+        if xr.dtype != torch.int8 or scale.dtype != torch.float32 or scale.shape != (B, S) or scale.device != dev:
+            raise ValueError("x must be int8 with a fp32 scale for each row, on one device")
+        if (ss % 16 and S != 1) or (sb % 16 and B != 1) or xr.data_ptr() % 16:
+            raise ValueError("x's rows must start on 16-byte boundaries, as quantize_rows() lays them out")
     if bias is not None and (bias.numel() != n or not bias.is_contiguous() or bias.dtype != dtype or bias.device != dev):
         raise ValueError("bias must be N contiguous elements of x's dtype, on its device")
-    gated = epilogue == "gate_residual"
+    gated = tail == _C.GEMM_BIAS_GATE_RESIDUAL
     if gated:
         if residual is None or gate is None:
             raise ValueError("the gate_residual epilogue needs residual and gate")
@@ -1050,32 +1066,35 @@ def linear_int8(x, weight, bias=None, epilogue="bias", residual=None, gate=None,
         if gate.shape != (B, n) or (gate.stride(1) != 1 and n != 1) or gate.dtype != dtype or gate.device != dev:
             raise ValueError("gate must be (B, N) of x's dtype, on its device")
     if out is None:
-        out = torch.empty((B, S, n), dtype=dtype, device=dev)
-    elif out.shape != (B, S, n) or out.dtype != dtype or out.device != dev or (out.stride(2) != 1 and n != 1):
-        raise ValueError("out does not match (B, S, N), x's dtype or its device")
+        out, so = w.new_empty((B, S, n), dtype=dtype), n
+    else:
+        if out.shape != (B, S, n) or out.dtype != dtype or out.device != dev or (out.stride(2) != 1 and n != 1):
+            raise ValueError("out does not match (B, S, N), x's dtype or its device")
+        so = out.stride(1)
     if B > 1 and not (_even_rows(out) and (not gated or _even_rows(residual)) and
-                      (not held or (_even_rows(x.q) and x.scale.is_contiguous()))):
+                      (not held or (sb == S * ss and scale.is_contiguous()))):
         for b in range(B):  # a slice of the rows of every entry: one launch per entry
             xb = Int8Rows(x.q[b:b + 1], x.scale[b:b + 1], dtype) if held else x[b:b + 1]
             linear_int8(xb, weight, bias, epilogue, residual[b:b + 1] if gated else None, gate[b:b + 1] if gated else None,
                         out[b:b + 1], tile, max_ctas)
         return out
-    m = B * S
     if m == 0:
         return out
     a = _C.Int8LinearArgs()
-    a.dtype, a.epilogue, a.m, a.n, a.k = _DTYPE_CODE[dtype], _TAILS[epilogue], m, n, k
+    a.dtype, a.epilogue, a.m, a.n, a.k = _DTYPE_CODE[dtype], tail, m, n, k
     if held:
-        q, scale = x.q, x.scale if x.scale.is_contiguous() else x.scale.contiguous()
-    else:
-        own = _empty_int8_rows((B, S), k, dev, dtype)
-        q, scale = own.q, own.scale
-        a.x, a.x_rows_per_batch, a.x_batch_stride, a.x_row_stride = x.data_ptr(), S, x.stride(0), x.stride(1)
-    a.a, a.a_scale, a.lda = q.data_ptr(), scale.data_ptr(), q.stride(1) if S > 1 or not held else (k + 15) & ~15
-    a.w, a.ldw, a.w_scale = w.data_ptr(), w.stride(0) if n > 1 else (k + 15) & ~15, w_scale.data_ptr()
+        if not scale.is_contiguous():
+            scale = scale.contiguous()
+        a.a, a.a_scale, a.lda = xr.data_ptr(), scale.data_ptr(), ss if S > 1 else pitch
+    else:  # the rows in 8 bits and their scales behind them: scratch of the call
+        scratch = w.new_empty(m * (pitch + 4))
+        a.a = a.a_scale = scratch.data_ptr()
+        a.a_scale += m * pitch
+        a.x, a.lda, a.x_rows_per_batch, a.x_batch_stride, a.x_row_stride = xr.data_ptr(), pitch, S, sb, ss
+    a.w, a.ldw, a.w_scale = w_ptr, wn if n > 1 else pitch, w_scale.data_ptr()
     if bias is not None:
         a.bias = bias.data_ptr()
-    a.out, a.ldo = out.data_ptr(), out.stride(1) if m > 1 else n
+    a.out, a.ldo = out.data_ptr(), so if m > 1 else n
     if gated:
         a.residual, a.ldr = residual.data_ptr(), residual.stride(1) if m > 1 else n
         a.gate, a.gate_batch_stride, a.rows_per_batch = gate.data_ptr(), gate.stride(0), S
@@ -1090,23 +1109,27 @@ def linear_int8(x, weight, bias=None, epilogue="bias", residual=None, gate=None,
 def _image_rows(x):
     """A channels-last image as (batch, rows, channels, batch stride, row stride): (B, S, C), or (B, C, H, W) / (B, C, T, H, W)
     with the channels contiguous and the pixels evenly strided."""
-    if x.dim() not in (3, 4, 5):
+    shape, strides = x.shape, x.stride()
+    if len(shape) == 3:
+        (B, rows, C), (sb, row, sc) = shape, strides
+        return _checked_rows(B, rows, C, sb, row, sc)
+    if len(shape) not in (4, 5):
         raise ValueError("expected (B, S, C), or (B, C, H, W) or (B, C, T, H, W) in channels-last layout")
-    v = x if x.dim() == 3 else x.movedim(1, -1)
-    B, C = v.shape[0], v.shape[-1]
-    rows, stride = 1, None
-    for n, s in zip(reversed(v.shape[1:-1]), reversed(v.stride()[1:-1])):
-        if n != 1 and stride is None:
-            rows, stride = n, s
-        elif n != 1 and s == rows * stride:
+    rows, row = shape[-1], strides[-1]
+    for n, s in zip(shape[-2:1:-1], strides[-2:1:-1]):
+        if n != 1:
+            if rows == 1:
+                row = s
+            elif s != rows * row:
+                raise ValueError("pixels must be evenly strided (channels-last layout)")
             rows *= n
-        elif n != 1:
-            raise ValueError("pixels must be evenly strided (channels-last layout)")
-    if C != 1 and v.stride(-1) != 1:
+    return _checked_rows(shape[0], rows, shape[1], strides[0], row, strides[1])
+
+
+def _checked_rows(B, rows, C, sb, row, sc):
+    if C != 1 and sc != 1:
         raise ValueError("channels must be contiguous (channels-last layout)")
-    if x.numel() == 0:
-        rows = 0
-    return B, rows, C, v.stride(0) if B > 1 else 0, C if stride is None else stride
+    return B, rows, C, sb if B > 1 else 0, row if rows > 1 else C
 
 
 _ACTS = {None: _C.ACT_NONE, "silu": _C.ACT_SILU}
@@ -1117,20 +1140,41 @@ def _group_norm_scratch(batch, rows, channels, groups):
     return _C.lib().hdit_group_norm_scratch(batch, rows, channels, groups)
 
 
-def _group_norm_args(x, groups, weight, bias, act):
+def _group_norm_args(x, groups, weight, bias, eps, act):
+    """The C call's arguments but for the results', and (B, rows, C)."""
     _require_cuda(x)
-    if x.dtype not in _DTYPE_CODE:
-        raise TypeError(f"unsupported dtype {x.dtype}")
+    dtype, dev = x.dtype, x.device
+    if dtype not in _DTYPE_CODE:
+        raise TypeError(f"unsupported dtype {dtype}")
     if act not in _ACTS:
         raise ValueError(f"unknown activation {act}")
     B, rows, C, sb, sr = _image_rows(x)
     groups = int(groups)
     if groups < 1 or C % groups:
         raise ValueError("channels must be a multiple of groups")
+    a = _C.GroupNormArgs()
     for t in (weight, bias):
-        if t is not None and (t.dtype != x.dtype or t.shape != (C,) or not t.is_contiguous() or t.device != x.device):
+        if t is not None and (t.dtype != dtype or t.shape != (C,) or not t.is_contiguous() or t.device != dev):
             raise ValueError("weight / bias must be C contiguous elements of x's dtype, on its device")
-    return B, rows, C, sb, sr, groups
+    if weight is not None:
+        a.weight = weight.data_ptr()
+    if bias is not None:
+        a.bias = bias.data_ptr()
+    a.dtype, a.act, a.x, a.batch, a.rows, a.channels, a.groups = _DTYPE_CODE[dtype], _ACTS[act], x.data_ptr(), B, rows, C, groups
+    a.x_batch_stride, a.x_row_stride, a.eps = sb, sr, eps
+    return a, B, rows, C
+
+
+def _group_norm_run(entry, a, x):
+    dev = x.device
+    need = _group_norm_scratch(a.batch, a.rows, a.channels, a.groups)
+    if need:
+        scratch = x.new_empty(need, dtype=torch.uint8)
+        a.scratch = scratch.data_ptr()
+    with _on(dev):
+        a.stream = _stream_ptr(dev)
+        _C.check(entry(ctypes.byref(a)))
+    _count(2 if need else 1)
 
 
 def group_norm(x, groups, weight=None, bias=None, eps=1e-6, act=None, out=None):
@@ -1138,35 +1182,32 @@ def group_norm(x, groups, weight=None, bias=None, eps=1e-6, act=None, out=None):
     torch's channels_last / channels_last_3d layout (channels contiguous, pixels evenly strided), or (B, S, C); C a multiple of
     8 and of `groups`, at most 4096. weight, bias: (C,) or None. Returns a tensor of x's shape in the same layout; `out` may be
     x."""
-    B, rows, C, sb, sr, groups = _group_norm_args(x, groups, weight, bias, act)
+    a, B, rows, C = _group_norm_args(x, groups, weight, bias, eps, act)
     if out is None:
-        out = torch.empty_like(x) if x.dim() == 3 else \
-            torch.empty((B, *x.shape[2:], C), dtype=x.dtype, device=x.device).movedim(-1, 1)
-    if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
-        raise ValueError("out does not match x")
-    _, _, _, osb, osr = _image_rows(out)
-    scratch = torch.empty(_group_norm_scratch(B, rows, C, groups), dtype=torch.uint8, device=x.device)
-    with _on(x.device):
-        _C.check(_C.lib().hdit_group_norm(_DTYPE_CODE[x.dtype], x.data_ptr(), weight.data_ptr() if weight is not None else None,
-                                          bias.data_ptr() if bias is not None else None, out.data_ptr(), scratch.data_ptr(), B,
-                                          rows, C, groups, sb, sr, osb, osr, eps, _ACTS[act], _stream_ptr(x.device)))
-    if B * rows:
-        _count(2)
+        if a.x_row_stride == C and (B == 1 or a.x_batch_stride == rows * C):  # dense: the same strides
+            out = torch.empty_like(x)
+            a.out_batch_stride, a.out_row_stride = a.x_batch_stride, C
+        else:
+            out = x.new_empty(x.shape) if x.dim() == 3 else x.new_empty((B, *x.shape[2:], C)).movedim(-1, 1)
+            a.out_batch_stride, a.out_row_stride = rows * C, C
+    else:
+        if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
+            raise ValueError("out does not match x")
+        _, _, _, a.out_batch_stride, a.out_row_stride = _image_rows(out)
+    if B * rows == 0:
+        return out
+    a.out = out.data_ptr()
+    _group_norm_run(_C.lib().hdit_group_norm, a, x)
     return out
 
 
 def group_norm_int8(x, groups, weight=None, bias=None, eps=1e-6, act=None):
     """group_norm() with its rows (all channels of a pixel) in 8 bits, see quantize_rows(); nothing is rounded to 16 bits in
     between. Returns Int8Rows (B, pixels, C), what linear_int8() takes."""
-    B, rows, C, sb, sr, groups = _group_norm_args(x, groups, weight, bias, act)
-    out = _empty_int8_rows((B, rows), C, x.device, x.dtype)
-    scratch = torch.empty(_group_norm_scratch(B, rows, C, groups), dtype=torch.uint8, device=x.device)
-    with _on(x.device):
-        _C.check(_C.lib().hdit_group_norm_int8(_DTYPE_CODE[x.dtype], x.data_ptr(),
-                                               weight.data_ptr() if weight is not None else None,
-                                               bias.data_ptr() if bias is not None else None, out.q.data_ptr(),
-                                               out.scale.data_ptr(), scratch.data_ptr(), B, rows, C, groups, sb, sr,
-                                               out.q.stride(1), eps, _ACTS[act], _stream_ptr(x.device)))
-    if B * rows:
-        _count(2)
+    a, B, rows, C = _group_norm_args(x, groups, weight, bias, eps, act)
+    out = _empty_int8_rows(x, (B, rows), C)
+    if B * rows == 0:
+        return out
+    a.out, a.out_scale, a.out_row_stride = out.q.data_ptr(), out.scale.data_ptr(), (C + 15) & ~15
+    _group_norm_run(_C.lib().hdit_group_norm_int8, a, x)
     return out

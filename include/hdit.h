@@ -601,22 +601,33 @@ HDIT_API int hdit_int8_linear(const hdit_int8_linear_args* args);
  * (batch, rows, channels) with contiguous channels, any batch and row strides (elements); channels a multiple of 8 and of
  * groups, at most 4096; weight and bias `channels` elements each or NULL (1 and 0). scratch: hdit_group_norm_scratch() bytes,
  * 8-byte aligned, of which nothing has to be kept before or after the call; calls that may overlap need one each. `out` may be x.
- * hdit_group_norm_int8 writes each row (all channels of a pixel) as an 8-bit row instead, rows of all images in order.
+ * hdit_group_norm_int8 writes each row (all channels of a pixel) as an 8-bit row instead: out is int8, rows of all images in
+ * order out_row_stride bytes apart, out_scale their scales.
  *
  * The reference takes the norm of its image decoder from diffusers and shards it over ranks
  * (hetu_dit/model_executor/vae_executor/models/layers/normalization.py:52-188), NCHW.
  */
 enum { HDIT_ACT_NONE = 0, HDIT_ACT_SILU = 1 };
 
+typedef struct hdit_group_norm_args {
+  int32_t dtype;
+  int32_t act;
+  const void* x;
+  const void* weight;
+  const void* bias;
+  void* out;
+  float* out_scale; /* hdit_group_norm_int8 only */
+  void* scratch;
+  int64_t batch, rows, channels, groups;
+  int64_t x_batch_stride, x_row_stride, out_batch_stride, out_row_stride;
+  void* stream;
+  float eps;
+  int32_t reserved0;
+} hdit_group_norm_args;
+
 HDIT_API int64_t hdit_group_norm_scratch(int64_t batch, int64_t rows, int64_t channels, int64_t groups);
-HDIT_API int hdit_group_norm(int32_t dtype, const void* x, const void* weight, const void* bias, void* out, void* scratch,
-                             int64_t batch, int64_t rows, int64_t channels, int64_t groups, int64_t x_batch_stride,
-                             int64_t x_row_stride, int64_t out_batch_stride, int64_t out_row_stride, float eps, int32_t act,
-                             void* stream);
-HDIT_API int hdit_group_norm_int8(int32_t dtype, const void* x, const void* weight, const void* bias, void* q, float* q_scale,
-                                  void* scratch, int64_t batch, int64_t rows, int64_t channels, int64_t groups,
-                                  int64_t x_batch_stride, int64_t x_row_stride, int64_t q_row_stride, float eps, int32_t act,
-                                  void* stream);
+HDIT_API int hdit_group_norm(const hdit_group_norm_args* args);
+HDIT_API int hdit_group_norm_int8(const hdit_group_norm_args* args);
 
 #ifdef __cplusplus
 }

@@ -119,11 +119,21 @@ def test_the_library_refuses_by_itself():
     ln = lambda **k: real.hdit_ln_modulate_int8(*{**dict(dtype=0, x=q, sh=q, sc=q, q=q, s=s, rows=4, dim=32, rpb=4, xb=0, xr=32, qr=32, mb=32, eps=1e-6, st=none), **k}.values())  # noqa: E731
     for bad in (dict(dim=20), dict(dim=8200, qr=8208), dict(sh=none), dict(sc=ctypes.c_void_p(4097))):
         assert ln(**bad) in (_C.HDIT_ERR_BAD_ARG, _C.HDIT_ERR_SHAPE), bad
-    gn = lambda **k: real.hdit_group_norm(*{**dict(dtype=0, x=q, w=none, b=none, out=q, scratch=q, batch=1, rows=4, c=64, g=8, xb=0, xr=64, ob=0, orow=64, eps=1e-6, act=0, st=none), **k}.values())  # noqa: E731
-    for bad in (dict(dtype=2), dict(batch=-1), dict(c=60), dict(g=7), dict(g=0), dict(c=4104), dict(act=2), dict(x=none), dict(scratch=none),
-                dict(batch=65536), dict(rows=1 << 31)):
-        assert gn(**bad) in (_C.HDIT_ERR_BAD_ARG, _C.HDIT_ERR_SHAPE, _C.HDIT_ERR_TOO_LARGE), bad
-    assert gn(batch=0) == 0 and gn(rows=0) == 0
+    def gn(entry=real.hdit_group_norm, **change):
+        a = _C.GroupNormArgs()
+        fields = dict(dtype=0, act=0, x=4096, out=4096, out_scale=4096, scratch=4096, batch=1, rows=4, channels=64, groups=8, x_row_stride=64,
+                      out_row_stride=64, eps=1e-6)
+        for name, v in {**fields, **change}.items():
+            setattr(a, name, v)
+        return entry(ctypes.byref(a))
+
+    for entry in (real.hdit_group_norm, real.hdit_group_norm_int8):
+        for bad in (dict(dtype=2), dict(batch=-1), dict(channels=60), dict(groups=7), dict(groups=0), dict(channels=4104), dict(act=2), dict(x=0),
+                    dict(out=0), dict(batch=65536), dict(rows=1 << 31), dict(scratch=4100)):
+            assert gn(entry, **bad) in (_C.HDIT_ERR_BAD_ARG, _C.HDIT_ERR_SHAPE, _C.HDIT_ERR_TOO_LARGE), bad
+        assert gn(entry, batch=0) == 0 and gn(entry, rows=0) == 0 and entry(None) == _C.HDIT_ERR_BAD_ARG
+    for bad in (dict(out=4104), dict(out_row_stride=72), dict(out_row_stride=48), dict(out_scale=0)):
+        assert gn(real.hdit_group_norm_int8, **bad) in (_C.HDIT_ERR_BAD_ARG, _C.HDIT_ERR_SHAPE), bad
 
     def linear(**change):
         a = _C.Int8LinearArgs()
