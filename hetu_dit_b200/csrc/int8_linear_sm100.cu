@@ -16,6 +16,7 @@
 
 #include "gemm_common.cuh"
 #include "host_common.h"
+#include "int8_linear.h"
 
 namespace hdit {
 namespace {
@@ -446,10 +447,10 @@ __global__ void __launch_bounds__(Int8Cfg<BN, PAIR, EPI>::kThreads, 1) int8_line
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const uint32_t* a4 = &r[j * 8 + h * 4];
-            v[h * 4 + 0] = fmaf(static_cast<float>(static_cast<int>(a4[0])) * my_scale, s4[h].x, b4[h].x);
-            v[h * 4 + 1] = fmaf(static_cast<float>(static_cast<int>(a4[1])) * my_scale, s4[h].y, b4[h].y);
-            v[h * 4 + 2] = fmaf(static_cast<float>(static_cast<int>(a4[2])) * my_scale, s4[h].z, b4[h].z);
-            v[h * 4 + 3] = fmaf(static_cast<float>(static_cast<int>(a4[3])) * my_scale, s4[h].w, b4[h].w);
+            v[h * 4 + 0] = int8_value(static_cast<int>(a4[0]), my_scale, s4[h].x, b4[h].x);
+            v[h * 4 + 1] = int8_value(static_cast<int>(a4[1]), my_scale, s4[h].y, b4[h].y);
+            v[h * 4 + 2] = int8_value(static_cast<int>(a4[2]), my_scale, s4[h].z, b4[h].z);
+            v[h * 4 + 3] = int8_value(static_cast<int>(a4[3]), my_scale, s4[h].w, b4[h].w);
           }
           if constexpr (EPI == HDIT_GEMM_BIAS_GELU_TANH) {
 #pragma unroll
@@ -621,6 +622,8 @@ extern "C" int hdit_int8_linear(const hdit_int8_linear_args* a) {
   if (gated && (a->residual == nullptr || a->gate == nullptr || a->rows_per_batch <= 0))
     return set_error(HDIT_ERR_BAD_ARG, "the gated-residual epilogue needs residual, gate and rows_per_batch > 0");
   if (gated && a->ldr < a->n) return set_error(HDIT_ERR_SHAPE, "rows of residual overlap");
+  if (a->x != nullptr && (a->x_rows_per_batch <= 0 || (reinterpret_cast<uintptr_t>(a->x) & 1) != 0))
+    return set_error(HDIT_ERR_BAD_ARG, "x needs x_rows_per_batch > 0 and the alignment of its elements");
   Int8Params p;
   memset(&p, 0, sizeof(p));
   p.M = static_cast<int>(a->m);
@@ -641,13 +644,16 @@ extern "C" int hdit_int8_linear(const hdit_int8_linear_args* a) {
   p.tma_residual = gated && whole(a->residual, a->ldr);
   p.status = device_status_ptr();
   if (p.status == nullptr) return HDIT_ERR_CUDA;
-  if (a->x != nullptr) {
+  if (a->tile < 0 || a->tile > 5) return set_error(HDIT_ERR_BAD_ARG, "tile must be 0 (choose) to 5");
+  if (a->tile == 5 && !int8_linear_few_takes(a)) return set_error(HDIT_ERR_SHAPE, "too many rows, or too long ones, for the kernel for a few rows");
+  const bool few = a->tile == 5 || (a->tile == 0 && int8_linear_few_takes(a));
+  if (a->x != nullptr && !(few && int8_linear_few_quantizes(a))) {
     // 16-bit rows: into 8 bits first, in the caller's a / a_scale
     const int rc = hdit_quantize_rows(a->dtype, a->x, const_cast<void*>(a->a), const_cast<float*>(a->a_scale), a->m, a->k, a->x_rows_per_batch,
                                       a->x_batch_stride, a->x_row_stride, a->lda, a->stream);
     if (rc != HDIT_OK) return rc;
   }
-  if (a->tile < 0 || a->tile > 4) return set_error(HDIT_ERR_BAD_ARG, "tile must be 0 (choose) to 4");
+  if (few) return int8_linear_few(a);
   int tile = a->tile;
   if (tile == 0) {
     // Fewest waves, each weighted by a tile's time relative to 128 x 128 of output per SM

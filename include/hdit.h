@@ -537,8 +537,8 @@ HDIT_API int hdit_linear_group(const hdit_linear_group_args* args);
  * 8-bit rows: a row y of values as signed integers q with one fp32 scale s,
  *   s = max|y| / 127,   q = y / s to the nearest integer, ties to even (so |q| <= 127 and y = q s up to half a step).
  * A row whose largest magnitude is below 2^-100 counts as zero (s = 0, q = 0). A row that holds an infinity or NaN gets s = NaN and
- * q = 0: what is computed from it is NaN. Memory: rows of `dim` bytes, 16-byte aligned, their stride a multiple of 16; bytes
- * behind a row's end are neither read nor written. (The reference has no 8-bit path.)
+ * q = 0: what is computed from it is NaN. Memory: rows of `dim` bytes, 16-byte aligned, their stride a multiple of 16; what
+ * lies behind a row's end up to the next multiple of 16 bytes may be read, but does not count, and is not written. (The reference has no 8-bit path.)
  *
  * hdit_quantize_rows    : y = x, 16-bit storage. q is exact for these inputs, borders between two integers included. Row r of x
  *                         starts at (r / rows_per_batch) * x_batch_stride + (r % rows_per_batch) * x_row_stride elements; any
@@ -562,8 +562,8 @@ HDIT_API int hdit_ln_modulate_int8(int32_t dtype, const void* x, const void* shi
  * scratch that hdit_quantize_rows fills from these 16-bit rows first (x_rows_per_batch, x_batch_stride, x_row_stride as there).
  * bias, gate, residual and out are 16-bit of `dtype`, any strides that keep rows of residual and out apart; m, n and k need not
  * be multiples of anything; rows_per_batch >= 1 (HDIT_GEMM_BIAS_GATE_RESIDUAL only). `out` may alias `residual`.
- * tile: 0 = the library chooses, 1 = 128 x 128 tiles, 2, 3, 4 = 256 x 128, 256 x 192, 256 x 256 on a CTA pair. max_ctas: 0 = one
- * persistent CTA per SM.
+ * tile: 0 = the library chooses, 1 = 128 x 128 tiles, 2, 3, 4 = 256 x 128, 256 x 192, 256 x 256 on a CTA pair, 5 = the kernel for
+ * a few rows (at most 8, and 160 KB of them); all give the same bits. max_ctas: 0 = one persistent CTA per SM.
  */
 #define HDIT_INT8_MAX_K 131072 /* 127 * 127 * k < 2^31 */
 

@@ -224,6 +224,20 @@ def test_every_tile_gives_the_same_bits(B, S, K, N, epilogue, tile):
         assert torch.equal(first, kernels.linear_int8(x8, w, b, epilogue, residual=res, gate=gate, tile=tile, max_ctas=ctas))
 
 
+@pytest.mark.parametrize("epilogue", EPILOGUES)
+@pytest.mark.parametrize("B,S,K,N", [(1, 1, 1536, 4608), (2, 1, 72, 40), (1, 3, 1000, 17), (2, 2, 4096, 160), (1, 5, 63, 100), (1, 8, 65, 33),
+                                     (7, 1, 700, 264), (2, 4, 2048, 96), (1, 8, 520, 1001), (1, 4, 20000, 50), (1, 2, 70000, 20)])
+def test_few_rows_give_the_bits_of_a_tile(B, S, K, N, epilogue):
+    from hetu_dit_b200 import kernels
+    x, w, b, res, gate = _layer(B, S, K, N, torch.float16, S + N)
+    x8 = kernels.quantize_rows(x)
+    tile = kernels.linear_int8(x8, w, b, epilogue, residual=res, gate=gate, tile=1)
+    want, tol = _tail64(x8, w, b, epilogue, res, gate, torch.float16)
+    _within(tile, want, tol)
+    for rows in (x, x8):
+        assert torch.equal(tile, kernels.linear_int8(rows, w, b, epilogue, residual=res, gate=gate, tile=5))
+
+
 def test_linear_int8_sums_are_exact_at_the_largest_k():
     """Rows of the largest and smallest integers only: a sum of 127 * 127 * 131072 fits 32 bits."""
     from hetu_dit_b200 import kernels
