@@ -340,7 +340,7 @@ def _declare(lib):
     lib.hdit_int8_linear.restype = ctypes.c_int
     lib.hdit_int8_linear.argtypes = [ctypes.POINTER(Int8LinearArgs)]
     lib.hdit_group_norm_scratch.restype = ctypes.c_int64
-    lib.hdit_group_norm_scratch.argtypes = [ctypes.c_int64] * 4
+    lib.hdit_group_norm_scratch.argtypes = [ctypes.c_int64] * 4 + [ctypes.c_int32]
     lib.hdit_group_norm.restype = ctypes.c_int
     lib.hdit_group_norm.argtypes = [ctypes.POINTER(GroupNormArgs)]
     lib.hdit_group_norm_int8.restype = ctypes.c_int

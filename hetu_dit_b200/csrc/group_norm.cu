@@ -3,15 +3,18 @@
 //   y[b, r, c] = (x[b, r, c] - mean[b, g]) / sqrt(var[b, g] + eps) * weight[c] + bias[c],   g = c / (channels / groups)
 // over rows r (pixels) and the channels of a group; biased variance.
 //
-// Two launches of one CTA per SM. The first one reads x once: a CTA takes a strip of rows of one image, each thread eight fixed
-// channels, and leaves {mean, sum of squared distances from it} per group and strip. Sums are taken relative to a value of the
-// strip's first row, so that a mean far from zero costs no digits. The second one joins the strips (Chan's formula) and reads x
-// again, each strip from its end to its start: what the first launch read last is still in L2. Every CTA joins the strips of
-// its image by itself; with four strips per SM, read eight at a time by a thread, that alone took 3 us.
+// Two launches of one CTA per SM. The first one reads x once: a strip (a CTA) takes every strips-th tile of rows of an image,
+// each thread eight fixed channels, and leaves {mean, sum of squared distances from it} per group and strip. Sums are taken
+// relative to a value of the strip's first row, so that a mean far from zero costs no digits. The second one joins the strips
+// (Chan's formula) and reads x again from its end to its start: what the first launch read last is still in L2. Every CTA joins
+// the strips of its image by itself; with four strips per SM, read eight at a time by a thread, that alone took 3 us.
+// All CTAs work on neighbouring tiles at a time: with one stretch of rows each, 1024 x 1024 x 128 took 148 us (4.8 TB/s of
+// traffic in both launches), 143 like this.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include "gemm_common.cuh"
 #include "host_common.h"
 #include "int8_rows.cuh"
 #include "ptx_sm100.cuh"
@@ -20,8 +23,23 @@ namespace hdit {
 namespace {
 
 constexpr int kMaxChannels = 4096;
+constexpr int kAhead = 6;         // rows of a thread in flight
+constexpr int kClusterThreads = 256;  // two CTAs to an SM
 constexpr int kGnThreads = 512;  // what a CTA does beside its rows costs every warp some hundred instructions
-constexpr int kAhead = 6;        // rows of a thread in flight
+
+// How the rows of an image lie in tiles of `lanes` rows and the tiles in strips: strip k has tiles k, k + strips, ...; the last
+// tile of all is `missing` rows short. Worked out on the host: a thread's 64-bit divisions cost more than its sums.
+struct Strips {
+  int strips, lanes;
+  int tiles, longer;  // of a strip; the first `longer` strips have one more
+  int last, missing;  // the strip with the last tile
+  __host__ __device__ int tiles_of(int k) const { return tiles + (k < longer ? 1 : 0); }
+  __host__ __device__ int rows_of(int k) const { return tiles_of(k) * lanes - (k == last ? missing : 0); }
+  // rows of a lane of strip k
+  __device__ __forceinline__ int rows_of_lane(int k, int lane) const { return tiles_of(k) - (k == last && lane >= lanes - missing ? 1 : 0); }
+  __device__ __forceinline__ long long first(int k, int lane) const { return static_cast<long long>(k) * lanes + lane; }
+  __device__ __forceinline__ long long step() const { return static_cast<long long>(strips) * lanes; }
+};
 
 struct GnParams {
   const uint16_t* x;
@@ -32,8 +50,8 @@ struct GnParams {
   float* q_scale;
   float2* partial;  // (batch, strips, groups): mean, sum of squared distances from it
   long long rows, x_batch_stride, x_row_stride, out_batch_stride, out_row_stride;  // q: out_row_stride only, rows of all images
-  long long strip_rows;
-  int strips, channels, groups, act;
+  Strips strips;
+  int channels, groups, act, slab;
   float eps;
   bool vec;
 };
@@ -80,20 +98,18 @@ __device__ __forceinline__ void walk_rows(const uint16_t* x, int c, int channels
     if (at + k < count) use(next[k], at + k);
 }
 
-template <bool FP16, bool VEC>
-__global__ void __launch_bounds__(kGnThreads, 1) group_norm_stats_kernel(const __grid_constant__ GnParams p) {
-  grid_dependency_release();
-  grid_dependency_wait();
-  extern __shared__ float smem[];  // [lanes][channels] sums, then the same of squares
-  const int chunks = p.channels / 8;
-  const int lanes = kGnThreads / chunks;  // rows at a time
+// Statistics of strip k of an image of `rows` rows of `channels` channels at `x`. A thread passes its eight channels of every lanes-th
+// row to keep(raw, index). smem: [lanes][channels] sums, then the same of squares. put(group, {mean, sum of squared distances from it}).
+template <int THREADS, bool FP16, bool VEC, typename K, typename P>
+__device__ __forceinline__ void strip_stats(const uint16_t* x, long long row_stride, const Strips& strips, int strip, int channels, int per, float* smem, K keep,
+                                            P put) {
+  const int chunks = channels / 8;
+  const int lanes = strips.lanes;  // rows at a time
   const int lane = threadIdx.x / chunks, c = (threadIdx.x - lane * chunks) * 8;
-  const long long r0 = static_cast<long long>(blockIdx.x) * p.strip_rows;
-  const int rows = static_cast<int>(r0 + p.strip_rows < p.rows ? p.strip_rows : p.rows - r0);
-  const uint16_t* xs = p.x + blockIdx.y * p.x_batch_stride + r0 * p.x_row_stride;
+  const uint16_t* xs = x + static_cast<long long>(strip) * lanes * row_stride;  // the strip's first row
   if (lane < lanes) {
     float s[8], ss[8], pivot[8];
-    const uint4 first = int8_load8(xs, c, p.channels, VEC);
+    const uint4 first = int8_load8(xs, c, channels, VEC);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float2 v = int8_unpack2<FP16>(reinterpret_cast<const uint32_t*>(&first)[i]);
@@ -101,8 +117,8 @@ __global__ void __launch_bounds__(kGnThreads, 1) group_norm_stats_kernel(const _
       pivot[2 * i + 1] = v.y;
       s[2 * i] = s[2 * i + 1] = ss[2 * i] = ss[2 * i + 1] = 0.f;
     }
-    const int count = rows > lane ? (rows - lane + lanes - 1) / lanes : 0;
-    walk_rows<VEC>(xs + lane * p.x_row_stride, c, p.channels, count, lanes * p.x_row_stride, [&](const uint4& raw, int) {
+    walk_rows<VEC>(x + strips.first(strip, lane) * row_stride, c, channels, strips.rows_of_lane(strip, lane), strips.step() * row_stride, [&](const uint4& raw, int at) {
+      keep(raw, at);
       const uint32_t* u = reinterpret_cast<const uint32_t*>(&raw);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -114,10 +130,10 @@ __global__ void __launch_bounds__(kGnThreads, 1) group_norm_stats_kernel(const _
         ss[2 * i + 1] = fmaf(d1, d1, ss[2 * i + 1]);
       }
     });
-    float4* to = reinterpret_cast<float4*>(smem + lane * p.channels + c);
+    float4* to = reinterpret_cast<float4*>(smem + lane * channels + c);
     to[0] = make_float4(s[0], s[1], s[2], s[3]);
     to[1] = make_float4(s[4], s[5], s[6], s[7]);
-    to = reinterpret_cast<float4*>(smem + (lanes + lane) * p.channels + c);
+    to = reinterpret_cast<float4*>(smem + (lanes + lane) * channels + c);
     to[0] = make_float4(ss[0], ss[1], ss[2], ss[3]);
     to[1] = make_float4(ss[4], ss[5], ss[6], ss[7]);
   }
@@ -125,86 +141,100 @@ __global__ void __launch_bounds__(kGnThreads, 1) group_norm_stats_kernel(const _
   // Over the lanes: `parts` neighbouring lanes of a warp to a channel. Then per channel, in the first lane's places: the mean,
   // and the sum of squared distances from it.
   int parts = 1;
-  while (parts < 32 && parts < lanes && parts * 2 * p.channels <= kGnThreads) parts *= 2;
-  const float inv_rows = 1.f / static_cast<float>(rows);
-  for (int ch0 = 0; ch0 < p.channels; ch0 += kGnThreads / parts) {
+  while (parts < 32 && parts < lanes && parts * 2 * channels <= THREADS) parts *= 2;
+  const float n = static_cast<float>(strips.rows_of(strip)), inv_rows = 1.f / n;
+  for (int ch0 = 0; ch0 < channels; ch0 += THREADS / parts) {
     const int ch = ch0 + static_cast<int>(threadIdx.x) / parts, part = static_cast<int>(threadIdx.x) % parts;
     float a = 0.f, q = 0.f;
-    if (ch < p.channels)
+    if (ch < channels)
       for (int l = part; l < lanes; l += parts) {
-        a += smem[l * p.channels + ch];
-        q += smem[(lanes + l) * p.channels + ch];
+        a += smem[l * channels + ch];
+        q += smem[(lanes + l) * channels + ch];
       }
     a = sub_sum(a, parts);
     q = sub_sum(q, parts);
-    if (ch < p.channels && part == 0) {  // no other thread reads this channel's first lane
+    if (ch < channels && part == 0) {  // no other thread reads this channel's first lane
       const float m2 = q - a * a * inv_rows;
       smem[ch] = int8_unpack2<FP16>(xs[ch]).x + a * inv_rows;
-      smem[lanes * p.channels + ch] = m2 > 0.f ? m2 : m2 - m2;  // keeps NaN
+      smem[lanes * channels + ch] = m2 > 0.f ? m2 : m2 - m2;  // keeps NaN
     }
   }
   __syncthreads();
-  const int per = p.channels / p.groups;
-  const float n = static_cast<float>(rows), inv_per = 1.f / static_cast<float>(per);
-  float2* out = p.partial + (static_cast<long long>(blockIdx.y) * p.strips + blockIdx.x) * p.groups;
-  for_groups(p.groups, [&](int g, int sub, int n_sub) {
-    const bool live = g < p.groups;
+  const float inv_per = 1.f / static_cast<float>(per);
+  for_groups(channels / per, [&](int g, int sub, int n_sub) {
+    const bool live = g * per < channels;
     float mean = 0.f, m2 = 0.f;
     for (int k = sub; live && k < per; k += n_sub) mean += smem[g * per + k];
     mean = sub_sum(mean, n_sub) * inv_per;
     for (int k = sub; live && k < per; k += n_sub) {
       const float d = smem[g * per + k] - mean;
-      m2 += smem[lanes * p.channels + g * per + k] + n * d * d;
+      m2 += smem[lanes * channels + g * per + k] + n * d * d;
     }
     m2 = sub_sum(m2, n_sub);
-    if (live && sub == 0) out[g] = make_float2(mean, m2);
+    if (live && sub == 0) put(g, make_float2(mean, m2));
   });
 }
 
-// {mean, 1 / deviation} of every group of image b into stat[groups].
-__device__ __forceinline__ void group_norm_join(const GnParams& p, int b, float2* stat) {
-  const float2* in = p.partial + static_cast<long long>(b) * p.strips * p.groups;
-  const float per = static_cast<float>(p.channels / p.groups);
-  const float n_full = static_cast<float>(p.strip_rows) * per;
-  const float n_last = static_cast<float>(p.rows - p.strip_rows * (p.strips - 1)) * per;
-  const float total = static_cast<float>(p.rows) * per;
-  for_groups(p.groups, [&](int g, int sub, int n_sub) {
-    const bool live = g < p.groups;
-    const float base = live ? in[g].x : 0.f;
+template <bool FP16, bool VEC>
+__global__ void __launch_bounds__(kGnThreads, 1) group_norm_stats_kernel(const __grid_constant__ GnParams p) {
+  grid_dependency_release();
+  grid_dependency_wait();
+  extern __shared__ float smem[];
+  float2* out = p.partial + (static_cast<long long>(blockIdx.y) * p.strips.strips + blockIdx.x) * p.groups;
+  strip_stats<kGnThreads, FP16, VEC>(p.x + blockIdx.y * p.x_batch_stride, p.x_row_stride, p.strips, static_cast<int>(blockIdx.x), p.channels,
+                                     p.channels / p.groups, smem, [](const uint4&, int) {}, [&](int g, float2 v) { out[g] = v; });
+}
+
+// {mean, 1 / deviation} of `groups` groups from `strips` strips of an image, `per` channels to a group, into stat[groups].
+// in(strip, group): the strip's {mean, sum of squared distances from it}.
+template <typename F>
+__device__ __forceinline__ void join_strips(int groups, const Strips& strips, long long rows, int per, float eps, float2* stat, F in) {
+  const float inv_total = 1.f / (static_cast<float>(rows) * static_cast<float>(per));
+  for_groups(groups, [&](int g, int sub, int n_sub) {
+    const bool live = g < groups;
+    const float base = live ? in(0, g).x : 0.f;
     float a = 0.f, q = 0.f;
 #pragma unroll 4
-    for (int k = sub; k < (live ? p.strips : 0); k += n_sub) {
-      const float2 v = in[static_cast<long long>(k) * p.groups + g];
-      const float d = v.x - base, n = k == p.strips - 1 ? n_last : n_full;
+    for (int k = sub; k < (live ? strips.strips : 0); k += n_sub) {
+      const float2 v = in(k, g);
+      const float d = v.x - base, n = static_cast<float>(strips.rows_of(k)) * static_cast<float>(per);
       a = fmaf(n, d, a);
       q += fmaf(n * d, d, v.y);
     }
     a = sub_sum(a, n_sub);
     q = sub_sum(q, n_sub);
-    const float far = a / total;  // of the mean from the first strip's
-    const float var = q / total - far * far;
-    if (live && sub == 0) stat[g] = make_float2(base + far, rsqrtf((var > 0.f ? var : var - var) + p.eps));
+    const float far = a * inv_total;  // of the mean from the first strip's
+    const float var = q * inv_total - far * far;
+    if (live && sub == 0) stat[g] = make_float2(base + far, rsqrtf((var > 0.f ? var : var - var) + eps));
   });
 }
 
-// y = x * a + b with a = weight / deviation and b = bias - mean * a, for all channels of image blockIdx.y into shared memory:
-// `factors` holds a, then b, each first for the lower four channels of every chunk of eight, then for the upper four, so that
-// threads' 16 bytes lie side by side; behind them stand the groups' statistics.
+// y = x * a + b with a = weight / deviation and b = bias - mean * a, for each channel in shared memory: `factors` holds a, then b, each first for the lower four channels of every chunk of eight, then for the upper four, so
+// that threads' 16 bytes lie side by side.
 // Against (x - mean) * a + bias this form costs half a unit of 2^-24 of mean * a: a 16-bit x resolves the deviation only while
 // |mean| is below some 2^11 deviations, where that is under 2^-13 of the result's deviation.
 template <bool FP16>
+__device__ __forceinline__ void put_factor(int c, int chunks, float2 stat, float weight, float bias, float4* factors) {
+  const float a = stat.y * weight;
+  float* to = reinterpret_cast<float*>(factors) + (c >> 3) * 4 + ((c >> 2) & 1) * chunks * 4 + (c & 3);
+  to[0] = a;
+  to[8 * chunks] = fmaf(-stat.x, a, bias);
+}
+template <bool FP16>
+__device__ __forceinline__ float gn_weight(const GnParams& p, int c) { return p.weight != nullptr ? int8_unpack2<FP16>(p.weight[c]).x : 1.f; }
+template <bool FP16>
+__device__ __forceinline__ float gn_bias(const GnParams& p, int c) { return p.bias != nullptr ? int8_unpack2<FP16>(p.bias[c]).x : 0.f; }
+
+// All channels' factors of image blockIdx.y; the groups' statistics stand behind them.
+template <bool FP16>
 __device__ __forceinline__ void group_norm_factors(const GnParams& p, float4* factors) {
-  const int chunks = p.channels / 8, per = p.channels / p.groups;
-  float2* stat = reinterpret_cast<float2*>(factors + 4 * chunks);
-  group_norm_join(p, blockIdx.y, stat);
+  const int per = p.channels / p.groups;
+  float2* stat = reinterpret_cast<float2*>(factors + p.channels / 2);
+  const float2* in = p.partial + static_cast<long long>(blockIdx.y) * p.strips.strips * p.groups;
+  join_strips(p.groups, p.strips, p.rows, per, p.eps, stat, [&](int k, int g) { return in[static_cast<long long>(k) * p.groups + g]; });
   __syncthreads();
-  for (int c = threadIdx.x; c < p.channels; c += blockDim.x) {
-    const float2 st = stat[c / per];
-    const float a = st.y * (p.weight != nullptr ? int8_unpack2<FP16>(p.weight[c]).x : 1.f);
-    float* to = reinterpret_cast<float*>(factors) + (c >> 3) * 4 + ((c >> 2) & 1) * chunks * 4 + (c & 3);
-    to[0] = a;
-    to[8 * chunks] = fmaf(-st.x, a, p.bias != nullptr ? int8_unpack2<FP16>(p.bias[c]).x : 0.f);
-  }
+  for (int c = threadIdx.x; c < p.channels; c += kGnThreads)
+    put_factor<FP16>(c, p.channels / 8, stat[c / per], gn_weight<FP16>(p, c), gn_bias<FP16>(p, c), factors);
   __syncthreads();
 }
 
@@ -226,113 +256,193 @@ __device__ __forceinline__ uint32_t gn_pack(float lo, float hi) {
   }
 }
 
+// Eight channels of a row, normalised, to dst.
+template <bool FP16, bool SILU, bool VEC>
+__device__ __forceinline__ void apply8(const uint4& raw, const float (&a)[8], const float (&b)[8], uint16_t* dst) {
+  uint4 y = raw;
+  uint32_t* u = reinterpret_cast<uint32_t*>(&y);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float2 v = int8_unpack2<FP16>(u[k]);
+    float y0 = fmaf(v.x, a[2 * k], b[2 * k]), y1 = fmaf(v.y, a[2 * k + 1], b[2 * k + 1]);
+    if constexpr (SILU) y0 = silu(y0), y1 = silu(y1);
+    u[k] = gn_pack<FP16>(y0, y1);
+  }
+  if constexpr (VEC) {
+    *reinterpret_cast<uint4*>(dst) = y;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) dst[k] = static_cast<uint16_t>(u[k / 2] >> (16 * (k & 1)));
+  }
+}
+__device__ __forceinline__ void read_factors(const float4* factors, int chunks, int chunk, float (&a)[8], float (&b)[8]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    *reinterpret_cast<float4*>(a + 4 * h) = factors[h * chunks + chunk];
+    *reinterpret_cast<float4*>(b + 4 * h) = factors[(2 + h) * chunks + chunk];
+  }
+}
+
 template <bool FP16, bool SILU, bool VEC>
 __global__ void __launch_bounds__(kGnThreads, 1) group_norm_apply_kernel(const __grid_constant__ GnParams p) {
   grid_dependency_release();
   grid_dependency_wait();
   extern __shared__ float4 factors[];
   const int chunks = p.channels / 8;
-  const int lanes = kGnThreads / chunks;
+  const int lanes = p.strips.lanes;
   const int lane = threadIdx.x / chunks, chunk = threadIdx.x - lane * chunks, c = chunk * 8;
-  const long long r0 = static_cast<long long>(blockIdx.x) * p.strip_rows;
-  const int rows = static_cast<int>(r0 + p.strip_rows < p.rows ? p.strip_rows : p.rows - r0);
   group_norm_factors<FP16>(p, factors);
   if (lane >= lanes) return;
   float a[8], b[8];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    *reinterpret_cast<float4*>(a + 4 * h) = factors[h * chunks + chunk];
-    *reinterpret_cast<float4*>(b + 4 * h) = factors[(2 + h) * chunks + chunk];
-  }
-  // from the strip's end to its start
-  const int count = rows > lane ? (rows - lane + lanes - 1) / lanes : 0;
-  const long long out_step = lanes * p.out_row_stride;
-  uint16_t* out = p.out + blockIdx.y * p.out_batch_stride + (r0 + rows - 1 - lane) * p.out_row_stride + c;
-  walk_rows<VEC>(p.x + blockIdx.y * p.x_batch_stride + (r0 + rows - 1 - lane) * p.x_row_stride, c, p.channels, count, -lanes * p.x_row_stride,
-                 [&](const uint4& raw, int i) {
-                   uint4 y = raw;
-                   uint32_t* u = reinterpret_cast<uint32_t*>(&y);
-#pragma unroll
-                   for (int k = 0; k < 4; ++k) {
-                     const float2 v = int8_unpack2<FP16>(u[k]);
-                     float y0 = fmaf(v.x, a[2 * k], b[2 * k]), y1 = fmaf(v.y, a[2 * k + 1], b[2 * k + 1]);
-                     if constexpr (SILU) y0 = silu(y0), y1 = silu(y1);
-                     u[k] = gn_pack<FP16>(y0, y1);
-                   }
-                   uint16_t* dst = out - i * out_step;
-                   if constexpr (VEC) {
-                     *reinterpret_cast<uint4*>(dst) = y;
-                   } else {
-#pragma unroll
-                     for (int k = 0; k < 8; ++k) dst[k] = static_cast<uint16_t>(u[k / 2] >> (16 * (k & 1)));
-                   }
-                 });
+  read_factors(factors, chunks, chunk, a, b);
+  // the strip's rows from the last to the first
+  const int strip = static_cast<int>(blockIdx.x), count = p.strips.rows_of_lane(strip, lane);
+  const long long step = p.strips.step(), last = p.strips.first(strip, lane) + (count - 1) * step, out_step = step * p.out_row_stride;
+  uint16_t* out = p.out + blockIdx.y * p.out_batch_stride + last * p.out_row_stride + c;
+  walk_rows<VEC>(p.x + blockIdx.y * p.x_batch_stride + last * p.x_row_stride, c, p.channels, count, -step * p.x_row_stride,
+                 [&](const uint4& raw, int i) { apply8<FP16, SILU, VEC>(raw, a, b, out - i * out_step); });
 }
 
-// The rows in 8 bits: TEAM threads hold a row of at most TEAM * NCH * 8 channels and have the next one on its way; factors of
-// all channels in shared memory.
-template <bool FP16, bool SILU, int TEAM, int NCH, bool VEC>
+// A row in 8 bits, held by a team as NCH chunks of eight channels a thread.
+template <bool FP16, bool SILU, int TEAM, int NCH, int THREADS>
+__device__ __forceinline__ void row_to_int8(const GnParams& p, const Team<TEAM, THREADS>& team, int turn, const uint4 (&raw)[NCH], const float4* factors,
+                                            int c0, long long row, bool live) {
+  const int chunks = p.channels / 8;
+  float y[NCH][8];
+  float top = 0.f;
+#pragma unroll
+  for (int k = 0; k < NCH; ++k) {
+    const int c = c0 + k * TEAM * 8;
+    if (c >= p.channels) continue;
+    const uint32_t* u = reinterpret_cast<const uint32_t*>(&raw[k]);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float4 av = factors[h * chunks + (c >> 3)], bv = factors[(2 + h) * chunks + (c >> 3)];
+      const float2 v0 = int8_unpack2<FP16>(u[2 * h]), v1 = int8_unpack2<FP16>(u[2 * h + 1]);
+      y[k][4 * h] = fmaf(v0.x, av.x, bv.x);
+      y[k][4 * h + 1] = fmaf(v0.y, av.y, bv.y);
+      y[k][4 * h + 2] = fmaf(v1.x, av.z, bv.z);
+      y[k][4 * h + 3] = fmaf(v1.y, av.w, bv.w);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (SILU) y[k][i] = silu(y[k][i]);
+      top = max_magnitude(top, y[k][i]);
+    }
+  }
+  const Int8Scale s = int8_scale(team.max(__float_as_uint(top) & 0x7FFFFFFFu, turn));
+#pragma unroll
+  for (int k = 0; k < NCH; ++k)
+    if (live && c0 + k * TEAM * 8 < p.channels) int8_put8_of(p.q + row * p.out_row_stride, c0 + k * TEAM * 8, s, y[k]);
+  if (live && c0 == 0) p.q_scale[row] = int8_step(s);
+}
+
+// The rows in 8 bits: TEAM threads hold a row of at most TEAM * NCH * 8 channels, ROWS of them at a time, and have the next ones
+// on their way.
+template <bool FP16, bool SILU, int TEAM, int NCH, int ROWS, bool VEC>
 __global__ void __launch_bounds__(kGnThreads, 1) group_norm_int8_kernel(const __grid_constant__ GnParams p) {
   grid_dependency_release();
   grid_dependency_wait();
   extern __shared__ float4 factors[];
   __shared__ float red[2][kGnThreads / 32];
-  const int chunks = p.channels / 8;
   const Team<TEAM, kGnThreads> team{red};
   constexpr int kTeams = kGnThreads / TEAM;
-  const int c0 = static_cast<int>(threadIdx.x % TEAM) * 8, first = static_cast<int>(threadIdx.x) / TEAM;
-  const long long s0 = static_cast<long long>(blockIdx.x) * p.strip_rows;
-  const int rows = static_cast<int>(s0 + p.strip_rows < p.rows ? p.strip_rows : p.rows - s0);
-  const uint16_t* x = p.x + blockIdx.y * p.x_batch_stride + (s0 + rows - 1 - first) * p.x_row_stride;  // from the strip's end to its start
-  uint4 next[NCH];
-  auto fetch = [&] {
+  const int c0 = static_cast<int>(threadIdx.x % TEAM) * 8;
+  // every gridDim.x-th tile of kTeams * ROWS rows, from the last row to the first; a team has every kTeams-th row of a tile
+  const long long step = static_cast<long long>(gridDim.x) * kTeams * ROWS, x_step = static_cast<long long>(kTeams) * p.x_row_stride;
+  long long row = p.rows - 1 - (static_cast<long long>(blockIdx.x) * kTeams * ROWS + threadIdx.x / TEAM);
+  long long end = p.rows - 1 - static_cast<long long>(blockIdx.x) * kTeams * ROWS;  // the tile's last row: the same in all teams
+  const uint16_t* x = p.x + blockIdx.y * p.x_batch_stride + row * p.x_row_stride;
+  uint4 next[ROWS][NCH];
+  auto fetch = [&](long long at) {
 #pragma unroll
-    for (int k = 0; k < NCH; ++k) {
-      next[k] = make_uint4(0, 0, 0, 0);
-      if (c0 + k * TEAM * 8 < p.channels) next[k] = int8_load8(x, c0 + k * TEAM * 8, p.channels, VEC);
-    }
+    for (int i = 0; i < ROWS; ++i)
+#pragma unroll
+      for (int k = 0; k < NCH; ++k) {
+        next[i][k] = make_uint4(0, 0, 0, 0);
+        if (at >= i * kTeams && c0 + k * TEAM * 8 < p.channels) next[i][k] = int8_load8(x - i * x_step, c0 + k * TEAM * 8, p.channels, VEC);
+      }
   };
-  if (first < rows) fetch();
+  fetch(row);
   group_norm_factors<FP16>(p, factors);
-  int turn = 0;
-  for (int r = first; r < rows; r += kTeams, turn ^= 1) {
-    uint4 raw[NCH];
+  for (int turn = 0; end >= 0; row -= step, end -= step) {
+    uint4 raw[ROWS][NCH];
 #pragma unroll
-    for (int k = 0; k < NCH; ++k) raw[k] = next[k];
-    x -= kTeams * p.x_row_stride;
-    if (r + kTeams < rows) fetch();
-    float y[NCH][8];
-    float top = 0.f;
+    for (int i = 0; i < ROWS; ++i)
 #pragma unroll
-    for (int k = 0; k < NCH; ++k) {
-      const int c = c0 + k * TEAM * 8;
-      if (c >= p.channels) continue;
-      const uint32_t* u = reinterpret_cast<const uint32_t*>(&raw[k]);
+      for (int k = 0; k < NCH; ++k) raw[i][k] = next[i][k];
+    x -= step * p.x_row_stride;
+    if (end >= step) fetch(row - step);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float4 av = factors[h * chunks + (c >> 3)], bv = factors[(2 + h) * chunks + (c >> 3)];
-        const float2 v0 = int8_unpack2<FP16>(u[2 * h]), v1 = int8_unpack2<FP16>(u[2 * h + 1]);
-        y[k][4 * h] = fmaf(v0.x, av.x, bv.x);
-        y[k][4 * h + 1] = fmaf(v0.y, av.y, bv.y);
-        y[k][4 * h + 2] = fmaf(v1.x, av.z, bv.z);
-        y[k][4 * h + 3] = fmaf(v1.y, av.w, bv.w);
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if constexpr (SILU) y[k][i] = silu(y[k][i]);
-        top = max_magnitude(top, y[k][i]);
-      }
-    }
-    const Int8Scale s = int8_scale(team.max(__float_as_uint(top) & 0x7FFFFFFFu, turn));
-    const long long row = blockIdx.y * p.rows + s0 + rows - 1 - r;
-#pragma unroll
-    for (int k = 0; k < NCH; ++k)
-      if (c0 + k * TEAM * 8 < p.channels) int8_put8_of(p.q + row * p.out_row_stride, c0 + k * TEAM * 8, s, y[k]);
-    if (c0 == 0) p.q_scale[row] = int8_step(s);
+    for (int i = 0; i < ROWS; ++i, turn ^= 1)
+      row_to_int8<FP16, SILU, TEAM, NCH, kGnThreads>(p, team, turn, raw[i], factors, c0, blockIdx.y * p.rows + row - i * kTeams, row >= i * kTeams);
   }
 }
 
-// Strips per image: one CTA per SM over all images, at least two rows of every thread's channels each.
+// One launch for what fits the shared memory of a few SMs: a cluster of CTAs takes a slab of channels (whole groups) of an
+// image, each CTA a strip of its rows, which stay in its shared memory between the two passes; the CTAs read each other's
+// statistics there. p.strips: a strip is a CTA; p.slab: channels of a slab. Shared memory: the rows, the sums (then the
+// factors), the strip's statistics, the groups' statistics.
+template <bool FP16, bool SILU, bool VEC, bool INT8>
+__global__ void __launch_bounds__(kClusterThreads, 2) group_norm_cluster_kernel(const __grid_constant__ GnParams p) {
+  grid_dependency_release();
+  grid_dependency_wait();
+  extern __shared__ float4 smem4[];
+  __shared__ float red[2][kClusterThreads / 32];
+  const int chunks = p.slab / 8, per = p.channels / p.groups, groups = p.slab / per;
+  const int lanes = p.strips.lanes;
+  const int lane = threadIdx.x / chunks, chunk = threadIdx.x - lane * chunks;
+  const int slab0 = static_cast<int>(blockIdx.y) * p.slab;
+  const int rank = static_cast<int>(blockIdx.x);
+  uint4* held = reinterpret_cast<uint4*>(smem4);  // [tiles * lanes][chunks]
+  float4* factors = smem4 + p.strips.tiles_of(0) * lanes * chunks;
+  float2* strip = reinterpret_cast<float2*>(factors + lanes * p.slab / 2);
+  float2* stat = strip + groups;
+  float weight = 1.f, bias = 0.f;  // on their way while the statistics are made
+  if (threadIdx.x < p.slab) {
+    weight = gn_weight<FP16>(p, slab0 + threadIdx.x);
+    bias = gn_bias<FP16>(p, slab0 + threadIdx.x);
+  }
+  strip_stats<kClusterThreads, FP16, VEC>(
+      p.x + blockIdx.z * p.x_batch_stride + slab0, p.x_row_stride, p.strips, rank, p.slab, per, reinterpret_cast<float*>(factors),
+      [&](const uint4& raw, int at) { held[(at * lanes + lane) * chunks + chunk] = raw; }, [&](int g, float2 v) { strip[g] = v; });
+  __syncthreads();
+  cluster_sync_all();
+  join_strips(groups, p.strips, p.rows, per, p.eps, stat, [&](int k, int g) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(map_to_cta(strip + g, static_cast<uint32_t>(k))) : "memory");
+    return v;
+  });
+  __syncthreads();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // this CTA has read the others' statistics
+  if (threadIdx.x < p.slab) put_factor<FP16>(threadIdx.x, chunks, stat[threadIdx.x / per], weight, bias, factors);
+  for (int c = threadIdx.x + kClusterThreads; c < p.slab; c += kClusterThreads)
+    put_factor<FP16>(c, chunks, stat[c / per], gn_weight<FP16>(p, slab0 + c), gn_bias<FP16>(p, slab0 + c), factors);
+  __syncthreads();
+  if constexpr (INT8) {
+    const Team<32, kClusterThreads> team{red};
+    const int c0 = static_cast<int>(threadIdx.x & 31) * 8;
+    const int mine = p.strips.rows_of(rank);
+    for (int r = static_cast<int>(threadIdx.x) >> 5; r < mine; r += kClusterThreads / 32) {
+      uint4 raw[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) raw[k] = c0 + k * 256 < p.slab ? held[r * chunks + (c0 >> 3) + k * 32] : make_uint4(0, 0, 0, 0);
+      const long long row = p.strips.first(rank, r % lanes) + r / lanes * p.strips.step();
+      row_to_int8<FP16, SILU, 32, 4, kClusterThreads>(p, team, 0, raw, factors, c0, blockIdx.z * p.rows + row, true);
+    }
+  } else if (lane < lanes) {
+    float a[8], b[8];
+    read_factors(factors, chunks, chunk, a, b);
+    const int count = p.strips.rows_of_lane(rank, lane);
+    uint16_t* out = p.out + blockIdx.z * p.out_batch_stride + p.strips.first(rank, lane) * p.out_row_stride + slab0 + chunk * 8;
+    const long long out_step = p.strips.step() * p.out_row_stride;
+    for (int at = 0; at < count; ++at) apply8<FP16, SILU, VEC>(held[(at * lanes + lane) * chunks + chunk], a, b, out + at * out_step);
+  }
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // the others have read this CTA's
+}
+
+// Strips per image: one CTA per SM over all images, at least two tiles each.
 int strips_of(long long batch, long long rows, int channels) {
   const long long lanes = kGnThreads / (channels / 8);
   long long n = 148 / batch;
@@ -341,10 +451,36 @@ int strips_of(long long batch, long long rows, int channels) {
   return static_cast<int>(n < 1 ? 1 : n);
 }
 
-void set_strips(GnParams& p, long long batch) {
-  p.strips = strips_of(batch, p.rows, p.channels);
-  p.strip_rows = (p.rows + p.strips - 1) / p.strips;
-  p.strips = static_cast<int>((p.rows + p.strip_rows - 1) / p.strip_rows);
+Strips make_strips(long long rows, int strips, int lanes) {
+  const long long tiles = (rows + lanes - 1) / lanes;
+  return {strips, lanes, static_cast<int>(tiles / strips), static_cast<int>(tiles % strips), static_cast<int>((tiles - 1) % strips),
+          static_cast<int>(tiles * lanes - rows)};
+}
+
+// The one-launch form: whether the call fits it, and its slab, strips and shared memory.
+constexpr int kClusterCtas = 8;
+struct GnCluster {
+  int slab;
+  size_t smem;
+};
+bool cluster_of(long long batch, long long rows, int channels, int groups, bool int8, GnCluster* to) {
+  const int per = channels / groups;
+  int unit = per;  // whole groups and whole chunks
+  while (unit % 8 != 0) unit += per;
+  if ((int8 && channels > 1024) || batch > 33 || rows > 33LL * 8 * 100 * 1024 / 2 / (batch * channels)) return false;
+  for (int slab = int8 ? channels : unit; slab <= channels && slab / 8 <= kClusterThreads; slab += unit) {
+    if (channels % slab != 0 || (slab < 32 && slab < channels)) continue;  // 64 bytes of a row at least
+    const long long clusters = batch * (channels / slab), lanes = kClusterThreads / (slab / 8);
+    const long long tiles = ((rows + lanes - 1) / lanes + kClusterCtas - 1) / kClusterCtas;
+    if (rows <= lanes * (kClusterCtas - 1)) continue;  // each CTA has rows
+    const long long held = tiles * lanes * slab * 2, smem = held + lanes * slab * 8 + slab / per * 16;
+    // so many clusters of eight CTAs of this size are on the GPU at a time; a second wave costs more than a second launch
+    if (clusters <= (smem <= 100 * 1024 ? 33 : 15) && smem <= 200 * 1024 && (!int8 || held <= 32 * 1024)) {
+      *to = {slab, static_cast<size_t>(smem)};
+      return true;
+    }
+  }
+  return false;
 }
 
 int check_gn(const hdit_group_norm_args* a) {
@@ -356,8 +492,7 @@ int check_gn(const hdit_group_norm_args* a) {
     return set_error(HDIT_ERR_SHAPE, "channels must be a multiple of 8 and of groups, at most %d", kMaxChannels);
   if (a->batch > 65535 || a->rows > 0x7fffffffLL) return set_error(HDIT_ERR_TOO_LARGE, "at most 65535 images of 2^31 - 1 rows");
   if (a->batch == 0 || a->rows == 0) return HDIT_OK;
-  if (a->x == nullptr || a->out == nullptr || a->scratch == nullptr) return set_error(HDIT_ERR_BAD_ARG, "null x / out / scratch");
-  if ((reinterpret_cast<uintptr_t>(a->scratch) & 7) != 0) return set_error(HDIT_ERR_SHAPE, "scratch not 8-byte aligned");
+  if (a->x == nullptr || a->out == nullptr) return set_error(HDIT_ERR_BAD_ARG, "null x / out");
   return HDIT_OK;
 }
 
@@ -368,7 +503,7 @@ cudaError_t launch_strips(K kernel, const GnParams& p, long long batch, size_t s
   // static shared memory counts, too
   const cudaError_t e = smem > 47 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) : cudaSuccess;
   if (e != cudaSuccess) return e;
-  return launch_overlapped(kernel, dim3(static_cast<unsigned>(p.strips), static_cast<unsigned>(batch)), dim3(kGnThreads), smem, st, 1, p);
+  return launch_overlapped(kernel, dim3(static_cast<unsigned>(p.strips.strips), static_cast<unsigned>(batch)), dim3(kGnThreads), smem, st, 1, p);
 }
 
 GnParams params_of(const hdit_group_norm_args* a, bool out_vec) {
@@ -390,7 +525,6 @@ GnParams params_of(const hdit_group_norm_args* a, bool out_vec) {
   p.act = a->act;
   p.eps = a->eps;
   p.vec = out_vec && !off16(a->x, a->x_batch_stride, a->x_row_stride);
-  set_strips(p, a->batch);
   return p;
 }
 
@@ -410,10 +544,12 @@ cudaError_t launch_apply(const GnParams& p, long long batch, cudaStream_t st) {
 
 template <bool FP16, bool SILU, bool VEC>
 cudaError_t launch_int8_act(const GnParams& p, long long batch, cudaStream_t st) {
-  auto kernel = p.channels <= 256    ? group_norm_int8_kernel<FP16, SILU, 32, 1, VEC>
-                : p.channels <= 512  ? group_norm_int8_kernel<FP16, SILU, 32, 2, VEC>
-                : p.channels <= 1024 ? group_norm_int8_kernel<FP16, SILU, 32, 4, VEC>
-                                     : group_norm_int8_kernel<FP16, SILU, 128, 4, VEC>;
+  auto kernel = p.channels <= 64     ? group_norm_int8_kernel<FP16, SILU, 8, 1, 4, VEC>
+                : p.channels <= 128  ? group_norm_int8_kernel<FP16, SILU, 16, 1, 4, VEC>
+                : p.channels <= 256  ? group_norm_int8_kernel<FP16, SILU, 32, 1, 4, VEC>
+                : p.channels <= 512  ? group_norm_int8_kernel<FP16, SILU, 32, 2, 2, VEC>
+                : p.channels <= 1024 ? group_norm_int8_kernel<FP16, SILU, 32, 4, 1, VEC>
+                                     : group_norm_int8_kernel<FP16, SILU, 128, 4, 1, VEC>;
   return launch_strips(kernel, p, batch, factor_bytes(p), st);
 }
 
@@ -422,14 +558,50 @@ cudaError_t launch_int8(const GnParams& p, long long batch, cudaStream_t st) {
   return p.act == HDIT_ACT_SILU ? launch_int8_act<FP16, true, VEC>(p, batch, st) : launch_int8_act<FP16, false, VEC>(p, batch, st);
 }
 
+template <bool FP16, bool SILU, bool VEC>
+cudaError_t launch_cluster_act(const GnParams& p, const GnCluster& c, bool int8, long long batch, cudaStream_t st) {
+  auto kernel = int8 ? group_norm_cluster_kernel<FP16, SILU, VEC, true> : group_norm_cluster_kernel<FP16, SILU, VEC, false>;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+  if (e != cudaSuccess) return e;
+  return launch_overlapped(kernel, dim3(kClusterCtas, static_cast<unsigned>(p.channels / c.slab), static_cast<unsigned>(batch)), dim3(kClusterThreads), c.smem,
+                           st, kClusterCtas, p);
+}
+
+template <bool FP16, bool VEC>
+cudaError_t launch_cluster(const GnParams& p, const GnCluster& c, bool int8, long long batch, cudaStream_t st) {
+  return p.act == HDIT_ACT_SILU ? launch_cluster_act<FP16, true, VEC>(p, c, int8, batch, st) : launch_cluster_act<FP16, false, VEC>(p, c, int8, batch, st);
+}
+
 #define HDIT_GN_OF(f, fp16, vec) ((fp16) ? ((vec) ? f<true, true> : f<true, false>) : ((vec) ? f<false, true> : f<false, false>))
+
+int run_group_norm(const hdit_group_norm_args* a, bool int8) {
+  GnParams p = params_of(a, int8 || !off16(a->out, a->out_batch_stride, a->out_row_stride));
+  const bool fp16 = a->dtype == HDIT_FP16;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(a->stream);
+  GnCluster c;
+  if (cluster_of(a->batch, a->rows, p.channels, p.groups, int8, &c)) {
+    p.slab = c.slab;
+    p.strips = make_strips(a->rows, kClusterCtas, kClusterThreads / (c.slab / 8));
+    HDIT_CUDA_OK((HDIT_GN_OF(launch_cluster, fp16, p.vec)(p, c, int8, a->batch, st)));
+    return HDIT_OK;
+  }
+  if (a->scratch == nullptr || (reinterpret_cast<uintptr_t>(a->scratch) & 7) != 0) return set_error(HDIT_ERR_BAD_ARG, "scratch is null or not 8-byte aligned");
+  p.strips = make_strips(a->rows, strips_of(a->batch, a->rows, p.channels), kGnThreads / (p.channels / 8));
+  HDIT_CUDA_OK((HDIT_GN_OF(launch_stats, fp16, p.vec)(p, a->batch, st)));
+  if (int8) HDIT_CUDA_OK((HDIT_GN_OF(launch_int8, fp16, p.vec)(p, a->batch, st)));
+  else HDIT_CUDA_OK((HDIT_GN_OF(launch_apply, fp16, p.vec)(p, a->batch, st)));
+  return HDIT_OK;
+}
 
 }  // namespace
 }  // namespace hdit
 
-extern "C" int64_t hdit_group_norm_scratch(int64_t batch, int64_t rows, int64_t channels, int64_t groups) {
+extern "C" int64_t hdit_group_norm_scratch(int64_t batch, int64_t rows, int64_t channels, int64_t groups, int32_t int8_rows) {
   using namespace hdit;
-  if (batch <= 0 || rows <= 0 || channels <= 0 || groups <= 0 || channels % 8 != 0 || channels > kMaxChannels) return 0;
+  GnCluster c;
+  if (batch <= 0 || rows <= 0 || rows > 0x7fffffffLL || channels <= 0 || groups <= 0 || channels % 8 != 0 || channels > kMaxChannels || channels % groups != 0)
+    return 0;
+  if (cluster_of(batch, rows, static_cast<int>(channels), static_cast<int>(groups), int8_rows != 0, &c)) return 0;
   return batch * strips_of(batch, rows, static_cast<int>(channels)) * groups * static_cast<int64_t>(sizeof(float2));
 }
 
@@ -437,12 +609,7 @@ extern "C" int hdit_group_norm(const hdit_group_norm_args* a) {
   using namespace hdit;
   const int rc = check_gn(a);
   if (rc != HDIT_OK || a->batch == 0 || a->rows == 0) return rc;
-  const GnParams p = params_of(a, !off16(a->out, a->out_batch_stride, a->out_row_stride));
-  const bool fp16 = a->dtype == HDIT_FP16;
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(a->stream);
-  HDIT_CUDA_OK((HDIT_GN_OF(launch_stats, fp16, p.vec)(p, a->batch, st)));
-  HDIT_CUDA_OK((HDIT_GN_OF(launch_apply, fp16, p.vec)(p, a->batch, st)));
-  return HDIT_OK;
+  return run_group_norm(a, false);
 }
 
 extern "C" int hdit_group_norm_int8(const hdit_group_norm_args* a) {
@@ -453,10 +620,5 @@ extern "C" int hdit_group_norm_int8(const hdit_group_norm_args* a) {
     return set_error(HDIT_ERR_SHAPE, "8-bit rows need a 16-byte aligned pointer and a row stride that is a multiple of 16 and covers a row");
   if (a->batch == 0 || a->rows == 0) return HDIT_OK;
   if (a->out_scale == nullptr) return set_error(HDIT_ERR_BAD_ARG, "null scale");
-  const GnParams p = params_of(a, true);
-  const bool fp16 = a->dtype == HDIT_FP16;
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(a->stream);
-  HDIT_CUDA_OK((HDIT_GN_OF(launch_stats, fp16, p.vec)(p, a->batch, st)));
-  HDIT_CUDA_OK((HDIT_GN_OF(launch_int8, fp16, p.vec)(p, a->batch, st)));
-  return HDIT_OK;
+  return run_group_norm(a, true);
 }

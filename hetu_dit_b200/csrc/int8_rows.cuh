@@ -78,6 +78,11 @@ struct Team {
   float (*red)[THREADS / 32];
   __device__ __forceinline__ void sync() const { asm volatile("bar.sync %0, %1;" ::"r"(1 + threadIdx.x / TEAM), "n"(TEAM) : "memory"); }
   __device__ __forceinline__ uint32_t max(uint32_t v, int slot) const {
+    if constexpr (TEAM < 32) {
+#pragma unroll
+      for (int o = TEAM / 2; o > 0; o >>= 1) v = ::max(v, __shfl_xor_sync(0xffffffffu, v, o));
+      return v;
+    }
     v = __reduce_max_sync(0xffffffffu, v);
     if constexpr (kWarps > 1) {
       uint32_t* r = reinterpret_cast<uint32_t*>(red[slot]);

@@ -1136,8 +1136,8 @@ _ACTS = {None: _C.ACT_NONE, "silu": _C.ACT_SILU}
 
 
 @functools.lru_cache(maxsize=1024)
-def _group_norm_scratch(batch, rows, channels, groups):
-    return _C.lib().hdit_group_norm_scratch(batch, rows, channels, groups)
+def _group_norm_scratch(batch, rows, channels, groups, int8_rows):
+    return _C.lib().hdit_group_norm_scratch(batch, rows, channels, groups, int8_rows)
 
 
 def _group_norm_args(x, groups, weight, bias, eps, act):
@@ -1165,9 +1165,9 @@ def _group_norm_args(x, groups, weight, bias, eps, act):
     return a, B, rows, C
 
 
-def _group_norm_run(entry, a, x):
+def _group_norm_run(entry, a, x, int8_rows):
     dev = x.device
-    need = _group_norm_scratch(a.batch, a.rows, a.channels, a.groups)
+    need = _group_norm_scratch(a.batch, a.rows, a.channels, a.groups, int8_rows)
     if need:
         scratch = x.new_empty(need, dtype=torch.uint8)
         a.scratch = scratch.data_ptr()
@@ -1197,7 +1197,7 @@ def group_norm(x, groups, weight=None, bias=None, eps=1e-6, act=None, out=None):
     if B * rows == 0:
         return out
     a.out = out.data_ptr()
-    _group_norm_run(_C.lib().hdit_group_norm, a, x)
+    _group_norm_run(_C.lib().hdit_group_norm, a, x, 0)
     return out
 
 
@@ -1209,5 +1209,5 @@ def group_norm_int8(x, groups, weight=None, bias=None, eps=1e-6, act=None):
     if B * rows == 0:
         return out
     a.out, a.out_scale, a.out_row_stride = out.q.data_ptr(), out.scale.data_ptr(), (C + 15) & ~15
-    _group_norm_run(_C.lib().hdit_group_norm_int8, a, x)
+    _group_norm_run(_C.lib().hdit_group_norm_int8, a, x, 1)
     return out

@@ -599,8 +599,8 @@ HDIT_API int hdit_int8_linear(const hdit_int8_linear_args* args);
  *   out[b, r, c] = act((x[b, r, c] - mean[b, g]) / sqrt(var[b, g] + eps) * weight[c] + bias[c]),  g = c / (channels / groups)
  * with mean and biased variance over the rows r (pixels) and channels of group g, fp32 arithmetic, 16-bit storage. x and out are
  * (batch, rows, channels) with contiguous channels, any batch and row strides (elements); channels a multiple of 8 and of
- * groups, at most 4096; weight and bias `channels` elements each or NULL (1 and 0). scratch: hdit_group_norm_scratch() bytes,
- * 8-byte aligned, of which nothing has to be kept before or after the call; calls that may overlap need one each. `out` may be x.
+ * groups, at most 4096; weight and bias `channels` elements each or NULL (1 and 0). scratch: hdit_group_norm_scratch() bytes
+ * (0: none is needed), 8-byte aligned, of which nothing has to be kept before or after the call; calls that may overlap need one each. `out` may be x.
  * hdit_group_norm_int8 writes each row (all channels of a pixel) as an 8-bit row instead: out is int8, rows of all images in
  * order out_row_stride bytes apart, out_scale their scales.
  *
@@ -625,7 +625,8 @@ typedef struct hdit_group_norm_args {
   int32_t reserved0;
 } hdit_group_norm_args;
 
-HDIT_API int64_t hdit_group_norm_scratch(int64_t batch, int64_t rows, int64_t channels, int64_t groups);
+/* int8_rows != 0: for hdit_group_norm_int8 */
+HDIT_API int64_t hdit_group_norm_scratch(int64_t batch, int64_t rows, int64_t channels, int64_t groups, int32_t int8_rows);
 HDIT_API int hdit_group_norm(const hdit_group_norm_args* args);
 HDIT_API int hdit_group_norm_int8(const hdit_group_norm_args* args);
 

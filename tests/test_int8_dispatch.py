@@ -129,7 +129,7 @@ def test_the_library_refuses_by_itself():
 
     for entry in (real.hdit_group_norm, real.hdit_group_norm_int8):
         for bad in (dict(dtype=2), dict(batch=-1), dict(channels=60), dict(groups=7), dict(groups=0), dict(channels=4104), dict(act=2), dict(x=0),
-                    dict(out=0), dict(batch=65536), dict(rows=1 << 31), dict(scratch=4100)):
+                    dict(out=0), dict(batch=65536), dict(rows=1 << 31), dict(rows=1 << 22, scratch=4100), dict(rows=1 << 22, scratch=0)):
             assert gn(entry, **bad) in (_C.HDIT_ERR_BAD_ARG, _C.HDIT_ERR_SHAPE, _C.HDIT_ERR_TOO_LARGE), bad
         assert gn(entry, batch=0) == 0 and gn(entry, rows=0) == 0 and entry(None) == _C.HDIT_ERR_BAD_ARG
     for bad in (dict(out=4104), dict(out_row_stride=72), dict(out_row_stride=48), dict(out_scale=0)):
