@@ -24,7 +24,7 @@ namespace {
 
 constexpr int kMaxChannels = 4096;
 constexpr int kAhead = 6;         // rows of a thread in flight
-constexpr int kClusterThreads = 256;  // two CTAs to an SM
+constexpr int cluster_threads(bool int8) { return int8 ? 512 : 256; }  // two CTAs to an SM, or few CTAs at all
 constexpr int kGnThreads = 512;  // what a CTA does beside its rows costs every warp some hundred instructions
 
 // How the rows of an image lie in tiles of `lanes` rows and the tiles in strips: strip k has tiles k, k + strips, ...; the last
@@ -384,11 +384,12 @@ __global__ void __launch_bounds__(kGnThreads, 1) group_norm_int8_kernel(const __
 // statistics there. p.strips: a strip is a CTA; p.slab: channels of a slab. Shared memory: the rows, the sums (then the
 // factors), the strip's statistics, the groups' statistics.
 template <bool FP16, bool SILU, bool VEC, bool INT8>
-__global__ void __launch_bounds__(kClusterThreads, 2) group_norm_cluster_kernel(const __grid_constant__ GnParams p) {
+__global__ void __launch_bounds__(cluster_threads(INT8), INT8 ? 1 : 2) group_norm_cluster_kernel(const __grid_constant__ GnParams p) {
   grid_dependency_release();
   grid_dependency_wait();
+  constexpr int kThreads = cluster_threads(INT8);
   extern __shared__ float4 smem4[];
-  __shared__ float red[2][kClusterThreads / 32];
+  __shared__ float red[2][kThreads / 32];
   const int chunks = p.slab / 8, per = p.channels / p.groups, groups = p.slab / per;
   const int lanes = p.strips.lanes;
   const int lane = threadIdx.x / chunks, chunk = threadIdx.x - lane * chunks;
@@ -403,7 +404,7 @@ __global__ void __launch_bounds__(kClusterThreads, 2) group_norm_cluster_kernel(
     weight = gn_weight<FP16>(p, slab0 + threadIdx.x);
     bias = gn_bias<FP16>(p, slab0 + threadIdx.x);
   }
-  strip_stats<kClusterThreads, FP16, VEC>(
+  strip_stats<kThreads, FP16, VEC>(
       p.x + blockIdx.z * p.x_batch_stride + slab0, p.x_row_stride, p.strips, rank, p.slab, per, reinterpret_cast<float*>(factors),
       [&](const uint4& raw, int at) { held[(at * lanes + lane) * chunks + chunk] = raw; }, [&](int g, float2 v) { strip[g] = v; });
   __syncthreads();
@@ -416,19 +417,19 @@ __global__ void __launch_bounds__(kClusterThreads, 2) group_norm_cluster_kernel(
   __syncthreads();
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // this CTA has read the others' statistics
   if (threadIdx.x < p.slab) put_factor<FP16>(threadIdx.x, chunks, stat[threadIdx.x / per], weight, bias, factors);
-  for (int c = threadIdx.x + kClusterThreads; c < p.slab; c += kClusterThreads)
+  for (int c = threadIdx.x + kThreads; c < p.slab; c += kThreads)
     put_factor<FP16>(c, chunks, stat[c / per], gn_weight<FP16>(p, slab0 + c), gn_bias<FP16>(p, slab0 + c), factors);
   __syncthreads();
   if constexpr (INT8) {
-    const Team<32, kClusterThreads> team{red};
+    const Team<32, kThreads> team{red};
     const int c0 = static_cast<int>(threadIdx.x & 31) * 8;
     const int mine = p.strips.rows_of(rank);
-    for (int r = static_cast<int>(threadIdx.x) >> 5; r < mine; r += kClusterThreads / 32) {
+    for (int r = static_cast<int>(threadIdx.x) >> 5; r < mine; r += kThreads / 32) {
       uint4 raw[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) raw[k] = c0 + k * 256 < p.slab ? held[r * chunks + (c0 >> 3) + k * 32] : make_uint4(0, 0, 0, 0);
       const long long row = p.strips.first(rank, r % lanes) + r / lanes * p.strips.step();
-      row_to_int8<FP16, SILU, 32, 4, kClusterThreads>(p, team, 0, raw, factors, c0, blockIdx.z * p.rows + row, true);
+      row_to_int8<FP16, SILU, 32, 4, kThreads>(p, team, 0, raw, factors, c0, blockIdx.z * p.rows + row, true);
     }
   } else if (lane < lanes) {
     float a[8], b[8];
@@ -468,14 +469,16 @@ bool cluster_of(long long batch, long long rows, int channels, int groups, bool 
   int unit = per;  // whole groups and whole chunks
   while (unit % 8 != 0) unit += per;
   if ((int8 && channels > 1024) || batch > 33 || rows > 33LL * 8 * 100 * 1024 / 2 / (batch * channels)) return false;
-  for (int slab = int8 ? channels : unit; slab <= channels && slab / 8 <= kClusterThreads; slab += unit) {
+  for (int slab = int8 ? channels : unit; slab <= channels && slab / 8 <= cluster_threads(int8); slab += unit) {
     if (channels % slab != 0 || (slab < 32 && slab < channels)) continue;  // 64 bytes of a row at least
-    const long long clusters = batch * (channels / slab), lanes = kClusterThreads / (slab / 8);
+    const long long clusters = batch * (channels / slab), lanes = cluster_threads(int8) / (slab / 8);
     const long long tiles = ((rows + lanes - 1) / lanes + kClusterCtas - 1) / kClusterCtas;
     if (rows <= lanes * (kClusterCtas - 1)) continue;  // each CTA has rows
     const long long held = tiles * lanes * slab * 2, smem = held + lanes * slab * 8 + slab / per * 16;
-    // so many clusters of eight CTAs of this size are on the GPU at a time; a second wave costs more than a second launch
-    if (clusters <= (smem <= 100 * 1024 ? 33 : 15) && smem <= 200 * 1024 && (!int8 || held <= 32 * 1024)) {
+    // So many clusters of this size are on the GPU at a time; a second wave costs more than a second launch. 8-bit rows need all
+    // channels of a pixel in one CTA, which leaves few CTAs: with 82 KB each, two images of 32 x 32 x 640 took 15 us, in two
+    // launches 9.9.
+    if (clusters <= (smem <= 100 * 1024 && !int8 ? 33 : 15) && smem <= 200 * 1024 && (!int8 || held <= 32 * 1024)) {
       *to = {slab, static_cast<size_t>(smem)};
       return true;
     }
@@ -563,8 +566,8 @@ cudaError_t launch_cluster_act(const GnParams& p, const GnCluster& c, bool int8,
   auto kernel = int8 ? group_norm_cluster_kernel<FP16, SILU, VEC, true> : group_norm_cluster_kernel<FP16, SILU, VEC, false>;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
   if (e != cudaSuccess) return e;
-  return launch_overlapped(kernel, dim3(kClusterCtas, static_cast<unsigned>(p.channels / c.slab), static_cast<unsigned>(batch)), dim3(kClusterThreads), c.smem,
-                           st, kClusterCtas, p);
+  return launch_overlapped(kernel, dim3(kClusterCtas, static_cast<unsigned>(p.channels / c.slab), static_cast<unsigned>(batch)),
+                           dim3(cluster_threads(int8)), c.smem, st, kClusterCtas, p);
 }
 
 template <bool FP16, bool VEC>
@@ -581,7 +584,7 @@ int run_group_norm(const hdit_group_norm_args* a, bool int8) {
   GnCluster c;
   if (cluster_of(a->batch, a->rows, p.channels, p.groups, int8, &c)) {
     p.slab = c.slab;
-    p.strips = make_strips(a->rows, kClusterCtas, kClusterThreads / (c.slab / 8));
+    p.strips = make_strips(a->rows, kClusterCtas, cluster_threads(int8) / (c.slab / 8));
     HDIT_CUDA_OK((HDIT_GN_OF(launch_cluster, fp16, p.vec)(p, c, int8, a->batch, st)));
     return HDIT_OK;
   }
