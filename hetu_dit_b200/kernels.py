@@ -731,7 +731,9 @@ def _plain_weights(linear):
 def linear_tail(linear, x, epilogue, residual=None, gate=None, out=None):
     """A torch.nn.Linear followed by its elementwise tail ("gelu_tanh", or "gate_residual" = residual +
     gate[:, None] * linear(x)), as one kernel when _fusable_weights() has the layer, rows are evenly strided across
-    the batch and it pays, else as the call of `linear` plus hdit_gelu_tanh / hdit_gate_residual."""
+    the batch and it pays, else as the call of `linear` plus hdit_gelu_tanh / hdit_gate_residual. A layer of another class
+    that has a form with the tail of its own (with_tail, as model_executor.layers.int8_linear.Int8Linear does) takes that, where
+    nothing waits for its call."""
     if epilogue not in ("gelu_tanh", "gate_residual"):
         raise ValueError(epilogue)
     weights = _fusable_weights((x,), (linear,)) if epilogue in FUSED_LINEAR_TAILS else None
@@ -741,6 +743,9 @@ def linear_tail(linear, x, epilogue, residual=None, gate=None, out=None):
         if _even_rows(x) and FUSED_LINEAR_MIN_ROWS <= B * S <= FUSED_LINEAR_MAX_ROWS and _tail_fits(x, n, residual, gate, out) \
                 and (residual is None or _even_rows(residual)) and (out is None or _even_rows(out)) and _group_pays(((B * S, n),), k):
             return linear_fused(x, w, b, epilogue, residual=residual, gate=gate, out=out)
+    cls = type(linear)
+    if FUSED_LINEAR and epilogue in FUSED_LINEAR_TAILS and hasattr(cls, "with_tail") and is_plain(linear, cls):
+        return linear.with_tail(x, epilogue, residual=residual, gate=gate, out=out)
     y = linear(x)
     if epilogue == "gelu_tanh":
         return gelu_tanh(y, out=y if out is None else out)
@@ -779,7 +784,7 @@ def _fusable_weights(xs, linears):
     if dtype not in _DTYPE_CODE or k % 8:
         return None
     for x in xs:
-        if not x.is_cuda or x.dim() != 3 or x.dtype != dtype or x.device != dev:
+        if type(x) is Int8Rows or not x.is_cuda or x.dim() != 3 or x.dtype != dtype or x.device != dev:
             return None
         B, S, kx = x.shape
         if kx != k or (B > 1 and S < 32) or not _aligned(x):

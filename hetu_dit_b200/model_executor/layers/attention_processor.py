@@ -22,6 +22,7 @@ from ...core.distributed import parallel_state as ps
 from ...core.parallel import (hetuDiTFluxLongContextAttention, hetuDiTJointLongContextAttention,
                               hetuDiTLongContextAttention)
 from ...core.resource_manager.cache_manager import get_cache_manager
+from .int8_linear import Int8Linear, read_rows
 
 
 def _heads(x, attn):
@@ -85,6 +86,8 @@ def _qkv(attn, streams, rope):
             return outs
     outs = []
     for x, projs, (wq, wk), ranges in streams:
+        if read_rows(projs) and torch.is_tensor(x):
+            x = kernels.quantize_rows(x)  # once for all three
         q, k, v = (_heads(p(x), attn) for p in projs)
         for lo, hi, rotate, row0, seq_start in ranges:
             _norm_rope(attn, q[:, lo:hi], k[:, lo:hi], wq, wk, rope if rotate else None, row0, seq_start)
@@ -104,7 +107,9 @@ def _prologue_range(lo, hi, wq, wk, rope, row0):
 def _project_into(buf, row0, x, linear):
     """buf[:, row0:row0 + S] = linear(x) without a temporary when the rows are one contiguous block."""
     B, S, _ = x.shape
-    if B == 1 and not torch.is_grad_enabled():
+    if kernels.is_plain(linear, Int8Linear):
+        kernels.linear_int8(x, linear.rows, linear.bias, out=buf[:, row0:row0 + S])
+    elif B == 1 and not torch.is_grad_enabled():
         torch.addmm(linear.bias, x[0], linear.weight.t(), out=buf[0, row0:row0 + S])
     else:
         buf[:, row0:row0 + S] = linear(x)

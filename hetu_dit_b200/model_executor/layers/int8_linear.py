@@ -1,0 +1,78 @@
+"""Linear layers that hold their weight in 8-bit integers, for the blocks of the -shaped DiT models.
+
+A layer's weight has one scale per output channel, made once; the rows of its input are brought into 8 bits with a scale each
+when it is called (kernels.quantize_rows, kernels.ln_modulate_int8), so that no calibration is needed. The products run on
+the tensor cores in 8-bit integers at twice the rate of 16-bit values and read half the weight bytes. Each step is off by at
+most half a step, 1/254 of the row's or channel's largest value. Inference only. (The reference has no 8-bit path; the layers
+are the torch.nn.Linear of the blocks it wraps, hetu_dit/model_executor/diffusion_executor/layers/attention_processor.py:207-449
+and layers/feedforward.py:73-78.)
+"""
+import torch
+import torch.nn as nn
+
+from ... import kernels
+
+
+class Int8Linear(nn.Module):
+    """x @ weight.T + bias with the weight in 8 bits, in place of a torch.nn.Linear. x: a 16-bit tensor, or kernels.Int8Rows."""
+
+    def __init__(self, weight: kernels.Int8Rows, bias=None):
+        super().__init__()
+        self.out_features, self.in_features = weight.shape
+        pitch = weight.q.stride(0) if self.out_features > 1 else (self.in_features + 15) & ~15
+        # the whole rows, padding included: a copy of them keeps the rows on 16-byte boundaries
+        self.register_buffer("weight_q", weight.q if pitch == self.in_features else
+                             weight.q.as_strided((self.out_features, pitch), (pitch, 1)))
+        self.register_buffer("weight_scale", weight.scale)
+        self.register_buffer("bias", None if bias is None else bias.detach().clone())
+        self.dtype = weight.dtype
+
+    @classmethod
+    def from_linear(cls, linear: nn.Linear):
+        """The layer of a 16-bit torch.nn.Linear on the GPU."""
+        return cls(kernels.quantize_rows(linear.weight.detach()), linear.bias)
+
+    @property
+    def rows(self):
+        """The weight as kernels.linear_int8() takes it."""
+        q = self.weight_q
+        return kernels.Int8Rows(q if q.shape[1] == self.in_features else q[:, :self.in_features], self.weight_scale, self.dtype)
+
+    def _apply(self, fn, recurse=True):
+        scale = self.weight_scale
+        super()._apply(fn, recurse)
+        if self.weight_scale.dtype != scale.dtype:  # a change of the 16-bit type is not one of the scales' type
+            self.weight_scale = scale.to(self.weight_scale.device)
+        return self
+
+    def forward(self, x):
+        return kernels.linear_int8(x, self.rows, self.bias)
+
+    def with_tail(self, x, epilogue, residual=None, gate=None, out=None):
+        """kernels.linear_tail() of this layer in one launch (two with 16-bit x)."""
+        return kernels.linear_int8(x, self.rows, self.bias, epilogue, residual=residual, gate=gate, out=out)
+
+    def extra_repr(self):
+        return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"
+
+
+def read_rows(linears):
+    """Whether all that reads an input are 8-bit layers that nothing waits for the call of: they may be given Int8Rows, made
+    once, in its place."""
+    for layer in linears:
+        if not kernels.is_plain(layer, Int8Linear):
+            return False
+    return True
+
+
+@torch.no_grad()
+def quantize_linears_(module: nn.Module):
+    """Puts an Int8Linear in the place of every torch.nn.Linear below `module` (16-bit, on the GPU); returns module. What has
+    another class (an adapter) stays. Block caches address torch.nn.Linear weights by name: a module whose slices migrate
+    between plans keeps them."""
+    for name, child in module.named_children():
+        if type(child) is nn.Linear:
+            setattr(module, name, Int8Linear.from_linear(child))
+        else:
+            quantize_linears_(child)
+    return module

@@ -34,6 +34,7 @@ import torch.nn.functional as F
 from ... import kernels
 from ...core.distributed import parallel_state as ps
 from ..layers.attention_processor import CogVideoXAttnProcessor, JointAttnProcessor, SingleAttnProcessor
+from ..layers.int8_linear import quantize_linears_, read_rows
 
 
 @dataclass
@@ -241,6 +242,16 @@ class _Branch:
         self.main.wait_stream(self.side)
 
 
+def _sees_rows(attn, processor, projections, *others):
+    """Whether a wrapped attention layer on one GPU may be given its input as Int8Rows: its projections (by name) and whatever
+    else reads the input are 8-bit layers, and nothing else sees it."""
+    if ps.get_sequence_parallel_world_size() != 1 or not kernels.is_plain(attn, _Wrapped):
+        return False
+    inner = attn.module
+    return kernels.is_plain(inner, Attention) and type(inner.processor) is processor and \
+        read_rows([getattr(inner, name) for name in projections] + list(others))
+
+
 def _modulate(x, shift, scale):
     return x * (1 + scale[:, None]) + shift[:, None]
 
@@ -271,7 +282,10 @@ class JointBlock(nn.Module):
         d = self.d
         mod, cmod = mods if mods is not None else self.modulation(F.silu(temb))
         # LayerNorm + modulation and gate + residual are one fused pass each (csrc/elementwise.cu)
-        h, c = kernels.ln_modulate_pair(hidden, mod[0], mod[1], context, cmod[0], cmod[1])
+        if hidden.is_cuda and _sees_rows(self.attn, JointAttnProcessor, ("to_q", "to_k", "to_v", "add_q_proj", "add_k_proj", "add_v_proj")):
+            h, c = kernels.ln_modulate_int8(hidden, mod[0], mod[1]), kernels.ln_modulate_int8(context, cmod[0], cmod[1])
+        else:
+            h, c = kernels.ln_modulate_pair(hidden, mod[0], mod[1], context, cmod[0], cmod[1])
         sp = (ps.get_sequence_parallel_world_size() > 1 or BRANCH_TEXT_TAIL_ALWAYS) and hidden.is_cuda
         # with fused linear layers the gated residual of the image stream rides on the attention's output
         # projection (and the text stream's too, unless its tail runs on the branch stream below). Only where nothing
@@ -296,7 +310,11 @@ class JointBlock(nn.Module):
             return hidden, context
         hidden = a_img if fuse else kernels.gate_residual(hidden, mod[2], a_img)
         context = a_txt if fuse else kernels.gate_residual(context, cmod[2], a_txt)
-        h, c = kernels.ln_modulate_pair(hidden, mod[3], mod[4], context, cmod[3], cmod[4])
+        layers, layers_c = _mlp_layers(self.ff), _mlp_layers(self.ff_context)
+        if hidden.is_cuda and layers is not None and layers_c is not None and read_rows((layers[0], layers_c[0])):
+            h, c = kernels.ln_modulate_int8(hidden, mod[3], mod[4]), kernels.ln_modulate_int8(context, cmod[3], cmod[4])
+        else:
+            h, c = kernels.ln_modulate_pair(hidden, mod[3], mod[4], context, cmod[3], cmod[4])
         return feed_forward_pair(self.ff, h, hidden, mod[5], self.ff_context, c, context, cmod[5])
 
 
@@ -318,7 +336,10 @@ class SingleBlock(nn.Module):
 
     def forward(self, x, temb, rope, text_len, token_offset=0, text_offset=None, text_total=None, mods=None):
         shift, scale, gate = mods if mods is not None else self.modulation(F.silu(temb))
-        h = kernels.ln_modulate(x, shift, scale)
+        if x.is_cuda and _sees_rows(self.attn, SingleAttnProcessor, ("to_q", "to_k", "to_v"), self.proj_mlp):
+            h = kernels.ln_modulate_int8(x, shift, scale)
+        else:
+            h = kernels.ln_modulate(x, shift, scale)
         if ps.get_sequence_parallel_world_size() == 1:
             # attention output and GELU(MLP) land side by side in the buffer the output projection reads:
             # no concatenated copy
@@ -444,6 +465,15 @@ class ShapedDiT(nn.Module):
                 p.fill_(1.0)
             else:
                 p.copy_(torch.randn(p.shape, generator=gen, device=p.device, dtype=torch.float32) * std)
+        return self
+
+    def quantize_linears_(self):
+        """Brings the weights of the blocks' linear layers, adaLN among them, into 8 bits (layers.int8_linear): 16-bit model on
+        the GPU, inference only. The embedders and the output layer stay as they are. Not for a model whose blocks a block cache
+        moves between plans, which addresses torch.nn.Linear weights."""
+        for blk in list(self.transformer_blocks) + list(self.single_transformer_blocks):
+            quantize_linears_(blk)
+        self.__dict__.pop("_step_graphs", None)  # captured with the 16-bit weights
         return self
 
     def register_cache(self):

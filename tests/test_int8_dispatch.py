@@ -149,3 +149,64 @@ def test_the_library_refuses_by_itself():
         assert linear(**bad) in (_C.HDIT_ERR_BAD_ARG, _C.HDIT_ERR_SHAPE, _C.HDIT_ERR_TOO_LARGE), bad
     assert linear(m=0) == 0
     assert real.hdit_int8_linear(None) == _C.HDIT_ERR_BAD_ARG
+
+
+def test_an_8_bit_layer_takes_its_tail_where_nothing_waits_for_its_call(monkeypatch):
+    from hetu_dit_b200.model_executor.layers.int8_linear import Int8Linear, read_rows
+    layer = Int8Linear(rows8(24, 40), torch.zeros(24).bfloat16())
+    assert layer.rows.shape == (24, 40) and layer.rows.q.stride(0) == 48
+    seen = []
+
+    def linear_int8(x, weight, bias=None, epilogue="bias", residual=None, gate=None, out=None):
+        seen.append(epilogue)
+        return gpu_like(2, 40, 24)
+
+    monkeypatch.setattr(kernels, "linear_int8", linear_int8)
+    monkeypatch.setattr(kernels, "gelu_tanh", lambda y, out=None: seen.append("gelu kernel"))
+    monkeypatch.setattr(kernels, "gate_residual", lambda r, g, y, out=None: seen.append("gate kernel"))
+    x, res, gate = gpu_like(2, 40, 40), gpu_like(2, 40, 24), gpu_like(2, 24)
+    with torch.no_grad():
+        for held in (x, rows8(2, 40, 40)):
+            kernels.linear_tail(layer, held, "gelu_tanh")
+            kernels.linear_tails([(layer, held, "gate_residual", res, gate), (layer, held, "gelu_tanh")])
+        assert seen == ["gelu_tanh", "gate_residual", "gelu_tanh"] * 2 and read_rows((layer, layer))
+        seen.clear()
+        handle = layer.register_forward_hook(lambda m, i, o: seen.append("hook"))
+        kernels.linear_tail(layer, x, "gate_residual", residual=res, gate=gate)
+        assert seen == ["bias", "hook", "gate kernel"] and not read_rows((layer,))
+        handle.remove()
+        seen.clear()
+        monkeypatch.setattr(kernels, "FUSED_LINEAR", False)
+        kernels.linear_tail(layer, x, "gelu_tanh")
+        assert seen == ["bias", "gelu kernel"]
+
+
+def test_scales_of_an_8_bit_layer_keep_their_type():
+    from hetu_dit_b200.model_executor.layers.int8_linear import Int8Linear
+    scale = torch.rand(24)
+    layer = Int8Linear(kernels.Int8Rows(torch.zeros(24, 32, dtype=torch.int8), scale), torch.zeros(24).bfloat16())
+    layer.to(torch.float16)
+    assert layer.weight_scale.dtype == torch.float32 and torch.equal(layer.weight_scale, scale) and layer.bias.dtype == torch.float16
+    other = Int8Linear(kernels.Int8Rows(torch.zeros(24, 32, dtype=torch.int8), torch.zeros(24)), torch.zeros(24).bfloat16())
+    other.load_state_dict(layer.state_dict())
+    assert torch.equal(other.weight_scale, scale)
+
+
+def test_quantize_linears_replaces_plain_layers_only(monkeypatch):
+    from hetu_dit_b200.model_executor.layers import int8_linear
+
+    class Adapter(torch.nn.Linear):
+        pass
+
+    monkeypatch.setattr(kernels, "quantize_rows", lambda w: rows8(*w.shape))
+    net = torch.nn.ModuleDict({"a": torch.nn.Linear(8, 16), "b": torch.nn.ModuleList([torch.nn.Linear(16, 8, bias=False), Adapter(8, 8)])})
+    assert int8_linear.quantize_linears_(net) is net
+    assert type(net["a"]) is int8_linear.Int8Linear and type(net["b"][0]) is int8_linear.Int8Linear and type(net["b"][1]) is Adapter
+    assert net["b"][0].bias is None and (net["a"].out_features, net["a"].in_features) == (16, 8)
+
+
+def test_an_attention_of_its_own_needs_no_projections():
+    from hetu_dit_b200.model_executor.layers.attention_processor import JointAttnProcessor
+    from hetu_dit_b200.model_executor.models import shaped_dit
+    assert not shaped_dit._sees_rows(torch.nn.Identity(), JointAttnProcessor, ("to_q",))
+    assert not shaped_dit._sees_rows(shaped_dit._Wrapped(torch.nn.Identity()), JointAttnProcessor, ("to_q",))
