@@ -167,8 +167,9 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtas) int8_linear_few_kernel(
 #pragma unroll
       for (int w = 0; w < kFewWarps; ++w) sum += sums[w][ch][m];
       if (n < p.N) {
-        float v = int8_value(sum, row_scale[m], p.w_scale[n], p.bias != nullptr ? to_f<FP16>(p.bias[n]) : 0.f);
-        if (p.epilogue == HDIT_GEMM_BIAS_GELU_TANH) v = gelu_tanh_f(v);
+        const float bias = p.bias != nullptr ? to_f<FP16>(p.bias[n]) : 0.f;
+        float v = int8_value2(sum, sum, row_scale[m], make_float2(p.w_scale[n], p.w_scale[n]), make_float2(bias, bias)).x;
+        if (p.epilogue == HDIT_GEMM_BIAS_GELU_TANH) v = int8_gelu2(make_float2(v, v)).x;
         else if (p.epilogue == HDIT_GEMM_BIAS_GATE_RESIDUAL)
           v = fmaf(to_f<FP16>(p.gate[m / p.rows_per_batch * p.gate_batch_stride + n]), v, to_f<FP16>(p.residual[m * p.ldr + n]));
         p.out[m * p.ldo + n] = from_f<FP16>(v);

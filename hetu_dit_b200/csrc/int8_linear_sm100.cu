@@ -7,7 +7,7 @@
 // MMAs of 32 -- so operand bytes per clock are the same and the main loop of a tile takes half the time for the same K; the
 // epilogue has half the time to hide behind it.
 //
-//   epilogue     per 32 x 64 piece of a warp, a lane to a row: scales, bias and gate of the warp's columns wait in shared
+//   epilogue     per 32 x 32 piece of a warp, a lane to a row: scales, bias and gate of the warp's columns wait in shared
 //                memory (they are fetched while the tile before is worked on), the residual's piece comes into the staging
 //                buffer by TMA one piece ahead, the result takes its place there and leaves by TMA. Two staging buffers.
 //
@@ -22,6 +22,7 @@ namespace hdit {
 namespace {
 
 constexpr int kTileKBytes = 128;  // one swizzle row
+constexpr int kPieceBytes = 2048;  // 32 rows x 32 columns of 16 bits, 64-byte swizzle: chunk j of row r sits at chunk j ^ (r / 2 % 4)
 
 enum Int8Wait : int {
   Q_PROD_EMPTY = 211,
@@ -74,10 +75,15 @@ __device__ __forceinline__ void tma_store_wait_read() {
 }
 __device__ __forceinline__ void tma_store_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
+// Column k of row i of a staged piece.
+__device__ __forceinline__ uint16_t* staged(uint8_t* stage, int i, int k) {
+  return reinterpret_cast<uint16_t*>(stage + i * 64 + (((k >> 3) ^ ((i >> 1) & 3)) << 4) + (k & 7) * 2);
+}
+
 struct alignas(64) Int8Params {
   CUtensorMap a_map;
   CUtensorMap w_map;
-  CUtensorMap out_map;  // boxes of 64 columns x 32 rows, where tma_out / tma_residual say so
+  CUtensorMap out_map;  // boxes of 32 columns x 32 rows, where tma_out / tma_residual say so
   CUtensorMap residual_map;
   int M, N, k_blocks;
   int m_tiles, n_tiles, group_m;
@@ -97,10 +103,9 @@ struct alignas(64) Int8Params {
 
 template <int BN, bool PAIR, int EPI>
 struct Int8Cfg {
-  // Four warps reach the 128 lanes of an accumulator; a second team takes the other half of the columns
-  static constexpr int kPieces = BN / 64;
-  static constexpr int kColTeams = BN >= 128 ? 2 : 1;
-  static constexpr int kTeamPieces = (kPieces + kColTeams - 1) / kColTeams;  // the last team may have fewer
+  // Four warps, a team, reach the 128 lanes of an accumulator; each team has 64 of its columns in two pieces of 32
+  static constexpr int kTeamCols = 64, kTeamPieces = 2;
+  static constexpr int kColTeams = BN / kTeamCols;
   static constexpr int kEpiWarps = 4 * kColTeams;
   static constexpr int kThreads = 64 + 32 * kEpiWarps;
   static constexpr int kTileRows = PAIR ? 256 : 128;
@@ -108,11 +113,11 @@ struct Int8Cfg {
   static constexpr int kABytes = 128 * kTileKBytes;
   static constexpr int kBBytes = kBRows * kTileKBytes;
   static constexpr int kStageBytes = kABytes + kBBytes;
-  // pieces of 32 rows x 64 columns of 16 bits per epilogue warp: two where a residual comes in beside the result that leaves.
+  // pieces of 32 rows x 32 columns of 16 bits per epilogue warp: two where a residual comes in beside the result that leaves.
   // One more costs a stage of the ring, which 256 columns miss more: 4608 x 12288 x 3072 + GELU takes 137 us with 4 stages and
   // two buffers, 124 with 6 and one.
   static constexpr int kBufs = EPI == HDIT_GEMM_BIAS_GATE_RESIDUAL ? 2 : 1;
-  static constexpr int kStagingBytes = kEpiWarps * kBufs * 4096;
+  static constexpr int kStagingBytes = kEpiWarps * kBufs * kPieceBytes;
   // barriers and the columns' scales, bias and gate: what is left of 227 KB beside six stages of 32 KB and one piece per warp
   static constexpr int kSmallBytes = 3072;
   static constexpr int kStagesFit = (kMaxSmem - kSmallBytes - kStagingBytes) / kStageBytes;
@@ -120,7 +125,6 @@ struct Int8Cfg {
   static constexpr int kAccCols = BN == 192 ? 256 : BN;
   static constexpr int kTmemCols = 2 * kAccCols;
   static constexpr int kSmemBytes = kSmallBytes + kStages * kStageBytes + kStagingBytes;
-  static constexpr int kTeamCols = kTeamPieces * 64;  // at most one for each of the team's 128 threads
   static_assert(512 + kColTeams * kTeamCols * 10 <= kSmallBytes, "no room for the columns");
   static_assert(kStageBytes % 1024 == 0, "TMA tiles start at multiples of the swizzle's 1024 bytes");
   static_assert(kStages >= 3, "ring too short");
@@ -291,8 +295,7 @@ __global__ void __launch_bounds__(Int8Cfg<BN, PAIR, EPI>::kThreads, 1) int8_line
     constexpr bool kGated = EPI == HDIT_GEMM_BIAS_GATE_RESIDUAL;
     const int quarter = warp & 3;  // the TMEM lanes this warp may read: [32 * quarter, 32 * quarter + 32)
     const int team = (warp - 2) >> 2;
-    const int c0 = team * C::kTeamPieces, c1 = min(C::kPieces, c0 + C::kTeamPieces);
-    uint8_t* const staging = staging_base + (warp - 2) * (C::kBufs * 4096);
+    uint8_t* const staging = staging_base + (warp - 2) * (C::kBufs * kPieceBytes);
     uint64_t* const res_full = res_bars + (warp - 2) * 2;
     const int t_col = (threadIdx.x - 64) & 127;  // the column of its team that this thread fetches
     float* const col_scale = reinterpret_cast<float*>(col_base + team * (C::kTeamCols * 10));
@@ -301,7 +304,7 @@ __global__ void __launch_bounds__(Int8Cfg<BN, PAIR, EPI>::kThreads, 1) int8_line
     auto team_sync = [&] { asm volatile("bar.sync %0, 128;" ::"r"(1 + team) : "memory"); };
 
     // what the tile needs beside its sums; fetched one tile ahead
-    long long row0 = 0;     // first row of the warp
+    int row0 = 0;           // first row of the warp
     int tile_col = 0;       // first column of the team
     bool one_batch = true;  // all rows of the team have one batch entry: its gate waits in shared memory, else each row reads its own
     float row_scale = 0.f, f_scale = 0.f;
@@ -309,9 +312,9 @@ __global__ void __launch_bounds__(Int8Cfg<BN, PAIR, EPI>::kThreads, 1) int8_line
     auto fetch = [&](int tile) {
       int m_t, n_t;
       int8_tile_coords(p, tile, m_t, n_t);
-      const long long team_row0 = static_cast<long long>(m_t) * C::kTileRows + static_cast<long long>(rank) * 128;
+      const int team_row0 = m_t * C::kTileRows + static_cast<int>(rank) * 128;
       row0 = team_row0 + quarter * 32;
-      tile_col = n_t * BN + c0 * 64;
+      tile_col = n_t * BN + team * C::kTeamCols;
       unsigned batch = 0;
       if constexpr (kGated) {
         const unsigned first = static_cast<unsigned>(team_row0 < p.M ? team_row0 : 0);
@@ -331,10 +334,10 @@ __global__ void __launch_bounds__(Int8Cfg<BN, PAIR, EPI>::kThreads, 1) int8_line
     };
     // pieces are numbered through all tiles; piece i has staging buffer i % kBufs
     uint32_t piece = 0, res_phase = 0, res_pending = 0;
-    auto issue_residual = [&](long long row, int col, uint32_t buf) {
+    auto issue_residual = [&](int row, int col, uint32_t buf) {
       if (lane == 0 && row < p.M && col < p.N) {
-        mbar_expect_tx(&res_full[buf], 4096);
-        tma_load_2d(staging + buf * 4096, &p.residual_map, &res_full[buf], col, static_cast<int>(row));
+        mbar_expect_tx(&res_full[buf], kPieceBytes);
+        tma_load_2d(staging + buf * kPieceBytes, &p.residual_map, &res_full[buf], col, row);
       }
       if (row < p.M && col < p.N) res_pending |= 1u << buf;
     };
@@ -347,7 +350,7 @@ __global__ void __launch_bounds__(Int8Cfg<BN, PAIR, EPI>::kThreads, 1) int8_line
     }
     for (int tile = unit; tile < total_tiles; tile += n_units, ++local) {
       const uint32_t acc = local & 1, use = local >> 1;
-      const long long my_row0 = row0;
+      const int my_row0 = row0;
       const int my_col = tile_col;
       const bool my_one_batch = one_batch;
       const float my_scale = row_scale;
@@ -367,22 +370,21 @@ __global__ void __launch_bounds__(Int8Cfg<BN, PAIR, EPI>::kThreads, 1) int8_line
       }
       tc_fence_after();
 #pragma unroll 1
-      for (int c = c0; c < c1; ++c, ++piece) {
+      for (int c = 0; c < C::kTeamPieces; ++c, ++piece) {
         const uint32_t buf = C::kBufs == 1 ? 0 : piece & 1;
-        uint8_t* const stage = staging + buf * 4096;
-        const int at = (c - c0) * 64, col0 = my_col + at;
+        uint8_t* const stage = staging + buf * kPieceBytes;
+        const int at = c * 32, col0 = my_col + at;
         const bool in = my_row0 < p.M && col0 < p.N;
-        const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + acc * C::kAccCols + c * 64;
-        uint32_t r[64];
-        tmem_ld32(taddr, *reinterpret_cast<uint32_t(*)[32]>(&r[0]));
-        tmem_ld32(taddr + 32, *reinterpret_cast<uint32_t(*)[32]>(&r[32]));
+        const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + acc * C::kAccCols + team * C::kTeamCols + at;
+        uint32_t r[32];
+        tmem_ld32(taddr, r);
         if constexpr (kGated) {
           if (p.tma_residual) {
             // the next piece's residual, into the buffer that the previous piece's result has left
             if (!p.tma_out) fence_proxy_async_smem();  // it left by plain loads
             if (lane == 0) tma_store_wait_read<0>();
             __syncwarp();
-            if (c + 1 < c1) issue_residual(my_row0, col0 + 64, buf ^ 1);
+            if (c + 1 < C::kTeamPieces) issue_residual(my_row0, col0 + 32, buf ^ 1);
             else if (tile + n_units < total_tiles) issue_residual(row0, tile_col, buf ^ 1);
             if (in) {
               if (!__all_sync(0xffffffffu, mbar_wait_bounded(&res_full[buf], (res_phase >> buf) & 1, abort_flag, kSpinLimit))) {
@@ -396,16 +398,10 @@ __global__ void __launch_bounds__(Int8Cfg<BN, PAIR, EPI>::kThreads, 1) int8_line
           } else {
             if (lane == 0) tma_store_wait_read<1>();
             __syncwarp();
-            // 16-byte chunk j of row r sits at chunk j ^ (r & 7), as TMA lays it out
             for (int i = 0; i < 32 && in; ++i) {
               const long long row = my_row0 + i;
               if (row >= p.M) break;
-#pragma unroll
-              for (int h = 0; h < 64; h += 32) {
-                const int k = h + lane;
-                if (col0 + k < p.N)
-                  *reinterpret_cast<uint16_t*>(stage + i * 128 + (((k >> 3) ^ (i & 7)) << 4) + (k & 7) * 2) = p.residual[row * p.ldr + col0 + k];
-              }
+              if (col0 + lane < p.N) *staged(stage, i, lane) = p.residual[row * p.ldr + col0 + lane];
             }
             __syncwarp();
           }
@@ -414,7 +410,7 @@ __global__ void __launch_bounds__(Int8Cfg<BN, PAIR, EPI>::kThreads, 1) int8_line
           __syncwarp();
         }
         tc_wait_ld();
-        if (c == c1 - 1) {
+        if (c == C::kTeamPieces - 1) {
           // the accumulator is in registers: hand it back to the MMA warp
           tc_fence_before();
           __syncwarp();
@@ -426,7 +422,8 @@ __global__ void __launch_bounds__(Int8Cfg<BN, PAIR, EPI>::kThreads, 1) int8_line
         // Row `lane`: scale, bias, tail, one rounding. What eight columns need is read before the eight ones before are
         // written: the compiler cannot tell that the two do not overlap, and two warps per scheduler hide little of a chain of
         // reads and writes.
-        uint8_t* const own = stage + lane * 128;
+        uint8_t* const own = stage + lane * 64;
+        const int swizzle = (lane >> 1) & 3;
         float4 s4[2], b4[2];
         uint4 x4, g8;
         auto read = [&](int j) {
@@ -437,24 +434,22 @@ __global__ void __launch_bounds__(Int8Cfg<BN, PAIR, EPI>::kThreads, 1) int8_line
           }
           if constexpr (kGated) {
             g8 = *reinterpret_cast<const uint4*>(col_gate + at + j * 8);
-            x4 = *reinterpret_cast<const uint4*>(own + ((j ^ (lane & 7)) << 4));
+            x4 = *reinterpret_cast<const uint4*>(own + ((j ^ swizzle) << 4));
           }
         };
         read(0);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          float v[8];
+        for (int j = 0; j < 4; ++j) {
+          float2 v[4];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t* a4 = &r[j * 8 + h * 4];
-            v[h * 4 + 0] = int8_value(static_cast<int>(a4[0]), my_scale, s4[h].x, b4[h].x);
-            v[h * 4 + 1] = int8_value(static_cast<int>(a4[1]), my_scale, s4[h].y, b4[h].y);
-            v[h * 4 + 2] = int8_value(static_cast<int>(a4[2]), my_scale, s4[h].z, b4[h].z);
-            v[h * 4 + 3] = int8_value(static_cast<int>(a4[3]), my_scale, s4[h].w, b4[h].w);
+          for (int h = 0; h < 4; ++h) {
+            const float4 s = s4[h >> 1], b = b4[h >> 1];
+            v[h] = int8_value2(static_cast<int>(r[j * 8 + h * 2]), static_cast<int>(r[j * 8 + h * 2 + 1]), my_scale,
+                               h & 1 ? make_float2(s.z, s.w) : make_float2(s.x, s.y), h & 1 ? make_float2(b.z, b.w) : make_float2(b.x, b.y));
           }
           if constexpr (EPI == HDIT_GEMM_BIAS_GELU_TANH) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = gelu_tanh_f(v[k]);
+            for (int h = 0; h < 4; ++h) v[h] = int8_gelu2(v[h]);
           } else if constexpr (kGated) {
             const uint16_t* xe = reinterpret_cast<const uint16_t*>(&x4);
             const uint16_t* ge = reinterpret_cast<const uint16_t*>(&g8);
@@ -471,17 +466,18 @@ __global__ void __launch_bounds__(Int8Cfg<BN, PAIR, EPI>::kThreads, 1) int8_line
               }
             }
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = fmaf(g[k], v[k], to_f<FP16>(xe[k]));
+            for (int h = 0; h < 4; ++h)
+              v[h] = fma2(make_float2(g[2 * h], g[2 * h + 1]), v[h], make_float2(to_f<FP16>(xe[2 * h]), to_f<FP16>(xe[2 * h + 1])));
           }
-          if (j < 7) read(j + 1);
-          *reinterpret_cast<uint4*>(own + ((j ^ (lane & 7)) << 4)) =
-              make_uint4(pack2<FP16>(v[0], v[1]), pack2<FP16>(v[2], v[3]), pack2<FP16>(v[4], v[5]), pack2<FP16>(v[6], v[7]));
+          if (j < 3) read(j + 1);
+          *reinterpret_cast<uint4*>(own + ((j ^ swizzle) << 4)) =
+              make_uint4(pack2<FP16>(v[0].x, v[0].y), pack2<FP16>(v[1].x, v[1].y), pack2<FP16>(v[2].x, v[2].y), pack2<FP16>(v[3].x, v[3].y));
         }
         if (p.tma_out) {
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
-            if (in) tma_store_2d(&p.out_map, stage, col0, static_cast<int>(my_row0));
+            if (in) tma_store_2d(&p.out_map, stage, col0, my_row0);
             tma_store_commit();
           }
         } else {
@@ -489,12 +485,7 @@ __global__ void __launch_bounds__(Int8Cfg<BN, PAIR, EPI>::kThreads, 1) int8_line
           for (int i = 0; i < 32 && in; ++i) {
             const long long row = my_row0 + i;
             if (row >= p.M) break;
-#pragma unroll
-            for (int h = 0; h < 64; h += 32) {
-              const int k = h + lane;
-              if (col0 + k < p.N)
-                p.out[row * p.ldo + col0 + k] = *reinterpret_cast<const uint16_t*>(stage + i * 128 + (((k >> 3) ^ (i & 7)) << 4) + (k & 7) * 2);
-            }
+            if (col0 + lane < p.N) p.out[row * p.ldo + col0 + lane] = *staged(stage, i, lane);
           }
           __syncwarp();
         }
@@ -542,10 +533,10 @@ int encode_pieces(CUtensorMap* map, const void* ptr, long long rows, long long n
   if (enc == nullptr) return set_error(HDIT_ERR_CUDA, "cuTensorMapEncodeTiled entry point unavailable");
   cuuint64_t dims[2] = {static_cast<cuuint64_t>(n), static_cast<cuuint64_t>(rows)};
   cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * 2};
-  cuuint32_t box[2] = {64, 32};
+  cuuint32_t box[2] = {32, 32};
   cuuint32_t estr[2] = {1, 1};
   const CUtensorMapDataType dt = dtype == HDIT_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  const CUresult r = enc(map, dt, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+  const CUresult r = enc(map, dt, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B,
                          CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
     return set_error(HDIT_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d (rows=%lld n=%lld ld=%lld)", static_cast<int>(r), rows, n, ld);
