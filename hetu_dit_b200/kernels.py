@@ -954,9 +954,9 @@ class Int8Rows:
 
 def _empty_int8_rows(x, lead, k):
     """Int8Rows for rows of x's type on its device, rows on 16-byte boundaries."""
-    pitch = (k + 15) & ~15
-    q = x.new_empty((*lead, pitch), dtype=torch.int8)
-    return Int8Rows(q if pitch == k else q[..., :k], x.new_empty(lead, dtype=torch.float32), x.dtype)
+    pitch, dev = (k + 15) & ~15, x.device
+    q = torch.empty(*lead, pitch, dtype=torch.int8, device=dev)
+    return Int8Rows(q if pitch == k else q[..., :k], torch.empty(*lead, dtype=torch.float32, device=dev), x.dtype)
 
 
 def quantize_rows(x):
@@ -1071,7 +1071,7 @@ def linear_int8(x, weight, bias=None, epilogue="bias", residual=None, gate=None,
         if gate.shape != (B, n) or (gate.stride(1) != 1 and n != 1) or gate.dtype != dtype or gate.device != dev:
             raise ValueError("gate must be (B, N) of x's dtype, on its device")
     if out is None:
-        out, so = w.new_empty((B, S, n), dtype=dtype), n
+        out, so = torch.empty(B, S, n, dtype=dtype, device=dev), n
     else:
         if out.shape != (B, S, n) or out.dtype != dtype or out.device != dev or (out.stride(2) != 1 and n != 1):
             raise ValueError("out does not match (B, S, N), x's dtype or its device")
