@@ -308,7 +308,7 @@ template <bool FP16, bool SILU, int TEAM, int NCH, int THREADS>
 __device__ __forceinline__ void row_to_int8(const GnParams& p, const Team<TEAM, THREADS>& team, int turn, const uint4 (&raw)[NCH], const float4* factors,
                                             int c0, long long row, bool live) {
   const int chunks = p.channels / 8;
-  float y[NCH][8];
+  float2 y[NCH][4];
   float top = 0.f;
 #pragma unroll
   for (int k = 0; k < NCH; ++k) {
@@ -316,18 +316,11 @@ __device__ __forceinline__ void row_to_int8(const GnParams& p, const Team<TEAM, 
     if (c >= p.channels) continue;
     const uint32_t* u = reinterpret_cast<const uint32_t*>(&raw[k]);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const float4 av = factors[h * chunks + (c >> 3)], bv = factors[(2 + h) * chunks + (c >> 3)];
-      const float2 v0 = int8_unpack2<FP16>(u[2 * h]), v1 = int8_unpack2<FP16>(u[2 * h + 1]);
-      y[k][4 * h] = fmaf(v0.x, av.x, bv.x);
-      y[k][4 * h + 1] = fmaf(v0.y, av.y, bv.y);
-      y[k][4 * h + 2] = fmaf(v1.x, av.z, bv.z);
-      y[k][4 * h + 3] = fmaf(v1.y, av.w, bv.w);
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if constexpr (SILU) y[k][i] = silu(y[k][i]);
-      top = max_magnitude(top, y[k][i]);
+    for (int i = 0; i < 4; ++i) {
+      const float4 av = factors[(i >> 1) * chunks + (c >> 3)], bv = factors[(2 + (i >> 1)) * chunks + (c >> 3)];
+      y[k][i] = fma2(int8_unpack2<FP16>(u[i]), i & 1 ? make_float2(av.z, av.w) : make_float2(av.x, av.y), i & 1 ? make_float2(bv.z, bv.w) : make_float2(bv.x, bv.y));
+      if constexpr (SILU) y[k][i] = make_float2(silu(y[k][i].x), silu(y[k][i].y));
+      top = max_magnitude(max_magnitude(top, y[k][i].x), y[k][i].y);
     }
   }
   const Int8Scale s = int8_scale(team.max(__float_as_uint(top) & 0x7FFFFFFFu, turn));

@@ -106,16 +106,8 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtas) int8_linear_few_kernel(
       const float inv17 = 17.f * s.inv;
       const uint16_t* xr = p.x + m / p.x_rows_per_batch * p.x_batch_stride + m % p.x_rows_per_batch * p.x_row_stride;
       for (int c = threadIdx.x * 8; c < p.pitch; c += kFewThreads * 8) {
-        float y[8];
         const uint4 raw = c < p.K ? int8_load8(xr, c, p.K, p.vec) : make_uint4(0, 0, 0, 0);
-        const uint32_t* u = reinterpret_cast<const uint32_t*>(&raw);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 v = int8_unpack2<FP16>(u[i]);
-          y[2 * i] = int8_steps_of_16bit(v.x, s.inv, inv17);
-          y[2 * i + 1] = int8_steps_of_16bit(v.y, s.inv, inv17);
-        }
-        int8_put8(reinterpret_cast<int8_t*>(rows8) + m * p.pitch, c, s, y);
+        int8_put8<FP16>(reinterpret_cast<int8_t*>(rows8) + m * p.pitch, c, s, inv17, raw);
       }
       if (threadIdx.x == 0) row_scale[m] = int8_step(s);
     }

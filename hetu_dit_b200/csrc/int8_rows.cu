@@ -101,42 +101,32 @@ __global__ void __launch_bounds__(kRowThreads, rows_ctas(NCH, LN)) int8_rows_ker
 #pragma unroll
         for (int c = 0; c < NCH; ++c) {
           if (col0 + c * TEAM * 8 >= p.dim) continue;
-          const uint32_t* u = reinterpret_cast<const uint32_t*>(&raw[c]);
-          float t[8];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 v = int8_unpack2<FP16>(u[i]);
-            t[2 * i] = int8_steps_of_16bit(v.x, s.inv, inv17);
-            t[2 * i + 1] = int8_steps_of_16bit(v.y, s.inv, inv17);
-          }
-          int8_put8(qr, col0 + c * TEAM * 8, s, t);
+          int8_put8<FP16>(qr, col0 + c * TEAM * 8, s, inv17, raw[c]);
         }
       } else {
-        float y[NCH][8];  // x, its distance from the mean, the result
-        float sum = 0.f;
+        float2 y[NCH][4];  // x, its distance from the mean, the result
+        float2 sum = both(0.f);
 #pragma unroll
         for (int c = 0; c < NCH; ++c) {
           const uint32_t* u = reinterpret_cast<const uint32_t*>(&raw[c]);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float2 v = int8_unpack2<FP16>(u[i]);
-            y[c][2 * i] = v.x;
-            y[c][2 * i + 1] = v.y;
-            sum += v.x + v.y;
+            y[c][i] = int8_unpack2<FP16>(u[i]);
+            sum = add2(sum, y[c][i]);
           }
         }
-        const float mean = team.sum(sum, 0) * inv_dim;
-        float sq = 0.f;
+        const float mean = team.sum(sum.x + sum.y, 0) * inv_dim;
+        float2 sq = both(0.f);
 #pragma unroll
         for (int c = 0; c < NCH; ++c)
           if (col0 + c * TEAM * 8 < p.dim) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              y[c][i] -= mean;
-              sq = fmaf(y[c][i], y[c][i], sq);
+            for (int i = 0; i < 4; ++i) {
+              y[c][i] = add2(y[c][i], both(-mean));
+              sq = fma2(y[c][i], y[c][i], sq);
             }
           }
-        const float rstd = rsqrtf(team.sum(sq, 1) * inv_dim + p.eps);
+        const float rstd = rsqrtf(team.sum(sq.x + sq.y, 1) * inv_dim + p.eps);
         float top = 0.f;
 #pragma unroll
         for (int c = 0; c < NCH; ++c) {
@@ -145,14 +135,12 @@ __global__ void __launch_bounds__(kRowThreads, rows_ctas(NCH, LN)) int8_rows_ker
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const float4 g = mods[h * chunks + (col >> 3)], a = mods[(2 + h) * chunks + (col >> 3)];
-            float* v = &y[c][4 * h];
-            v[0] = fmaf(v[0] * rstd, g.x, a.x);
-            v[1] = fmaf(v[1] * rstd, g.y, a.y);
-            v[2] = fmaf(v[2] * rstd, g.z, a.z);
-            v[3] = fmaf(v[3] * rstd, g.w, a.w);
+            float2* v = &y[c][2 * h];
+            v[0] = fma2(mul2(v[0], both(rstd)), make_float2(g.x, g.y), make_float2(a.x, a.y));
+            v[1] = fma2(mul2(v[1], both(rstd)), make_float2(g.z, g.w), make_float2(a.z, a.w));
           }
 #pragma unroll
-          for (int i = 0; i < 8; ++i) top = max_magnitude(top, y[c][i]);
+          for (int i = 0; i < 4; ++i) top = max_magnitude(max_magnitude(top, y[c][i].x), y[c][i].y);
         }
         s = int8_scale(team.max(__float_as_uint(top) & 0x7FFFFFFFu, 2));
 #pragma unroll
@@ -182,10 +170,14 @@ __global__ void __launch_bounds__(kRowThreads) int8_any_rows_kernel(const __grid
       const Int8Scale s = int8_scale(__float_as_uint(int8_unpack2<FP16>(team.max(top, turn)).x));
       const float inv17 = 17.f * s.inv;
       for (int c = threadIdx.x * 4; c < p.dim; c += kRowThreads * 4) {
-        float t[4];
+        float2 t[2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) t[i] = c + i < p.dim && s.inv != 0.f ? int8_steps_of_16bit(int8_unpack2<FP16>(xr[c + i]).x, s.inv, inv17) : 0.f;
-        const uint32_t v = int8_pack4(t[0], t[1], t[2], t[3]);
+        for (int i = 0; i < 2; ++i) {
+          const float2 v = make_float2(c + 2 * i < p.dim ? int8_unpack2<FP16>(xr[c + 2 * i]).x : 0.f,
+                                       c + 2 * i + 1 < p.dim ? int8_unpack2<FP16>(xr[c + 2 * i + 1]).x : 0.f);
+          t[i] = add2(int8_steps_of_16bit(v, s.inv, inv17), both(kInt8Round));
+        }
+        const uint32_t v = s.inv == 0.f ? 0u : int8_bytes(t[0], t[1]);
         if (c + 4 <= p.dim) {
           *reinterpret_cast<uint32_t*>(qr + c) = v;
         } else {

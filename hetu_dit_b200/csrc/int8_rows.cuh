@@ -6,6 +6,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "ptx_sm100.cuh"
+
 namespace hdit {
 namespace {
 
@@ -31,24 +33,22 @@ __device__ __forceinline__ float int8_step(const Int8Scale& s) {
 
 constexpr float kInt8Round = 1.5f * 8388608.f;
 
-// Adding 1.5 * 2^23 rounds to the nearest integer, ties to even, and leaves it in the low bits as two's complement; the
-// low bytes of four of them are packed.
-__device__ __forceinline__ uint32_t int8_pack4(float a, float b, float c, float d) {
-  const uint32_t ua = __float_as_uint(__fadd_rn(a, kInt8Round)), ub = __float_as_uint(__fadd_rn(b, kInt8Round));
-  const uint32_t uc = __float_as_uint(__fadd_rn(c, kInt8Round)), ud = __float_as_uint(__fadd_rn(d, kInt8Round));
-  return __byte_perm(__byte_perm(ua, ub, 0x0040), __byte_perm(uc, ud, 0x0040), 0x5410);
+// Adding 1.5 * 2^23 rounds to the nearest integer, ties to even, and leaves it in the low bits as two's complement; the low
+// bytes of four of them are packed.
+__device__ __forceinline__ uint32_t int8_bytes(float2 a, float2 b) {
+  return __byte_perm(__byte_perm(__float_as_uint(a.x), __float_as_uint(a.y), 0x0040), __byte_perm(__float_as_uint(b.x), __float_as_uint(b.y), 0x0040), 0x5410);
 }
 
 // v / s for a 16-bit v, exact at the borders between two integers. 254 v - (2 n + 1) max is a whole number of units in the
 // last place of v (v <= max), so 127 v / max is n + 1/2 or at least 2^-19 of its size away from it (v has at most 11 bits);
 // v * inv is within 2^-24 of the quotient. The sum below is v * inv rounded to 20 bits (Dekker's splitting: both terms are
 // multiples of 16 units of the quotient's last place, the second one rounds the exact difference), which moves it by 2^-20 at
-// most: that restores n + 1/2 (8 bits) exactly and brings nothing else onto it or across. inv17 = 17 * inv. Three operations of
-// the FMA pipe; on the bits, (bits + 8) & ~15 behind the product, two of them would be the integer pipe's, which the packing
-// needs.
-__device__ __forceinline__ float int8_steps_of_16bit(float v, float inv, float inv17) {
-  const float p = __fmul_rn(v, inv17);
-  return __fadd_rn(p, __fmaf_rn(v, inv, -p));
+// most: that restores n + 1/2 (8 bits) exactly and brings nothing else onto it or across. inv17 = 17 * inv. Operations
+// on two values an instruction; on the bits, (bits + 8) & ~15 behind the product, it would take the integer pipe twice, which the
+// packing needs.
+__device__ __forceinline__ float2 int8_steps_of_16bit(float2 v, float inv, float inv17) {
+  const float2 p = mul2(v, both(inv17));
+  return add2(p, fma2(v, both(inv), make_float2(-p.x, -p.y)));
 }
 
 template <bool FP16>
@@ -110,21 +110,25 @@ struct Team {
   }
 };
 
-// Eight values in units of the row's step to column c of the row, which is on an 8-byte boundary; zeros where the row has no
-// step (an infinity times 0 is none).
-__device__ __forceinline__ void int8_put8(int8_t* row, int c, const Int8Scale& s, const float (&t)[8]) {
-  uint2 v = make_uint2(int8_pack4(t[0], t[1], t[2], t[3]), int8_pack4(t[4], t[5], t[6], t[7]));
+// Eight 16-bit values to column c of the row, which is on an 8-byte boundary; zeros where the row has no step (an infinity
+// times 0 is none).
+template <bool FP16>
+__device__ __forceinline__ void int8_put8(int8_t* row, int c, const Int8Scale& s, float inv17, const uint4& raw) {
+  const uint32_t* u = reinterpret_cast<const uint32_t*>(&raw);
+  float2 t[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) t[i] = add2(int8_steps_of_16bit(int8_unpack2<FP16>(u[i]), s.inv, inv17), both(kInt8Round));
+  uint2 v = make_uint2(int8_bytes(t[0], t[1]), int8_bytes(t[2], t[3]));
   if (s.inv == 0.f) v = make_uint2(0, 0);
   *reinterpret_cast<uint2*>(row + c) = v;
 }
 
-// The same for eight values: product with inv and rounding to an integer in one operation.
-__device__ __forceinline__ void int8_put8_of(int8_t* row, int c, const Int8Scale& s, const float (&y)[8]) {
-  uint32_t u[8];
+// The same for fp32 values: product with inv and rounding to an integer in one operation.
+__device__ __forceinline__ void int8_put8_of(int8_t* row, int c, const Int8Scale& s, const float2 (&y)[4]) {
+  float2 t[4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) u[i] = __float_as_uint(__fmaf_rn(y[i], s.inv, kInt8Round));
-  uint2 v = make_uint2(__byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410),
-                       __byte_perm(__byte_perm(u[4], u[5], 0x0040), __byte_perm(u[6], u[7], 0x0040), 0x5410));
+  for (int i = 0; i < 4; ++i) t[i] = fma2(y[i], both(s.inv), both(kInt8Round));
+  uint2 v = make_uint2(int8_bytes(t[0], t[1]), int8_bytes(t[2], t[3]));
   if (s.inv == 0.f) v = make_uint2(0, 0);
   *reinterpret_cast<uint2*>(row + c) = v;
 }
