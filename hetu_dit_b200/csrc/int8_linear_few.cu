@@ -191,7 +191,14 @@ int launch_few(const FewParams& p, cudaStream_t st) {
 bool int8_linear_few_takes(const hdit_int8_linear_args* a) {
   return a->m <= kInt8FewRows && a->m * few_pitch(a->k) <= 160 * 1024;
 }
-bool int8_linear_few_quantizes(const hdit_int8_linear_args* a) { return a->m <= kOwnRows; }
+// Not where the result may take x's place (x = residual = out): a CTA would write what another one has yet to read.
+bool int8_linear_few_quantizes(const hdit_int8_linear_args* a) {
+  if (a->m > kOwnRows) return false;
+  const int64_t per = a->x_rows_per_batch < a->m ? a->x_rows_per_batch : a->m, entries = (a->m + per - 1) / per;
+  const uintptr_t x0 = reinterpret_cast<uintptr_t>(a->x), x1 = x0 + 2 * ((entries - 1) * a->x_batch_stride + (per - 1) * a->x_row_stride + a->k);
+  const uintptr_t o0 = reinterpret_cast<uintptr_t>(a->out), o1 = o0 + 2 * ((a->m - 1) * a->ldo + a->n);
+  return x1 <= o0 || o1 <= x0;
+}
 
 int int8_linear_few(const hdit_int8_linear_args* a) {
   FewParams p{};

@@ -238,6 +238,23 @@ def test_few_rows_give_the_bits_of_a_tile(B, S, K, N, epilogue):
         assert torch.equal(tile, kernels.linear_int8(rows, w, b, epilogue, residual=res, gate=gate, tile=5))
 
 
+@pytest.mark.parametrize("B,S", [(1, 1), (2, 1), (1, 2), (1, 5), (1, 40)])
+def test_result_in_the_place_of_x(B, S):
+    """x = residual = out: a block's residual written over its input."""
+    from hetu_dit_b200 import kernels
+    x, w, b, _, gate = _layer(B, S, 4096, 4096, torch.bfloat16, 50 + S)
+    want = kernels.linear_int8(x, w, b, "gate_residual", residual=x, gate=gate)
+    for _ in range(20):
+        y = x.clone()
+        assert kernels.linear_int8(y, w, b, "gate_residual", residual=y, gate=gate, out=y) is y
+        assert torch.equal(y, want)
+    wide = torch.zeros(B, S, 5000, dtype=torch.bfloat16, device=DEV)
+    wide[..., 8:4104] = x
+    out = wide[..., 904:]
+    kernels.linear_int8(wide[..., 8:4104], w, b, out=out)  # the result over a part of x
+    assert torch.equal(out, kernels.linear_int8(x, w, b))
+
+
 def test_linear_int8_sums_are_exact_at_the_largest_k():
     """Rows of the largest and smallest integers only: a sum of 127 * 127 * 131072 fits 32 bits."""
     from hetu_dit_b200 import kernels
