@@ -10,7 +10,7 @@
 //
 // us, this kernel | 128 x 128 tiles, 8-bit rows: 9216 x 1536, 1 row 4.4 | 7.8, 8 rows 6.2 | 7.6, 16 rows 9.1 | 7.6 (as two column
 // tiles); 18432 x 3072, 1 row 12.4 | 16.2, 8 rows 16.1 | 16.0: taken for up to eight rows. One or two 16-bit rows are brought into 8
-// bits by every CTA for itself, which saves a launch: 1 row 5.3, 2 rows 6.5 and 3 us less on the host; with 4 rows it took 9.0, with
+// bits by every CTA for itself, which saves a launch: 1 row 4.6, 2 rows 6.5 and 3 us less on the host; with 4 rows it took 9.0, with
 // quantize_rows before it 7.2.
 #include "gemm_common.cuh"
 #include "host_common.h"

@@ -9,7 +9,9 @@
 //
 //   epilogue     per 32 x 32 piece of a warp, a lane to a row: scales, bias and gate of the warp's columns wait in shared
 //                memory (they are fetched while the tile before is worked on), the residual's piece comes into the staging
-//                buffer by TMA one piece ahead, the result takes its place there and leaves by TMA. Two staging buffers.
+//                buffer by TMA one piece ahead, the result takes its place there and leaves by TMA. Sixteen warps for 256 columns:
+//                with eight over pieces of 64 columns a scheduler had two to hide the chain TMEM - scales - staging behind, 3.5 k
+//                cycles a tile instead of 2.9 k (16384 x 512 -> 1536 19.9 us, now 18.0).
 //
 // All waits are bounded, see gemm_sm100.cu.
 #include <math.h>
@@ -114,8 +116,8 @@ struct Int8Cfg {
   static constexpr int kBBytes = kBRows * kTileKBytes;
   static constexpr int kStageBytes = kABytes + kBBytes;
   // pieces of 32 rows x 32 columns of 16 bits per epilogue warp: two where a residual comes in beside the result that leaves.
-  // One more costs a stage of the ring, which 256 columns miss more: 4608 x 12288 x 3072 + GELU takes 137 us with 4 stages and
-  // two buffers, 124 with 6 and one.
+  // A second buffer costs a stage or two of the ring, which 256 columns miss more: 4608 x 12288 x 3072 + GELU took 137 us with 4
+  // stages and two buffers (of 64 columns), 124 with 6 and one.
   static constexpr int kBufs = EPI == HDIT_GEMM_BIAS_GATE_RESIDUAL ? 2 : 1;
   static constexpr int kStagingBytes = kEpiWarps * kBufs * kPieceBytes;
   // barriers and the columns' scales, bias and gate: what is left of 227 KB beside six stages of 32 KB and one piece per warp
@@ -599,10 +601,16 @@ extern "C" int hdit_int8_linear(const hdit_int8_linear_args* a) {
   if (a->m > 0x7fffff00LL || a->n > 0x7fffff00LL) return set_error(HDIT_ERR_TOO_LARGE, "m and n must fit 31 bits");
   if (a->k > HDIT_INT8_MAX_K) return set_error(HDIT_ERR_TOO_LARGE, "k above %d could overflow the 32-bit sums", HDIT_INT8_MAX_K);
   if (a->m == 0) return HDIT_OK;
-  if (a->a == nullptr || a->a_scale == nullptr || a->w == nullptr || a->w_scale == nullptr || a->out == nullptr)
-    return set_error(HDIT_ERR_BAD_ARG, "null a / w / scale / out");
+  if (a->w == nullptr || a->w_scale == nullptr || a->out == nullptr) return set_error(HDIT_ERR_BAD_ARG, "null w / scale / out");
+  if (a->x != nullptr && (a->x_rows_per_batch <= 0 || (reinterpret_cast<uintptr_t>(a->x) & 1) != 0))
+    return set_error(HDIT_ERR_BAD_ARG, "x needs x_rows_per_batch > 0 and the alignment of its elements");
+  if (a->tile < 0 || a->tile > 5) return set_error(HDIT_ERR_BAD_ARG, "tile must be 0 (choose) to 5");
+  if (a->tile == 5 && !int8_linear_few_takes(a)) return set_error(HDIT_ERR_SHAPE, "too many rows, or too long ones, for the kernel for a few rows");
+  const bool few = a->tile == 5 || (a->tile == 0 && int8_linear_few_takes(a));
+  const bool own_rows = few && a->x != nullptr && int8_linear_few_quantizes(a);  // a and a_scale are not used
+  if (!own_rows && (a->a == nullptr || a->a_scale == nullptr)) return set_error(HDIT_ERR_BAD_ARG, "null a / a_scale");
   auto bad_rows = [&](const void* ptr, long long ld) { return (reinterpret_cast<uintptr_t>(ptr) & 15) != 0 || ld % 16 != 0 || ld < a->k; };
-  if (bad_rows(a->a, a->lda) || bad_rows(a->w, a->ldw))
+  if ((!own_rows && bad_rows(a->a, a->lda)) || bad_rows(a->w, a->ldw))
     return set_error(HDIT_ERR_SHAPE, "8-bit rows need a 16-byte aligned pointer and a row stride that is a multiple of 16 and covers a row");
   if (((reinterpret_cast<uintptr_t>(a->a_scale) | reinterpret_cast<uintptr_t>(a->w_scale)) & 3) != 0 ||
       ((reinterpret_cast<uintptr_t>(a->out) | reinterpret_cast<uintptr_t>(a->bias) | reinterpret_cast<uintptr_t>(a->residual) |
@@ -613,8 +621,6 @@ extern "C" int hdit_int8_linear(const hdit_int8_linear_args* a) {
   if (gated && (a->residual == nullptr || a->gate == nullptr || a->rows_per_batch <= 0))
     return set_error(HDIT_ERR_BAD_ARG, "the gated-residual epilogue needs residual, gate and rows_per_batch > 0");
   if (gated && a->ldr < a->n) return set_error(HDIT_ERR_SHAPE, "rows of residual overlap");
-  if (a->x != nullptr && (a->x_rows_per_batch <= 0 || (reinterpret_cast<uintptr_t>(a->x) & 1) != 0))
-    return set_error(HDIT_ERR_BAD_ARG, "x needs x_rows_per_batch > 0 and the alignment of its elements");
   Int8Params p;
   memset(&p, 0, sizeof(p));
   p.M = static_cast<int>(a->m);
@@ -635,10 +641,7 @@ extern "C" int hdit_int8_linear(const hdit_int8_linear_args* a) {
   p.tma_residual = gated && whole(a->residual, a->ldr);
   p.status = device_status_ptr();
   if (p.status == nullptr) return HDIT_ERR_CUDA;
-  if (a->tile < 0 || a->tile > 5) return set_error(HDIT_ERR_BAD_ARG, "tile must be 0 (choose) to 5");
-  if (a->tile == 5 && !int8_linear_few_takes(a)) return set_error(HDIT_ERR_SHAPE, "too many rows, or too long ones, for the kernel for a few rows");
-  const bool few = a->tile == 5 || (a->tile == 0 && int8_linear_few_takes(a));
-  if (a->x != nullptr && !(few && int8_linear_few_quantizes(a))) {
+  if (a->x != nullptr && !own_rows) {
     // 16-bit rows: into 8 bits first, in the caller's a / a_scale
     const int rc = hdit_quantize_rows(a->dtype, a->x, const_cast<void*>(a->a), const_cast<float*>(a->a_scale), a->m, a->k, a->x_rows_per_batch,
                                       a->x_batch_stride, a->x_row_stride, a->lda, a->stream);
@@ -647,15 +650,19 @@ extern "C" int hdit_int8_linear(const hdit_int8_linear_args* a) {
   if (few) return int8_linear_few(a);
   int tile = a->tile;
   if (tile == 0) {
-    // Fewest waves, each weighted by a tile's time relative to 128 x 128 of output per SM
+    // Fewest waves, each weighted by a tile's time relative to 128 x 128 of output per SM (0.145 us per 128 of K), as for the 16-bit
+    // layers, whose operands take as many bytes per clock; a pair starts 0.3 us later. us with 128 x 128, 256 x 128, 256 x 192, 256 x 256:
+    // 154 x 1536 -> 1536 5.7, 5.9, 7.1, 8.4; 512 x 12288 -> 3072 25.5, 22.5, 28.3, 34.2; 2192 x 3072 -> 3072 19.3, 18.3, 16.9, 19.8; 8192 x
+    // 1536 -> 4608 54, 50, 45, 43; 16384 x 512 -> 512 10.7, 10.7, 10.2, 9.5. Over 24 shapes the choice is 2 % from the best.
     const long long sms = a->max_ctas > 0 ? a->max_ctas : sm_count();
     struct Cand { int tile, rows, cols, units_div; double per_tile; };
     const Cand cand[4] = {{1, 128, 128, 1, 1.25}, {2, 256, 128, 2, 1.2}, {3, 256, 192, 2, 1.725}, {4, 256, 256, 2, 2.1}};
+    const double pair_start = 2.0 / p.k_blocks;
     double best = -1.0;
     for (const Cand& c : cand) {
       const long long units = sms / c.units_div > 0 ? sms / c.units_div : 1;
       const long long tiles = ((a->m + c.rows - 1) / c.rows) * ((a->n + c.cols - 1) / c.cols);
-      const double cost = static_cast<double>((tiles + units - 1) / units) * c.per_tile;
+      const double cost = static_cast<double>((tiles + units - 1) / units) * c.per_tile + (c.units_div == 2 ? pair_start : 0.0);
       if (best < 0 || cost < best) best = cost, tile = c.tile;
     }
   }

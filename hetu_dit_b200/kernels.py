@@ -938,25 +938,52 @@ class Int8Rows:
     """Rows of 16-bit values held in 8 bits: row r stands for q[r] * scale[r]. q: (..., K) int8, K contiguous, rows on 16-byte
     boundaries (quantize_rows() lays them out so); scale: (...) fp32, contiguous; dtype: the 16-bit type of what they stand
     for, and of what a layer computes from them. A linear layer's weight (N, K) has a row per output channel."""
-    __slots__ = ("q", "scale", "dtype")
+    __slots__ = ("_q", "_scale", "dtype", "_buf", "_laid")
 
     def __init__(self, q, scale, dtype=torch.bfloat16):
-        self.q, self.scale, self.dtype = q, scale, dtype
+        self._q, self._scale, self.dtype, self._laid = q, scale, dtype, None
 
-    shape = property(lambda self: self.q.shape)
-    device = property(lambda self: self.q.device)
-    is_cuda = property(lambda self: self.q.is_cuda)
+    @classmethod
+    def _empty(cls, lead, k, dtype, device):
+        """Rows that a kernel is about to fill: integers `pitch` bytes apart and behind them the scales, in one allocation;
+        the two tensors are made when someone asks for them. _laid: (leading sizes, K, pitch, rows, device)."""
+        r = cls.__new__(cls)
+        rows, pitch = lead[0] * lead[1] if len(lead) == 2 else lead[0], (k + 15) & ~15
+        r._q = r._scale = None
+        r.dtype, r._laid = dtype, (lead, k, pitch, rows, device)
+        r._buf = torch.empty(rows * (pitch + 4), dtype=torch.int8, device=device)
+        return r
+
+    @property
+    def q(self):
+        if self._q is None:
+            lead, k, pitch, rows, _ = self._laid
+            q = self._buf[:rows * pitch].view(*lead, pitch)
+            self._q = q if pitch == k else q[..., :k]
+        return self._q
+
+    @property
+    def scale(self):
+        if self._scale is None:
+            lead, _, pitch, rows, _ = self._laid
+            self._scale = self._buf[rows * pitch:].view(torch.float32).view(lead)
+        return self._scale
+
+    @property
+    def shape(self):
+        return self.q.shape if self._laid is None else torch.Size((*self._laid[0], self._laid[1]))
+
+    @property
+    def device(self):
+        return self._q.device if self._laid is None else self._laid[4]
+
+    @property
+    def is_cuda(self):
+        return self._q.is_cuda if self._laid is None else self._buf.is_cuda
 
     def dequantize(self):
         """The values as a tensor of `dtype`."""
         return (self.q.float() * self.scale[..., None]).to(self.dtype)
-
-
-def _empty_int8_rows(x, lead, k):
-    """Int8Rows for rows of x's type on its device, rows on 16-byte boundaries."""
-    pitch, dev = (k + 15) & ~15, x.device
-    q = torch.empty(*lead, pitch, dtype=torch.int8, device=dev)
-    return Int8Rows(q if pitch == k else q[..., :k], torch.empty(*lead, dtype=torch.float32, device=dev), x.dtype)
 
 
 def quantize_rows(x):
@@ -978,13 +1005,14 @@ def quantize_rows(x):
         raise ValueError("expected (B, S, K) or (rows, K)")
     if k == 0 or (sk != 1 and k != 1):
         raise ValueError("expected (B, S, K) or (rows, K) with contiguous K")
-    out = _empty_int8_rows(x, lead, k)
-    if B * S == 0:
+    dev, rows, pitch = x.device, B * S, (k + 15) & ~15
+    out = Int8Rows._empty(lead, k, dtype, dev)
+    if rows == 0:
         return out
-    dev = x.device
+    ptr = out._buf.data_ptr()
     with _on(dev):
-        _C.check(_C.lib().hdit_quantize_rows(_DTYPE_CODE[dtype], x.data_ptr(), out.q.data_ptr(), out.scale.data_ptr(), B * S, k, S,
-                                             sb, ss, (k + 15) & ~15, _stream_ptr(dev)))
+        _C.check(_C.lib().hdit_quantize_rows(_DTYPE_CODE[dtype], x.data_ptr(), ptr, ptr + rows * pitch, rows, k, S, sb, ss, pitch,
+                                             _stream_ptr(dev)))
     _count()
     return out
 
@@ -1006,13 +1034,14 @@ def ln_modulate_int8(x, shift, scale, eps=1e-6):
         raise ValueError("shift / scale must be (B, Dm) views with contiguous last dim and equal batch stride")
     if shift.device != dev or scale.device != dev:
         raise ValueError("x, shift and scale must be on one device")
-    out = _empty_int8_rows(x, (B, S), dim)
-    if B * S == 0:
+    rows, pitch = B * S, (dim + 15) & ~15
+    out = Int8Rows._empty((B, S), dim, dtype, dev)
+    if rows == 0:
         return out
+    ptr = out._buf.data_ptr()
     with _on(dev):
-        _C.check(_C.lib().hdit_ln_modulate_int8(_DTYPE_CODE[dtype], x.data_ptr(), shift.data_ptr(), scale.data_ptr(),
-                                                out.q.data_ptr(), out.scale.data_ptr(), B * S, dim, S, sb, ss, (dim + 15) & ~15,
-                                                mod[0], eps, _stream_ptr(dev)))
+        _C.check(_C.lib().hdit_ln_modulate_int8(_DTYPE_CODE[dtype], x.data_ptr(), shift.data_ptr(), scale.data_ptr(), ptr,
+                                                ptr + rows * pitch, rows, dim, S, sb, ss, pitch, mod[0], eps, _stream_ptr(dev)))
     _count()
     return out
 
@@ -1028,9 +1057,15 @@ def linear_int8(x, weight, bias=None, epilogue="bias", residual=None, gate=None,
     16-bit type once. B, S, K, N need not be multiples of anything. `out` may be a column block of a wider buffer, or
     `residual` itself."""
     held = type(x) is Int8Rows
-    xr = x.q if held else x
+    laid = x._laid if held else None  # rows that a kernel of this module has laid out need no look at their tensors
+    if laid is not None:
+        lead, k, ss, m, dev = laid
+        shape, xr = (*lead, k), x._buf
+    else:
+        xr = x.q if held else x
+        shape, dev = xr.shape, xr.device
     _require_cuda(xr)
-    dtype, dev, shape = x.dtype, xr.device, xr.shape
+    dtype = x.dtype
     if dtype not in _DTYPE_CODE:
         raise TypeError(f"unsupported dtype {dtype}")
     tail = _TAILS.get(epilogue)
@@ -1045,21 +1080,25 @@ def linear_int8(x, weight, bias=None, epilogue="bias", residual=None, gate=None,
     w, w_scale = weight.q, weight.scale
     if len(shape) != 3 or w.dim() != 2:
         raise ValueError("x must be (B, S, K) or (rows, K), weight (N, K)")
-    (B, S, k), (n, kw), (sb, ss, sk), (wn, wk) = shape, w.shape, xr.stride(), w.stride()
+    (B, S, k), (n, kw), (wn, wk) = shape, w.shape, w.stride()
     m, pitch, w_ptr = B * S, (k + 15) & ~15, w.data_ptr()
     if k != kw or k == 0 or n == 0 or w.dtype != torch.int8 or w.device != dev or w_scale.dtype != torch.float32 or \
             w_scale.device != dev or w_scale.shape != (n,) or not w_scale.is_contiguous():
         raise ValueError("weight must be (N, K) int8 with N contiguous fp32 scales, on x's device")
     if (wk != 1 and k != 1) or (wn % 16 and n != 1) or w_ptr % 16:
         raise ValueError("weight rows must be contiguous and start on 16-byte boundaries, as quantize_rows() lays them out")
-    if sk != 1 and k != 1:
-        raise ValueError("x must have contiguous K")
-    if held:
-        scale = x.scale
-        if xr.dtype != torch.int8 or scale.dtype != torch.float32 or scale.shape != (B, S) or scale.device != dev:
-            raise ValueError("x must be int8 with a fp32 scale for each row, on one device")
-        if (ss % 16 and S != 1) or (sb % 16 and B != 1) or xr.data_ptr() % 16:
-            raise ValueError("x's rows must start on 16-byte boundaries, as quantize_rows() lays them out")
+    one_pitch = True  # a row stride for the rows of all entries
+    if laid is None:
+        sb, ss, sk = xr.stride()
+        if sk != 1 and k != 1:
+            raise ValueError("x must have contiguous K")
+        if held:
+            scale = x.scale
+            if xr.dtype != torch.int8 or scale.dtype != torch.float32 or scale.shape != (B, S) or scale.device != dev:
+                raise ValueError("x must be int8 with a fp32 scale for each row, on one device")
+            if (ss % 16 and S != 1) or (sb % 16 and B != 1) or xr.data_ptr() % 16:
+                raise ValueError("x's rows must start on 16-byte boundaries, as quantize_rows() lays them out")
+            one_pitch = sb == S * ss and scale.is_contiguous()
     if bias is not None and (bias.numel() != n or not bias.is_contiguous() or bias.dtype != dtype or bias.device != dev):
         raise ValueError("bias must be N contiguous elements of x's dtype, on its device")
     gated = tail == _C.GEMM_BIAS_GATE_RESIDUAL
@@ -1070,14 +1109,14 @@ def linear_int8(x, weight, bias=None, epilogue="bias", residual=None, gate=None,
             raise ValueError("residual does not match (B, S, N), x's dtype or its device")
         if gate.shape != (B, n) or (gate.stride(1) != 1 and n != 1) or gate.dtype != dtype or gate.device != dev:
             raise ValueError("gate must be (B, N) of x's dtype, on its device")
-    if out is None:
+    own = out is None
+    if own:
         out, so = torch.empty(B, S, n, dtype=dtype, device=dev), n
     else:
         if out.shape != (B, S, n) or out.dtype != dtype or out.device != dev or (out.stride(2) != 1 and n != 1):
             raise ValueError("out does not match (B, S, N), x's dtype or its device")
         so = out.stride(1)
-    if B > 1 and not (_even_rows(out) and (not gated or _even_rows(residual)) and
-                      (not held or (sb == S * ss and scale.is_contiguous()))):
+    if B > 1 and not (one_pitch and _even_rows(out) and (not gated or _even_rows(residual))):
         for b in range(B):  # a slice of the rows of every entry: one launch per entry
             xb = Int8Rows(x.q[b:b + 1], x.scale[b:b + 1], dtype) if held else x[b:b + 1]
             linear_int8(xb, weight, bias, epilogue, residual[b:b + 1] if gated else None, gate[b:b + 1] if gated else None,
@@ -1087,15 +1126,22 @@ def linear_int8(x, weight, bias=None, epilogue="bias", residual=None, gate=None,
         return out
     a = _C.Int8LinearArgs()
     a.dtype, a.epilogue, a.m, a.n, a.k = _DTYPE_CODE[dtype], tail, m, n, k
-    if held:
+    if laid is not None:
+        a.a = a.a_scale = xr.data_ptr()
+        a.a_scale += m * pitch
+        a.lda = pitch
+    elif held:
         if not scale.is_contiguous():
             scale = scale.contiguous()
         a.a, a.a_scale, a.lda = xr.data_ptr(), scale.data_ptr(), ss if S > 1 else pitch
-    else:  # the rows in 8 bits and their scales behind them: scratch of the call
-        scratch = w.new_empty(m * (pitch + 4))
-        a.a = a.a_scale = scratch.data_ptr()
-        a.a_scale += m * pitch
+    else:
         a.x, a.lda, a.x_rows_per_batch, a.x_batch_stride, a.x_row_stride = xr.data_ptr(), pitch, S, sb, ss
+        launches = 1
+        if not (own and m <= 2 and k <= 65536 and tile in (0, 5)):  # the rows in 8 bits, their scales behind them: scratch of the call
+            scratch = torch.empty(m * (pitch + 4), dtype=torch.int8, device=dev)
+            a.a = a.a_scale = scratch.data_ptr()
+            a.a_scale += m * pitch
+            launches = 2
     a.w, a.ldw, a.w_scale = w_ptr, wn if n > 1 else pitch, w_scale.data_ptr()
     if bias is not None:
         a.bias = bias.data_ptr()
@@ -1107,7 +1153,7 @@ def linear_int8(x, weight, bias=None, epilogue="bias", residual=None, gate=None,
     with _on(dev):
         a.stream = _stream_ptr(dev)
         _C.check(_C.lib().hdit_int8_linear(ctypes.byref(a)))
-    _count(1 if held else 2)
+    _count(1 if held else launches)
     return out
 
 
@@ -1210,9 +1256,11 @@ def group_norm_int8(x, groups, weight=None, bias=None, eps=1e-6, act=None):
     """group_norm() with its rows (all channels of a pixel) in 8 bits, see quantize_rows(); nothing is rounded to 16 bits in
     between. Returns Int8Rows (B, pixels, C), what linear_int8() takes."""
     a, B, rows, C = _group_norm_args(x, groups, weight, bias, eps, act)
-    out = _empty_int8_rows(x, (B, rows), C)
+    out, pitch = Int8Rows._empty((B, rows), C, x.dtype, x.device), (C + 15) & ~15
     if B * rows == 0:
         return out
-    a.out, a.out_scale, a.out_row_stride = out.q.data_ptr(), out.scale.data_ptr(), (C + 15) & ~15
+    a.out = a.out_scale = out._buf.data_ptr()
+    a.out_scale += B * rows * pitch
+    a.out_row_stride = pitch
     _group_norm_run(_C.lib().hdit_group_norm_int8, a, x, 1)
     return out

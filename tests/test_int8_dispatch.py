@@ -148,6 +148,10 @@ def test_the_library_refuses_by_itself():
                 dict(gate=0), dict(rows_per_batch=0), dict(out=4097), dict(a_scale=4098), dict(residual=4097)):
         assert linear(**bad) in (_C.HDIT_ERR_BAD_ARG, _C.HDIT_ERR_SHAPE, _C.HDIT_ERR_TOO_LARGE), bad
     assert linear(m=0) == 0
+    few = dict(epilogue=0, m=2, x=1 << 20, x_rows_per_batch=2, x_row_stride=32)  # two rows need no scratch, but where they may be overwritten
+    for bad in (dict(x=4096, a=0), dict(x=4096, a_scale=0), dict(m=3, a=0), dict(tile=1, a=0), dict(x_rows_per_batch=0), dict(x=(1 << 20) + 1),
+                dict(tile=5, m=9), dict(tile=6), dict(tile=5, k=131072, ldw=131072, m=2)):
+        assert linear(**{**few, **bad}) in (_C.HDIT_ERR_BAD_ARG, _C.HDIT_ERR_SHAPE), bad
     assert real.hdit_int8_linear(None) == _C.HDIT_ERR_BAD_ARG
 
 
