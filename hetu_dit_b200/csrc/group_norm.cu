@@ -194,7 +194,7 @@ __device__ __forceinline__ void join_strips(int groups, const Strips& strips, lo
     const bool live = g < groups;
     const float base = live ? in(0, g).x : 0.f;
     float a = 0.f, q = 0.f;
-#pragma unroll 4
+#pragma unroll 10
     for (int k = sub; k < (live ? strips.strips : 0); k += n_sub) {
       const float2 v = in(k, g);
       const float d = v.x - base, n = static_cast<float>(strips.rows_of(k)) * static_cast<float>(per);
@@ -231,9 +231,15 @@ __device__ __forceinline__ void group_norm_factors(const GnParams& p, float4* fa
   const int per = p.channels / p.groups;
   float2* stat = reinterpret_cast<float2*>(factors + p.channels / 2);
   const float2* in = p.partial + static_cast<long long>(blockIdx.y) * p.strips.strips * p.groups;
+  float weight = 1.f, bias = 0.f;  // on their way while the strips are joined
+  if (threadIdx.x < p.channels) {
+    weight = gn_weight<FP16>(p, threadIdx.x);
+    bias = gn_bias<FP16>(p, threadIdx.x);
+  }
   join_strips(p.groups, p.strips, p.rows, per, p.eps, stat, [&](int k, int g) { return in[static_cast<long long>(k) * p.groups + g]; });
   __syncthreads();
-  for (int c = threadIdx.x; c < p.channels; c += kGnThreads)
+  if (threadIdx.x < p.channels) put_factor<FP16>(threadIdx.x, p.channels / 8, stat[threadIdx.x / per], weight, bias, factors);
+  for (int c = threadIdx.x + kGnThreads; c < p.channels; c += kGnThreads)
     put_factor<FP16>(c, p.channels / 8, stat[c / per], gn_weight<FP16>(p, c), gn_bias<FP16>(p, c), factors);
   __syncthreads();
 }
