@@ -109,7 +109,7 @@ def _project_into(buf, row0, x, linear):
     B, S, _ = x.shape
     if kernels.is_plain(linear, Int8Linear):
         kernels.linear_int8(x, linear.rows, linear.bias, out=buf[:, row0:row0 + S])
-    elif B == 1 and not torch.is_grad_enabled():
+    elif B == 1 and not torch.is_grad_enabled() and not isinstance(linear, Int8Linear):
         torch.addmm(linear.bias, x[0], linear.weight.t(), out=buf[0, row0:row0 + S])
     else:
         buf[:, row0:row0 + S] = linear(x)

@@ -185,6 +185,30 @@ def test_an_8_bit_layer_takes_its_tail_where_nothing_waits_for_its_call(monkeypa
         assert seen == ["bias", "gelu kernel"]
 
 
+@pytest.mark.parametrize("batch", [1, 2])
+def test_an_8_bit_projection_writes_its_rows_of_a_shared_buffer(monkeypatch, batch):
+    from hetu_dit_b200.model_executor.layers.attention_processor import _project_into
+    from hetu_dit_b200.model_executor.layers.int8_linear import Int8Linear
+    layer = Int8Linear(rows8(24, 40), torch.zeros(24).bfloat16())
+    outs = []
+
+    def linear_int8(x, weight, bias=None, epilogue="bias", residual=None, gate=None, out=None):
+        outs.append(out)
+        return torch.full((batch, x.shape[1], 24), 3.0, dtype=torch.bfloat16) if out is None else out.fill_(3.0)
+
+    monkeypatch.setattr(kernels, "linear_int8", linear_int8)
+    x, want = torch.zeros(batch, 5, 40).bfloat16(), torch.zeros(batch, 9, 24).bfloat16()
+    want[:, 2:7] = 3.0
+    with torch.no_grad():
+        for hooks in (0, 1):  # what waits for the layer's call gets it
+            buf = torch.zeros(batch, 9, 24).bfloat16()
+            calls = []
+            if hooks:
+                layer.register_forward_hook(lambda m, i, o: calls.append(1))
+            _project_into(buf, 2, x, layer)
+            assert torch.equal(buf, want) and len(calls) == hooks and (outs.pop() is None) == bool(hooks)
+
+
 def test_scales_of_an_8_bit_layer_keep_their_type():
     from hetu_dit_b200.model_executor.layers.int8_linear import Int8Linear
     scale = torch.rand(24)
