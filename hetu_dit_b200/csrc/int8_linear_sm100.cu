@@ -14,6 +14,7 @@
 //                cycles a tile instead of 2.9 k (16384 x 512 -> 1536 19.9 us, now 18.0).
 //
 // All waits are bounded, see gemm_sm100.cu.
+#include <limits.h>
 #include <math.h>
 
 #include "gemm_common.cuh"
@@ -100,6 +101,7 @@ struct alignas(64) Int8Params {
   long long gate_batch_stride;
   int rows_per_batch;
   bool tma_out, tma_residual;  // rows start on 16-byte boundaries
+  int tma_cols;                // results' pieces up to this column leave by TMA
   int32_t* status;
 };
 
@@ -383,7 +385,7 @@ __global__ void __launch_bounds__(Int8Cfg<BN, PAIR, EPI>::kThreads, 1) int8_line
         if constexpr (kGated) {
           if (p.tma_residual) {
             // the next piece's residual, into the buffer that the previous piece's result has left
-            if (!p.tma_out) fence_proxy_async_smem();  // it left by plain loads
+            fence_proxy_async_smem();  // where it left by plain loads
             if (lane == 0) tma_store_wait_read<0>();
             __syncwarp();
             if (c + 1 < C::kTeamPieces) issue_residual(my_row0, col0 + 32, buf ^ 1);
@@ -475,7 +477,7 @@ __global__ void __launch_bounds__(Int8Cfg<BN, PAIR, EPI>::kThreads, 1) int8_line
           *reinterpret_cast<uint4*>(own + ((j ^ swizzle) << 4)) =
               make_uint4(pack2<FP16>(v[0].x, v[0].y), pack2<FP16>(v[1].x, v[1].y), pack2<FP16>(v[2].x, v[2].y), pack2<FP16>(v[3].x, v[3].y));
         }
-        if (p.tma_out) {
+        if (p.tma_out && col0 + 32 <= p.tma_cols) {
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
@@ -638,6 +640,8 @@ extern "C" int hdit_int8_linear(const hdit_int8_linear_args* a) {
   p.rows_per_batch = static_cast<int>(a->rows_per_batch > 0 && a->rows_per_batch < a->m ? a->rows_per_batch : a->m);
   auto whole = [&](const void* ptr, long long ld) { return (reinterpret_cast<uintptr_t>(ptr) & 15) == 0 && ld % 8 == 0; };
   p.tma_out = whole(a->out, a->ldo);
+  // A copy writes whole 16 bytes of a row: where N ends inside of them, the last piece would overwrite what lies behind the row.
+  p.tma_cols = p.N % 8 == 0 ? INT_MAX : p.N;
   p.tma_residual = gated && whole(a->residual, a->ldr);
   p.status = device_status_ptr();
   if (p.status == nullptr) return HDIT_ERR_CUDA;

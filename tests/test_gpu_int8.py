@@ -270,6 +270,25 @@ def test_linear_int8_sums_are_exact_at_the_largest_k():
         _within(kernels.linear_int8(x8, w8), want, tol)
 
 
+@pytest.mark.parametrize("S", [5, 70])
+@pytest.mark.parametrize("epilogue", EPILOGUES)
+@pytest.mark.parametrize("N", [1, 9, 31, 60, 67, 129, 258, 300])
+def test_columns_behind_a_result_of_odd_width_stay(N, epilogue, S):
+    from hetu_dit_b200 import kernels
+    x, w, b, res, gate = _layer(2, S, 96, N, torch.bfloat16, N)
+    pitch = (N + 15) // 8 * 8
+    x8 = kernels.quantize_rows(x)
+    want, tol = _tail64(x8, w, b, epilogue, res, gate, torch.bfloat16)
+    wide_res = torch.zeros(2, S, pitch, dtype=torch.bfloat16, device=DEV)
+    wide_res[..., :N] = res
+    for residual in (res, wide_res[..., :N]):
+        for tile in (0, 1, 2, 3, 4):
+            wide = torch.full((2, S, pitch), 7.0, dtype=torch.bfloat16, device=DEV)
+            kernels.linear_int8(x8, w, b, epilogue, residual=residual, gate=gate, out=wide[..., :N], tile=tile)
+            _within(wide[..., :N], want, tol)
+            assert (wide[..., N:] == 7).all()
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=ids)
 @pytest.mark.parametrize("S", [3, 100])
 def test_linear_int8_layouts(S, dtype):
