@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtas) int8_linear_few_kernel(
       const uint16_t* xr = p.x + m / p.x_rows_per_batch * p.x_batch_stride + m % p.x_rows_per_batch * p.x_row_stride;
       for (int c = threadIdx.x * 8; c < p.pitch; c += kFewThreads * 8) {
         const uint4 raw = c < p.K ? int8_load8(xr, c, p.K, p.vec) : make_uint4(0, 0, 0, 0);
-        int8_put8<FP16>(reinterpret_cast<int8_t*>(rows8) + m * p.pitch, c, s, inv17, raw);
+        int8_put8<FP16, false>(reinterpret_cast<int8_t*>(rows8) + m * p.pitch, c, p.pitch, s, inv17, raw);
       }
       if (threadIdx.x == 0) row_scale[m] = int8_step(s);
     }

@@ -9,6 +9,8 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <type_traits>
+
 #include "host_common.h"
 #include "int8_rows.cuh"
 
@@ -17,6 +19,7 @@ namespace {
 
 struct RowsParams {
   const uint16_t* x;
+  const uint16_t* x_end;  // the end of the last row
   const uint16_t* shift;  // ln_modulate_int8 only
   const uint16_t* scale;
   int8_t* q;
@@ -28,15 +31,16 @@ struct RowsParams {
 };
 
 // CTAs that are to fit an SM beside one another
-constexpr int rows_ctas(int nch, bool ln) { return ln ? (nch <= 2 ? 4 : nch <= 4 ? 3 : 2) : nch <= 4 ? 4 : 2; }
+constexpr int rows_ctas(int nch, bool ln, bool vec) { return ln || !vec ? (nch <= 2 ? 4 : nch <= 4 ? 3 : 2) : nch <= 4 ? 4 : 2; }
 
 // TEAM threads hold a row of at most TEAM * NCH * 8 elements as the 16-bit values that were read, and have the next row on its
 // way while they work on one. What a row costs beside its elements (reductions, divisions, addresses) is paid by every warp of
 // the team, so a thread has up to 32 elements: with eight a thread 8192 x 1536 with the norm took 28 us, with a warp to a row, 128
-// registers and no row ahead 20, in this form 11. Modulation vectors wait in shared memory as fp32 (1 + scale, shift); a CTA stays with
+// registers and no row ahead 20, in this form 11. Rows that start anywhere come as 16-byte blocks whose bits are moved into place (VEC
+// false without LN). Modulation vectors wait in shared memory as fp32 (1 + scale, shift); a CTA stays with
 // one batch entry at a time.
 template <bool FP16, int TEAM, int NCH, bool LN, bool VEC>
-__global__ void __launch_bounds__(kRowThreads, rows_ctas(NCH, LN)) int8_rows_kernel(const __grid_constant__ RowsParams p) {
+__global__ void __launch_bounds__(kRowThreads, rows_ctas(NCH, LN, VEC)) int8_rows_kernel(const __grid_constant__ RowsParams p) {
   grid_dependency_release();
   grid_dependency_wait();
   // 1 + scale, then shift: first the lower four columns of every chunk, then the upper four, so that the lanes' 16 bytes lie
@@ -52,12 +56,16 @@ __global__ void __launch_bounds__(kRowThreads, rows_ctas(NCH, LN)) int8_rows_ker
   for (long long b = blockIdx.y; b < p.batches; b += gridDim.y) {
     const uint16_t* xr = p.x + b * p.x_batch_stride + first * p.x_row_stride;
     const long long row0 = b * p.rows_per_batch;
-    uint4 next[NCH];
+    constexpr bool kBlocks = !LN && !VEC;
+    using Next = std::conditional_t<kBlocks, Int8Blocks, uint4>;
+    Next next[NCH];
     auto fetch = [&] {
 #pragma unroll
       for (int c = 0; c < NCH; ++c) {
-        next[c] = make_uint4(0, 0, 0, 0);
-        if (col0 + c * TEAM * 8 < p.dim) next[c] = int8_load8(xr, col0 + c * TEAM * 8, p.dim, VEC);
+        next[c] = Next{};
+        if (col0 + c * TEAM * 8 >= p.dim) continue;
+        if constexpr (kBlocks) next[c] = int8_load_blocks(xr, col0 + c * TEAM * 8, p.dim, p.x, p.x_end);
+        else next[c] = int8_load8(xr, col0 + c * TEAM * 8, p.dim, VEC);
       }
     };
     if (first < p.rows_per_batch) fetch();
@@ -81,7 +89,10 @@ __global__ void __launch_bounds__(kRowThreads, rows_ctas(NCH, LN)) int8_rows_ker
     for (long long r = first; r < p.rows_per_batch; r += step, turn ^= 1) {
       uint4 raw[NCH];
 #pragma unroll
-      for (int c = 0; c < NCH; ++c) raw[c] = next[c];
+      for (int c = 0; c < NCH; ++c) {
+        if constexpr (kBlocks) raw[c] = int8_from_blocks(next[c], xr, col0 + c * TEAM * 8, p.dim);
+        else raw[c] = next[c];
+      }
       xr += step * p.x_row_stride;
       if (r + step < p.rows_per_batch) fetch();
       int8_t* const qr = p.q + (row0 + r) * p.q_row_stride;
@@ -101,7 +112,7 @@ __global__ void __launch_bounds__(kRowThreads, rows_ctas(NCH, LN)) int8_rows_ker
 #pragma unroll
         for (int c = 0; c < NCH; ++c) {
           if (col0 + c * TEAM * 8 >= p.dim) continue;
-          int8_put8<FP16>(qr, col0 + c * TEAM * 8, s, inv17, raw[c]);
+          int8_put8<FP16, !VEC>(qr, col0 + c * TEAM * 8, p.dim, s, inv17, raw[c]);
         }
       } else {
         float2 y[NCH][4];  // x, its distance from the mean, the result
@@ -152,7 +163,7 @@ __global__ void __launch_bounds__(kRowThreads, rows_ctas(NCH, LN)) int8_rows_ker
   }
 }
 
-// Rows of any length and alignment: read twice, the second time from the caches.
+// Rows of any length: read twice, the second time from the caches.
 template <bool FP16>
 __global__ void __launch_bounds__(kRowThreads) int8_any_rows_kernel(const __grid_constant__ RowsParams p) {
   grid_dependency_release();
@@ -204,24 +215,24 @@ cudaError_t launch_rows(const RowsParams& p, cudaStream_t st) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) return e;
   }
-  return launch_overlapped(kernel, rows_grid(p, kRowThreads / TEAM, rows_ctas(NCH, LN)), dim3(kRowThreads), smem, st, 1, p);
+  return launch_overlapped(kernel, rows_grid(p, kRowThreads / TEAM, rows_ctas(NCH, LN, VEC)), dim3(kRowThreads), smem, st, 1, p);
 }
 
-template <bool FP16>
-cudaError_t launch_plain(const RowsParams& p, bool vec, cudaStream_t st) {
+template <bool FP16, bool VEC>
+cudaError_t launch_plain(const RowsParams& p, cudaStream_t st) {
   const int chunks = (p.dim + 7) / 8;
-  if (!vec || chunks > 2048) return launch_overlapped(int8_any_rows_kernel<FP16>, rows_grid(p, 1, 8), dim3(kRowThreads), 0, st, 1, p);
-  if (chunks <= 32) return launch_rows<FP16, 32, 1, false, true>(p, st);
-  if (chunks <= 64) return launch_rows<FP16, 32, 2, false, true>(p, st);
-  if (chunks <= 96) return launch_rows<FP16, 32, 3, false, true>(p, st);
-  if (chunks <= 128) return launch_rows<FP16, 32, 4, false, true>(p, st);
-  if (chunks <= 192) return launch_rows<FP16, 64, 3, false, true>(p, st);
-  if (chunks <= 256) return launch_rows<FP16, 64, 4, false, true>(p, st);
-  if (chunks <= 384) return launch_rows<FP16, 128, 3, false, true>(p, st);
-  if (chunks <= 512) return launch_rows<FP16, 128, 4, false, true>(p, st);
-  if (chunks <= 768) return launch_rows<FP16, 256, 3, false, true>(p, st);
-  if (chunks <= 1024) return launch_rows<FP16, 256, 4, false, true>(p, st);
-  return launch_rows<FP16, 256, 8, false, true>(p, st);
+  if (chunks <= 32) return launch_rows<FP16, 32, 1, false, VEC>(p, st);
+  if (chunks <= 64) return launch_rows<FP16, 32, 2, false, VEC>(p, st);
+  if (chunks <= 96) return launch_rows<FP16, 32, 3, false, VEC>(p, st);
+  if (chunks <= 128) return launch_rows<FP16, 32, 4, false, VEC>(p, st);
+  if (chunks <= 192) return launch_rows<FP16, 64, 3, false, VEC>(p, st);
+  if (chunks <= 256) return launch_rows<FP16, 64, 4, false, VEC>(p, st);
+  if (chunks <= 384) return launch_rows<FP16, 128, 3, false, VEC>(p, st);
+  if (chunks <= 512) return launch_rows<FP16, 128, 4, false, VEC>(p, st);
+  if (chunks <= 768) return launch_rows<FP16, 256, 3, false, VEC>(p, st);
+  if (chunks <= 1024) return launch_rows<FP16, 256, 4, false, VEC>(p, st);
+  if (chunks <= 2048) return launch_rows<FP16, 256, 8, false, VEC>(p, st);
+  return launch_overlapped(int8_any_rows_kernel<FP16>, rows_grid(p, 1, 8), dim3(kRowThreads), 0, st, 1, p);
 }
 
 // Unaligned rows: the teams, and so the sums, of aligned ones.
@@ -265,11 +276,14 @@ extern "C" int hdit_quantize_rows(int32_t dtype, const void* x, void* q, float* 
   if (rc != HDIT_OK || rows == 0) return rc;
   const bool flat = rows <= rows_per_batch || x_batch_stride == rows_per_batch * x_row_stride;  // one stride for all rows
   if (!flat && rows % rows_per_batch != 0) return set_error(HDIT_ERR_SHAPE, "rows must be a multiple of rows_per_batch");
-  RowsParams p{static_cast<const uint16_t*>(x), nullptr, nullptr, static_cast<int8_t*>(q), scale, flat ? 1 : rows / rows_per_batch,
-               flat ? rows : rows_per_batch, x_batch_stride, x_row_stride, q_row_stride, 0, static_cast<int>(dim), 0.f, false};
+  const long long batches = flat ? 1 : rows / rows_per_batch, per = flat ? rows : rows_per_batch;
+  const uint16_t* const x_end = static_cast<const uint16_t*>(x) + (batches - 1) * x_batch_stride + (per - 1) * x_row_stride + dim;
+  RowsParams p{static_cast<const uint16_t*>(x), x_end, nullptr, nullptr, static_cast<int8_t*>(q), scale, batches, per,
+               x_batch_stride, x_row_stride, q_row_stride, 0, static_cast<int>(dim), 0.f, false};
   const bool vec = dim % 8 == 0 && !misaligned(x, x_row_stride) && (flat || x_batch_stride % 8 == 0);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  HDIT_CUDA_OK(dtype == HDIT_FP16 ? launch_plain<true>(p, vec, st) : launch_plain<false>(p, vec, st));
+  HDIT_CUDA_OK((dtype == HDIT_FP16 ? (vec ? launch_plain<true, true>(p, st) : launch_plain<true, false>(p, st))
+                                   : (vec ? launch_plain<false, true>(p, st) : launch_plain<false, false>(p, st))));
   return HDIT_OK;
 }
 
@@ -286,7 +300,7 @@ extern "C" int hdit_ln_modulate_int8(int32_t dtype, const void* x, const void* s
     return set_error(HDIT_ERR_SHAPE, "shift / scale not aligned to their elements");
   if (rows > rows_per_batch && rows % rows_per_batch != 0) return set_error(HDIT_ERR_SHAPE, "rows must be a multiple of rows_per_batch");
   const bool one = rows <= rows_per_batch;
-  RowsParams p{static_cast<const uint16_t*>(x), static_cast<const uint16_t*>(shift), static_cast<const uint16_t*>(scale),
+  RowsParams p{static_cast<const uint16_t*>(x), nullptr, static_cast<const uint16_t*>(shift), static_cast<const uint16_t*>(scale),
                static_cast<int8_t*>(q), q_scale, one ? 1 : rows / rows_per_batch, one ? rows : rows_per_batch, x_batch_stride, x_row_stride,
                q_row_stride, mod_batch_stride, static_cast<int>(dim), eps, !misaligned(shift, mod_batch_stride) && !misaligned(scale, mod_batch_stride)};
   const bool vec = !misaligned(x, x_row_stride) && (one || x_batch_stride % 8 == 0);

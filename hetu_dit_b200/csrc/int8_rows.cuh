@@ -67,6 +67,46 @@ __device__ __forceinline__ uint4 int8_load8(const uint16_t* row, int c, int dim,
   return make_uint4(e[0] | (e[1] << 16), e[2] | (e[3] << 16), e[4] | (e[5] << 16), e[6] | (e[7] << 16));
 }
 
+// The same eight elements of a row that starts anywhere, in two steps: the two 16-byte blocks that hold them, then their bits moved
+// into place, so that nothing waits for the loads in between. lo, hi: the first element of all rows and the end of the last one. A
+// block that reaches outside (the first one of the first row, the last ones of the last row) is put together from the elements; what
+// lies between rows may be read, and goes no further.
+struct Int8Blocks {
+  uint4 a, b;
+};
+__device__ __forceinline__ Int8Blocks int8_load_blocks(const uint16_t* row, int c, int dim, const uint16_t* lo, const uint16_t* hi) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(row + c);
+  const uint16_t* const base = reinterpret_cast<const uint16_t*>(at & ~static_cast<uintptr_t>(15));
+  const int skip = static_cast<int>(at & 15) >> 1, live = min(8, dim - c);
+  const bool second = skip + live > 8;
+  Int8Blocks r{make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+  if (base >= lo && base + (second ? 16 : 8) <= hi) {
+    r.a = *reinterpret_cast<const uint4*>(base);
+    if (second) r.b = *reinterpret_cast<const uint4*>(base + 8);
+  } else {
+    uint32_t* u = reinterpret_cast<uint32_t*>(&r);
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      if (e >= skip && e < skip + live) u[e >> 1] |= static_cast<uint32_t>(base[e]) << (16 * (e & 1));
+  }
+  return r;
+}
+__device__ __forceinline__ uint4 int8_from_blocks(const Int8Blocks& r, const uint16_t* row, int c, int dim) {
+  const int skip = static_cast<int>(reinterpret_cast<uintptr_t>(row) & 15) >> 1;  // of the row: c is a multiple of 8
+  uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+#pragma unroll
+  for (int i = 0; i < 6; ++i) w[i] = skip & 4 ? w[i + 2] : w[i];
+#pragma unroll
+  for (int i = 0; i < 5; ++i) w[i] = skip & 2 ? w[i + 1] : w[i];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], (skip & 1) * 16);
+  if (c + 8 > dim) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = c + 2 * i + 1 < dim ? w[i] : c + 2 * i < dim ? w[i] & 0xFFFFu : 0u;
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 constexpr int kRowThreads = 256;  // of a CTA that works on rows
 
 // TEAM threads of a CTA that share a row. A reduction over several warps has one barrier, of the team: each has places of its
@@ -111,16 +151,20 @@ struct Team {
 };
 
 // Eight 16-bit values to column c of the row, which is on an 8-byte boundary; zeros where the row has no step (an infinity
-// times 0 is none).
-template <bool FP16>
-__device__ __forceinline__ void int8_put8(int8_t* row, int c, const Int8Scale& s, float inv17, const uint4& raw) {
+// times 0 is none). TAIL: the row may end before, and what lies behind it stays as it was.
+template <bool FP16, bool TAIL>
+__device__ __forceinline__ void int8_put8(int8_t* row, int c, int dim, const Int8Scale& s, float inv17, const uint4& raw) {
   const uint32_t* u = reinterpret_cast<const uint32_t*>(&raw);
   float2 t[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) t[i] = add2(int8_steps_of_16bit(int8_unpack2<FP16>(u[i]), s.inv, inv17), both(kInt8Round));
   uint2 v = make_uint2(int8_bytes(t[0], t[1]), int8_bytes(t[2], t[3]));
   if (s.inv == 0.f) v = make_uint2(0, 0);
-  *reinterpret_cast<uint2*>(row + c) = v;
+  if (!TAIL || c + 8 <= dim) {
+    *reinterpret_cast<uint2*>(row + c) = v;
+  } else {
+    for (int i = 0; c + i < dim; ++i) row[c + i] = static_cast<int8_t>((i < 4 ? v.x >> (8 * i) : v.y >> (8 * (i - 4))) & 0xFFu);
+  }
 }
 
 // The same for fp32 values: product with inv and rounding to an integer in one operation.

@@ -90,6 +90,25 @@ def test_quantize_rows_strides_batches_and_what_lies_behind(dtype):
     assert torch.equal(kernels.quantize_rows(same).q, _rows64(same)[0])
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("k", [1, 2, 5, 7, 8, 9, 13, 16, 31, 250, 1001, 2050, 5003, 9001])
+def test_rows_that_start_anywhere(k, dtype):
+    """What stands before, between and behind the rows is larger than they are and must not be seen."""
+    from hetu_dit_b200 import kernels
+    rows = 5
+    want = _randn(_gen(k), rows, k, dtype=dtype)
+    q, s = _rows64(want)
+    for off in range(9):
+        for pitch in (k, k + 1, k + 6):
+            flat = torch.full((off + rows * pitch + 3,), float("inf"), dtype=dtype, device=DEV)
+            x = flat[off:off + rows * pitch].view(rows, pitch)[:, :k]
+            x.copy_(want)
+            got = kernels.quantize_rows(x)
+            assert torch.equal(got.q, q) and torch.equal(got.scale, s)
+    exact = torch.empty(rows * k, dtype=dtype, device=DEV).view(rows, k).copy_(want)  # nothing before or behind it
+    assert torch.equal(kernels.quantize_rows(exact).q, q)
+
+
 def test_bytes_behind_a_row_stay():
     from hetu_dit_b200 import _C
     x = _randn(_gen(5), 9, 77, dtype=torch.bfloat16)
