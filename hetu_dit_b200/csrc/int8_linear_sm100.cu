@@ -83,6 +83,70 @@ __device__ __forceinline__ uint16_t* staged(uint8_t* stage, int i, int k) {
   return reinterpret_cast<uint16_t*>(stage + i * 64 + (((k >> 3) ^ ((i >> 1) & 3)) << 4) + (k & 7) * 2);
 }
 
+// Pieces of matrices whose rows start on no 16-byte boundary, which TMA cannot move: 32-bit words where they lie on one, half a
+// warp to a row, and what a row has before its first and behind its last whole word by a lane to a row. A row that starts inside
+// of a word is staged one element to the left in between, so that words go from and to shared memory as they are. g: the piece's
+// first element, `rows` x `cols` of it exist. All of a warp's loads are on their way before the first is needed: one row after the
+// other, 1813 x 3122 -> 6387 with a gated residual took 100 us.
+struct RaggedPiece {
+  uint32_t word[16];
+  uint16_t first, last;
+};
+__device__ __forceinline__ int starts_inside(const uint16_t* row) { return static_cast<int>(reinterpret_cast<uintptr_t>(row) >> 1) & 1; }
+// Word `lane & 15` of row `lane >> 4` + 2 i; (row >> 1) & 3 is i & 3.
+__device__ __forceinline__ uint32_t* staged_word(uint8_t* stage, int i, int lane) {
+  return reinterpret_cast<uint32_t*>(stage + ((lane >> 4) + 2 * i) * 64 + ((((lane >> 2) & 3) ^ (i & 3)) << 4) + (lane & 3) * 4);
+}
+__device__ __forceinline__ void ragged_load(RaggedPiece& v, const uint16_t* g, long long ld, int rows, int cols, int lane) {
+  const uint16_t* at = g + (lane >> 4) * ld;
+  const int col = 2 * (lane & 15) + starts_inside(at), live = col + 1 < cols ? rows - (lane >> 4) : 0;
+  at += col;
+#pragma unroll
+  for (int i = 0; i < 16; ++i, at += 2 * ld) v.word[i] = 2 * i < live ? *reinterpret_cast<const uint32_t*>(at) : 0u;
+  const uint16_t* own = g + lane * ld;
+  v.first = lane < rows && starts_inside(own) ? own[0] : uint16_t(0);
+  v.last = lane < rows && ((cols - starts_inside(own)) & 1) ? own[cols - 1] : uint16_t(0);
+}
+__device__ __forceinline__ void ragged_stage(const RaggedPiece& v, uint8_t* stage, const uint16_t* g, long long ld, int rows, int cols, int lane) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) *staged_word(stage, i, lane) = v.word[i];
+  __syncwarp();
+  const int inside = starts_inside(g + lane * ld);
+  uint32_t before = static_cast<uint32_t>(v.first) << 16;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    uint4* const chunk = reinterpret_cast<uint4*>(staged(stage, lane, j * 8));
+    const uint4 w = *chunk;
+    *chunk = make_uint4(__funnelshift_l(before, w.x, inside * 16), __funnelshift_l(w.x, w.y, inside * 16), __funnelshift_l(w.y, w.z, inside * 16),
+                        __funnelshift_l(w.z, w.w, inside * 16));
+    before = w.w;
+  }
+  if ((cols - inside) & 1) *staged(stage, lane, cols - 1) = v.last;
+}
+__device__ __forceinline__ void ragged_store(uint16_t* g, long long ld, int rows, int cols, uint8_t* stage, int lane) {
+  uint16_t* const own = g + lane * ld;
+  const int inside = starts_inside(own);
+  if (lane < rows) {
+    if (inside) own[0] = *staged(stage, lane, 0);
+    if ((cols - inside) & 1) own[cols - 1] = *staged(stage, lane, cols - 1);
+  }
+  uint4 w[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) w[j] = *reinterpret_cast<const uint4*>(staged(stage, lane, j * 8));
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    *reinterpret_cast<uint4*>(staged(stage, lane, j * 8)) =
+        make_uint4(__funnelshift_r(w[j].x, w[j].y, inside * 16), __funnelshift_r(w[j].y, w[j].z, inside * 16), __funnelshift_r(w[j].z, w[j].w, inside * 16),
+                   __funnelshift_r(w[j].w, j < 3 ? w[j + 1 < 4 ? j + 1 : 3].x : 0u, inside * 16));
+  __syncwarp();
+  uint16_t* at = g + (lane >> 4) * ld;
+  const int col = 2 * (lane & 15) + starts_inside(at), live = col + 1 < cols ? rows - (lane >> 4) : 0;
+  at += col;
+#pragma unroll
+  for (int i = 0; i < 16; ++i, at += 2 * ld)
+    if (2 * i < live) *reinterpret_cast<uint32_t*>(at) = *staged_word(stage, i, lane);
+}
+
 struct alignas(64) Int8Params {
   CUtensorMap a_map;
   CUtensorMap w_map;
@@ -367,6 +431,25 @@ __global__ void __launch_bounds__(Int8Cfg<BN, PAIR, EPI>::kThreads, 1) int8_line
       team_sync();
       if (!ok) continue;  // after a failure: the team's other warps still meet the barriers
       if (tile + n_units < total_tiles) fetch(tile + n_units);
+      if constexpr (kGated) {
+        if (!p.tma_residual) {
+          // both pieces, into buffers that the tile before has left, while its sums are on their way
+          static_assert(C::kTeamPieces == 2 && C::kBufs == 2, "a buffer for each piece of a tile");
+          RaggedPiece v[2];
+          auto piece_at = [&](int c, auto f) {
+            if (my_row0 < p.M && my_col + c * 32 < p.N)
+              f(p.residual + my_row0 * p.ldr + my_col + c * 32, min(32, p.M - my_row0), min(32, p.N - my_col - c * 32));
+          };
+#pragma unroll
+          for (int c = 0; c < 2; ++c) piece_at(c, [&](const uint16_t* g, int rows, int cols) { ragged_load(v[c], g, p.ldr, rows, cols, lane); });
+          if (lane == 0) tma_store_wait_read<0>();
+          __syncwarp();
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+            piece_at(c, [&](const uint16_t* g, int rows, int cols) { ragged_stage(v[c], staging + c * kPieceBytes, g, p.ldr, rows, cols, lane); });
+          __syncwarp();
+        }
+      }
       if (!__all_sync(0xffffffffu, mbar_wait_bounded(&acc_full[acc], use & 1, abort_flag, kSpinLimit))) {
         if (lane == 0) report_failure(p.status, abort_flag, HDIT_ERR_PEER_TIMEOUT, Q_EPI_ACC_FULL, static_cast<int>(local));
         ok = false;
@@ -399,15 +482,6 @@ __global__ void __launch_bounds__(Int8Cfg<BN, PAIR, EPI>::kThreads, 1) int8_line
               res_phase ^= 1u << buf;
               res_pending &= ~(1u << buf);
             }
-          } else {
-            if (lane == 0) tma_store_wait_read<1>();
-            __syncwarp();
-            for (int i = 0; i < 32 && in; ++i) {
-              const long long row = my_row0 + i;
-              if (row >= p.M) break;
-              if (col0 + lane < p.N) *staged(stage, i, lane) = p.residual[row * p.ldr + col0 + lane];
-            }
-            __syncwarp();
           }
         } else {
           if (lane == 0) tma_store_wait_read<C::kBufs - 1>();  // the buffer's last result has left
@@ -486,11 +560,7 @@ __global__ void __launch_bounds__(Int8Cfg<BN, PAIR, EPI>::kThreads, 1) int8_line
           }
         } else {
           __syncwarp();
-          for (int i = 0; i < 32 && in; ++i) {
-            const long long row = my_row0 + i;
-            if (row >= p.M) break;
-            if (col0 + lane < p.N) p.out[row * p.ldo + col0 + lane] = *staged(stage, i, lane);
-          }
+          if (in) ragged_store(p.out + my_row0 * p.ldo + col0, p.ldo, min(32, p.M - my_row0), min(32, p.N - col0), stage, lane);
           __syncwarp();
         }
       }

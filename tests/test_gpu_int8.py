@@ -289,6 +289,31 @@ def test_linear_int8_sums_are_exact_at_the_largest_k():
         _within(kernels.linear_int8(x8, w8), want, tol)
 
 
+@pytest.mark.parametrize("tile", [1, 4])
+@pytest.mark.parametrize("epilogue", ["bias", "gate_residual"])
+@pytest.mark.parametrize("N", [1, 2, 3, 30, 31, 32, 33, 34, 63, 65, 97, 130, 259])
+def test_results_and_residuals_that_start_anywhere(N, epilogue, tile):
+    """Columns at any offset of rows of any pitch: the bits of the aligned form, and everything around stays."""
+    from hetu_dit_b200 import kernels
+    B, S, K = 2, 70, 96
+    x, w, b, res, gate = _layer(B, S, K, N, torch.bfloat16, N)
+    x8 = kernels.quantize_rows(x)
+    want, tol = _tail64(x8, w, b, epilogue, res, gate, torch.bfloat16)
+    pad = torch.zeros(B, S, (N + 7) // 8 * 8, dtype=torch.bfloat16, device=DEV)
+    pad[..., :N] = res
+    first = torch.empty_like(pad)
+    kernels.linear_int8(x8, w, b, epilogue, residual=pad[..., :N], gate=gate, out=first[..., :N], tile=tile)
+    _within(first[..., :N], want, tol)
+    for pitch in (N + 7, N + 8, N + 10):
+        for off, res_off in ((0, 1), (1, 0), (3, 3), (4, 6), (6, 7)):
+            wide = torch.full((B, S, pitch), 7.0, dtype=torch.bfloat16, device=DEV)
+            wide_res = torch.full((B, S, pitch), float("nan"), dtype=torch.bfloat16, device=DEV)
+            wide_res[..., res_off:res_off + N] = res
+            kernels.linear_int8(x8, w, b, epilogue, residual=wide_res[..., res_off:res_off + N], gate=gate, out=wide[..., off:off + N], tile=tile)
+            assert torch.equal(wide[..., off:off + N], first[..., :N])
+            assert (wide[..., :off] == 7).all() and (wide[..., off + N:] == 7).all()
+
+
 @pytest.mark.parametrize("S", [5, 70])
 @pytest.mark.parametrize("epilogue", EPILOGUES)
 @pytest.mark.parametrize("N", [1, 9, 31, 60, 67, 129, 258, 300])
