@@ -98,13 +98,16 @@ __device__ __forceinline__ void walk_rows(const uint16_t* x, int c, int channels
     if (at + k < count) use(next[k], at + k);
 }
 
+// Floats from one lane's sums to the next one's: lanes that are summed side by side are in banks of their own (two launches over 64 x 16 8.0 -> 6.5 us; the cluster over 4096 x 512 8.8 -> 7.9)
+__host__ __device__ constexpr int stats_pitch(int channels) { return channels + 4; }
+
 // Statistics of strip k of an image of `rows` rows of `channels` channels at `x`. A thread passes its eight channels of every lanes-th
-// row to keep(raw, index). smem: [lanes][channels] sums, then the same of squares. put(group, {mean, sum of squared distances from it}).
+// row to keep(raw, index). smem: [lanes][stats_pitch(channels)] sums, then the same of squares. put(group, {mean, sum of squared distances from it}).
 template <int THREADS, bool FP16, bool VEC, typename K, typename P>
 __device__ __forceinline__ void strip_stats(const uint16_t* x, long long row_stride, const Strips& strips, int strip, int channels, int per, float* smem, K keep,
                                             P put) {
   const int chunks = channels / 8;
-  const int lanes = strips.lanes;  // rows at a time
+  const int lanes = strips.lanes, pitch = stats_pitch(channels);  // rows at a time
   const int lane = threadIdx.x / chunks, c = (threadIdx.x - lane * chunks) * 8;
   const uint16_t* xs = x + static_cast<long long>(strip) * lanes * row_stride;  // the strip's first row
   if (lane < lanes) {
@@ -130,10 +133,10 @@ __device__ __forceinline__ void strip_stats(const uint16_t* x, long long row_str
         ss[2 * i + 1] = fmaf(d1, d1, ss[2 * i + 1]);
       }
     });
-    float4* to = reinterpret_cast<float4*>(smem + lane * channels + c);
+    float4* to = reinterpret_cast<float4*>(smem + lane * pitch + c);
     to[0] = make_float4(s[0], s[1], s[2], s[3]);
     to[1] = make_float4(s[4], s[5], s[6], s[7]);
-    to = reinterpret_cast<float4*>(smem + (lanes + lane) * channels + c);
+    to = reinterpret_cast<float4*>(smem + (lanes + lane) * pitch + c);
     to[0] = make_float4(ss[0], ss[1], ss[2], ss[3]);
     to[1] = make_float4(ss[4], ss[5], ss[6], ss[7]);
   }
@@ -148,15 +151,15 @@ __device__ __forceinline__ void strip_stats(const uint16_t* x, long long row_str
     float a = 0.f, q = 0.f;
     if (ch < channels)
       for (int l = part; l < lanes; l += parts) {
-        a += smem[l * channels + ch];
-        q += smem[(lanes + l) * channels + ch];
+        a += smem[l * pitch + ch];
+        q += smem[(lanes + l) * pitch + ch];
       }
     a = sub_sum(a, parts);
     q = sub_sum(q, parts);
     if (ch < channels && part == 0) {  // no other thread reads this channel's first lane
       const float m2 = q - a * a * inv_rows;
       smem[ch] = int8_unpack2<FP16>(xs[ch]).x + a * inv_rows;
-      smem[lanes * channels + ch] = m2 > 0.f ? m2 : m2 - m2;  // keeps NaN
+      smem[lanes * pitch + ch] = m2 > 0.f ? m2 : m2 - m2;  // keeps NaN
     }
   }
   __syncthreads();
@@ -168,7 +171,7 @@ __device__ __forceinline__ void strip_stats(const uint16_t* x, long long row_str
     mean = sub_sum(mean, n_sub) * inv_per;
     for (int k = sub; live && k < per; k += n_sub) {
       const float d = smem[g * per + k] - mean;
-      m2 += smem[lanes * channels + g * per + k] + n * d * d;
+      m2 += smem[lanes * pitch + g * per + k] + n * d * d;
     }
     m2 = sub_sum(m2, n_sub);
     if (live && sub == 0) put(g, make_float2(mean, m2));
@@ -396,7 +399,7 @@ __global__ void __launch_bounds__(cluster_threads(INT8), INT8 ? 1 : 2) group_nor
   const int rank = static_cast<int>(blockIdx.x);
   uint4* held = reinterpret_cast<uint4*>(smem4);  // [tiles * lanes][chunks]
   float4* factors = smem4 + p.strips.tiles_of(0) * lanes * chunks;
-  float2* strip = reinterpret_cast<float2*>(factors + lanes * p.slab / 2);
+  float2* strip = reinterpret_cast<float2*>(factors + lanes * stats_pitch(p.slab) / 2);
   float2* stat = strip + groups;
   float weight = 1.f, bias = 0.f;  // on their way while the statistics are made
   if (threadIdx.x < p.slab) {
@@ -467,16 +470,17 @@ bool cluster_of(long long batch, long long rows, int channels, int groups, bool 
   const int per = channels / groups;
   int unit = per;  // whole groups and whole chunks
   while (unit % 8 != 0) unit += per;
-  if ((int8 && channels > 1024) || batch > 33 || rows > 33LL * 8 * 100 * 1024 / 2 / (batch * channels)) return false;
+  if ((int8 && (channels > 1024 || rows > 384)) || batch > 33 || rows > 33LL * 8 * 100 * 1024 / 2 / (batch * channels)) return false;
   for (int slab = int8 ? channels : unit; slab <= channels && slab / 8 <= cluster_threads(int8); slab += unit) {
     if (channels % slab != 0 || (slab < 32 && slab < channels)) continue;  // 64 bytes of a row at least
     const long long clusters = batch * (channels / slab), lanes = cluster_threads(int8) / (slab / 8);
     const long long tiles = ((rows + lanes - 1) / lanes + kClusterCtas - 1) / kClusterCtas;
     if (rows <= lanes * (kClusterCtas - 1)) continue;  // each CTA has rows
-    const long long held = tiles * lanes * slab * 2, smem = held + lanes * slab * 8 + slab / per * 16;
+    const long long held = tiles * lanes * slab * 2, smem = held + lanes * stats_pitch(slab) * 8 + slab / per * 16;
     // So many clusters of this size are on the GPU at a time; a second wave costs more than a second launch. 8-bit rows need all
     // channels of a pixel in one CTA, which leaves few CTAs: with 82 KB each, two images of 32 x 32 x 640 took 15 us, in two
-    // launches 9.9.
+    // launches 9.9; and a warp has a row, so many rows take long however short they are: 384 x 256 7.3 us against 7.6 in two
+    // launches, 512 x 256 7.9 against 7.5, 6560 x 16 41 against 10.
     if (clusters <= (smem <= 100 * 1024 && !int8 ? 33 : 15) && smem <= 200 * 1024 && (!int8 || held <= 32 * 1024)) {
       *to = {slab, static_cast<size_t>(smem)};
       return true;
@@ -534,7 +538,7 @@ size_t factor_bytes(const GnParams& p) { return static_cast<size_t>(p.channels) 
 
 template <bool FP16, bool VEC>
 cudaError_t launch_stats(const GnParams& p, long long batch, cudaStream_t st) {
-  const size_t smem = static_cast<size_t>(kGnThreads / (p.channels / 8)) * p.channels * 2 * sizeof(float);
+  const size_t smem = static_cast<size_t>(kGnThreads / (p.channels / 8)) * stats_pitch(p.channels) * 2 * sizeof(float);
   return launch_strips(group_norm_stats_kernel<FP16, VEC>, p, batch, smem, st);
 }
 
