@@ -24,6 +24,7 @@ __device__ __forceinline__ float2 int8_gelu2(float2 x) {
 // int8_linear_few.cu
 constexpr int kInt8FewRows = 8;
 bool int8_linear_few_takes(const hdit_int8_linear_args* a);
+bool int8_linear_few_pays(const hdit_int8_linear_args* a);       // against tiles
 bool int8_linear_few_quantizes(const hdit_int8_linear_args* a);  // brings 16-bit rows into 8 bits by itself
 int int8_linear_few(const hdit_int8_linear_args* a);             // checked arguments
 

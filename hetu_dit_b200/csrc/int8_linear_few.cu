@@ -9,9 +9,10 @@
 //   matter as long as both operands agree, so the rows of x lie in shared memory as they are.
 //
 // us, this kernel | 128 x 128 tiles, 8-bit rows: 9216 x 1536, 1 row 4.4 | 7.8, 8 rows 6.2 | 7.6, 16 rows 9.1 | 7.6 (as two column
-// tiles); 18432 x 3072, 1 row 12.4 | 16.2, 8 rows 16.1 | 16.0: taken for up to eight rows. One or two 16-bit rows are brought into 8
-// bits by every CTA for itself, which saves a launch: 1 row 4.6, 2 rows 6.5 and 3 us less on the host; with 4 rows it took 9.0, with
-// quantize_rows before it 7.2.
+// tiles); 18432 x 3072, 1 row 12.4 | 16.2, 8 rows 16.1 | 16.0: taken for up to eight rows. 16-bit rows are brought into 8 bits by every
+// CTA for itself where there are one or two, or at most 8192 elements: a launch less, 3 us on the host. us on the device, so |
+// after quantize_rows: 9216 x 1536, 2 rows 5.9 | 6.2, 4 rows 7.5 | 6.9, 8 rows 9.3 | 8.0; 2048 x 2048, 4 rows 5.5 | 6.3, 8 rows
+// 7.4 | 7.0; 500 x 200, 8 rows 3.2 | 4.2; 1536 x 6144, 2 rows 7.6 | 8.0, 6 rows 16.6 | 11.2.
 #include "gemm_common.cuh"
 #include "host_common.h"
 #include "int8_linear.h"
@@ -22,7 +23,6 @@ namespace {
 
 constexpr int kFewThreads = 256;
 constexpr int kFewWarps = kFewThreads / 32;
-constexpr int kOwnRows = 2;  // 16-bit rows that a CTA brings into 8 bits by itself
 constexpr int kChunksAhead = 4;
 constexpr int kFewCtas = 4;  // to an SM
 
@@ -59,7 +59,7 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtas) int8_linear_few_kernel(
   extern __shared__ __align__(16) uint8_t rows8[];  // M rows of x, `pitch` bytes apart, zeros behind K
   __shared__ int sums[kFewWarps][16][kInt8FewRows + 1];
   __shared__ float row_scale[kInt8FewRows];
-  __shared__ uint32_t tops[kOwnRows][kFewWarps];
+  __shared__ uint32_t tops[kFewWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   const int n_chunks = (p.K + 63) / 64, groups = (p.N + 15) / 16;
@@ -87,29 +87,33 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtas) int8_linear_few_kernel(
   fetch(warp);
 
   if (p.x != nullptr) {
-    for (int m = 0; m < p.M; ++m) {
-      const uint16_t* xr = p.x + m / p.x_rows_per_batch * p.x_batch_stride + m % p.x_rows_per_batch * p.x_row_stride;
+    // all rows at a time, a power of two of the warps to each
+    const int per = kFewWarps >> (p.M > 4 ? 3 : p.M > 2 ? 2 : p.M - 1), m = warp / per;
+    const int c0 = (static_cast<int>(threadIdx.x) - m * per * 32) * 8, step = per * 256;
+    const uint16_t* xr = p.x;
+    if (m < p.M) {
+      xr += m / p.x_rows_per_batch * p.x_batch_stride + m % p.x_rows_per_batch * p.x_row_stride;
       uint32_t top2 = 0;
-      for (int c = threadIdx.x * 8; c < p.K; c += kFewThreads * 8) {
+#pragma unroll 4
+      for (int c = c0; c < p.K; c += step) {
         const uint4 raw = int8_load8(xr, c, p.K, p.vec);
         top2 = __vmaxu2(__vmaxu2(top2, __vmaxu2(raw.x & 0x7FFF7FFFu, raw.y & 0x7FFF7FFFu)), __vmaxu2(raw.z & 0x7FFF7FFFu, raw.w & 0x7FFF7FFFu));
       }
       const uint32_t v = __reduce_max_sync(0xffffffffu, (top2 & 0xFFFFu) > (top2 >> 16) ? top2 & 0xFFFFu : top2 >> 16);
-      if (lane == 0) tops[m][warp] = v;
+      if (lane == 0) tops[warp] = v;
     }
     __syncthreads();
-    for (int m = 0; m < p.M; ++m) {
+    if (m < p.M) {
       uint32_t top = 0;
-#pragma unroll
-      for (int w = 0; w < kFewWarps; ++w) top = max(top, tops[m][w]);
+      for (int w = 0; w < per; ++w) top = max(top, tops[m * per + w]);
       const Int8Scale s = int8_scale(__float_as_uint(int8_unpack2<FP16>(top).x));
       const float inv17 = 17.f * s.inv;
-      const uint16_t* xr = p.x + m / p.x_rows_per_batch * p.x_batch_stride + m % p.x_rows_per_batch * p.x_row_stride;
-      for (int c = threadIdx.x * 8; c < p.pitch; c += kFewThreads * 8) {
+#pragma unroll 4
+      for (int c = c0; c < p.pitch; c += step) {
         const uint4 raw = c < p.K ? int8_load8(xr, c, p.K, p.vec) : make_uint4(0, 0, 0, 0);
         int8_put8<FP16, false>(reinterpret_cast<int8_t*>(rows8) + m * p.pitch, c, p.pitch, s, inv17, raw);
       }
-      if (threadIdx.x == 0) row_scale[m] = int8_step(s);
+      if (c0 == 0) row_scale[m] = int8_step(s);
     }
   } else {
     const int chunks16 = p.pitch / 16;
@@ -191,9 +195,13 @@ int launch_few(const FewParams& p, cudaStream_t st) {
 bool int8_linear_few_takes(const hdit_int8_linear_args* a) {
   return a->m <= kInt8FewRows && a->m * few_pitch(a->k) <= 160 * 1024;
 }
+// Rows that take more than 44 KB leave the weights' stream too little of an SM's first-level cache, or room for one CTA only. us, here |
+// in tiles: 3 rows of 8192 -> 3072 12.9 | 16.5, 5 rows (40 KB) 15.4 | 16.4, 6 rows (48 KB) 21.5 | 16.4; 12288 -> 12288, 3 rows (36 KB)
+// 38 | 45, 4 rows (48 KB) 64 | 45. One or two rows always come here: they need no scratch.
+bool int8_linear_few_pays(const hdit_int8_linear_args* a) { return a->m <= 2 || a->m * few_pitch(a->k) <= 44 * 1024; }
 // Not where the result may take x's place (x = residual = out): a CTA would write what another one has yet to read.
 bool int8_linear_few_quantizes(const hdit_int8_linear_args* a) {
-  if (a->m > kOwnRows) return false;
+  if (a->m > 2 && a->m * a->k > 8192) return false;
   const int64_t per = a->x_rows_per_batch < a->m ? a->x_rows_per_batch : a->m, entries = (a->m + per - 1) / per;
   const uintptr_t x0 = reinterpret_cast<uintptr_t>(a->x), x1 = x0 + 2 * ((entries - 1) * a->x_batch_stride + (per - 1) * a->x_row_stride + a->k);
   const uintptr_t o0 = reinterpret_cast<uintptr_t>(a->out), o1 = o0 + 2 * ((a->m - 1) * a->ldo + a->n);

@@ -678,9 +678,9 @@ extern "C" int hdit_int8_linear(const hdit_int8_linear_args* a) {
     return set_error(HDIT_ERR_BAD_ARG, "x needs x_rows_per_batch > 0 and the alignment of its elements");
   if (a->tile < 0 || a->tile > 5) return set_error(HDIT_ERR_BAD_ARG, "tile must be 0 (choose) to 5");
   if (a->tile == 5 && !int8_linear_few_takes(a)) return set_error(HDIT_ERR_SHAPE, "too many rows, or too long ones, for the kernel for a few rows");
-  const bool few = a->tile == 5 || (a->tile == 0 && int8_linear_few_takes(a));
+  const bool few = a->tile == 5 || (a->tile == 0 && int8_linear_few_takes(a) && int8_linear_few_pays(a));
   const bool own_rows = few && a->x != nullptr && int8_linear_few_quantizes(a);  // a and a_scale are not used
-  if (!own_rows && (a->a == nullptr || a->a_scale == nullptr)) return set_error(HDIT_ERR_BAD_ARG, "null a / a_scale");
+  if (!(own_rows && a->m <= 2) && (a->a == nullptr || a->a_scale == nullptr)) return set_error(HDIT_ERR_BAD_ARG, "null a / a_scale");
   auto bad_rows = [&](const void* ptr, long long ld) { return (reinterpret_cast<uintptr_t>(ptr) & 15) != 0 || ld % 16 != 0 || ld < a->k; };
   if ((!own_rows && bad_rows(a->a, a->lda)) || bad_rows(a->w, a->ldw))
     return set_error(HDIT_ERR_SHAPE, "8-bit rows need a 16-byte aligned pointer and a row stride that is a multiple of 16 and covers a row");

@@ -1136,12 +1136,12 @@ def linear_int8(x, weight, bias=None, epilogue="bias", residual=None, gate=None,
         a.a, a.a_scale, a.lda = xr.data_ptr(), scale.data_ptr(), ss if S > 1 else pitch
     else:
         a.x, a.lda, a.x_rows_per_batch, a.x_batch_stride, a.x_row_stride = xr.data_ptr(), pitch, S, sb, ss
-        launches = 1
-        if not (own and m <= 2 and k <= 65536 and tile in (0, 5)):  # the rows in 8 bits, their scales behind them: scratch of the call
+        one = own and tile in (0, 5) and (m <= 2 and k <= 65536 or m <= 8 and m * k <= 8192)  # the kernel for a few rows does it all
+        launches = 1 if one else 2
+        if not one or m > 2:  # the rows in 8 bits, their scales behind them: scratch of the call
             scratch = torch.empty(m * (pitch + 4), dtype=torch.int8, device=dev)
             a.a = a.a_scale = scratch.data_ptr()
             a.a_scale += m * pitch
-            launches = 2
     a.w, a.ldw, a.w_scale = w_ptr, wn if n > 1 else pitch, w_scale.data_ptr()
     if bias is not None:
         a.bias = bias.data_ptr()

@@ -560,7 +560,8 @@ HDIT_API int hdit_ln_modulate_int8(int32_t dtype, const void* x, const void* shi
  * result is rounded to 16 bits once (hdit_linear_fused rounds before the tail, too).
  * a (m, k) and w (n, k) are 8-bit rows as above, a_scale and w_scale m and n contiguous floats. x != NULL: a and a_scale are
  * scratch that hdit_quantize_rows fills from these 16-bit rows first (x_rows_per_batch, x_batch_stride, x_row_stride as there); for one
- * or two rows of at most 65536 elements, with tile 0 or 5 and a result that lies apart from x, they are not used and may be NULL.
+ * or two rows of at most 65536 elements, with tile 0 or 5 and a result that lies apart from x, they are not used and may be NULL; for a
+ * few more short rows they may stay unused.
  * bias, gate, residual and out are 16-bit of `dtype`, any strides that keep rows of residual and out apart; m, n and k need not
  * be multiples of anything; rows_per_batch >= 1 (HDIT_GEMM_BIAS_GATE_RESIDUAL only). `out` may alias `residual`.
  * tile: 0 = the library chooses, 1 = 128 x 128 tiles, 2, 3, 4 = 256 x 128, 256 x 192, 256 x 256 on a CTA pair, 5 = the kernel for

@@ -257,6 +257,22 @@ def test_few_rows_give_the_bits_of_a_tile(B, S, K, N, epilogue):
         assert torch.equal(tile, kernels.linear_int8(rows, w, b, epilogue, residual=res, gate=gate, tile=5))
 
 
+@pytest.mark.parametrize("B,S,K", [(1, 3, 8), (3, 1, 2048), (1, 4, 2048), (2, 3, 1365), (5, 1, 1637), (1, 7, 999), (2, 4, 1024), (4, 2, 1025), (1, 8, 1)])
+def test_a_few_16_bit_rows_are_the_rows_in_8_bits(B, S, K):
+    """Up to 8192 elements the kernel brings them into 8 bits by itself, a row to some of its warps; one row without a number."""
+    from hetu_dit_b200 import kernels
+    x, w, b, res, gate = _layer(B, S, K, 75, torch.bfloat16, K)
+    wide = torch.full((B, S + 1, K + 3), float("inf"), dtype=torch.bfloat16, device=DEV)
+    wide[:, :S, 3:] = x
+    for rows in (x, wide[:, :S, 3:]):
+        want = kernels.linear_int8(kernels.quantize_rows(x), w, b, "gate_residual", residual=res, gate=gate, tile=1)
+        assert torch.equal(want, kernels.linear_int8(rows, w, b, "gate_residual", residual=res, gate=gate))
+    x[-1, 1 if S > 1 else 0, K // 2] = float("nan")
+    got = kernels.linear_int8(x, w, b)
+    want = kernels.linear_int8(kernels.quantize_rows(x), w, b, tile=1)
+    assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(got.nan_to_num(), want.nan_to_num()) and torch.isnan(got).sum() == 75
+
+
 @pytest.mark.parametrize("B,S", [(1, 1), (2, 1), (1, 2), (1, 5), (1, 40)])
 def test_result_in_the_place_of_x(B, S):
     """x = residual = out: a block's residual written over its input."""
