@@ -330,6 +330,20 @@ def test_results_and_residuals_that_start_anywhere(N, epilogue, tile):
             assert (wide[..., :off] == 7).all() and (wide[..., off + N:] == 7).all()
 
 
+@pytest.mark.parametrize("tile", [0, 1, 2, 3, 4, 5])
+@pytest.mark.parametrize("K", [1, 7, 15, 17, 33, 100, 127, 129, 250, 1001])
+def test_bytes_behind_8_bit_rows_are_not_summed(K, tile):
+    from hetu_dit_b200 import kernels
+    S, N = (6, 70) if tile in (0, 5) else (140, 300)
+    gen, rows = _gen(K), []
+    for n in (S, N):
+        q = torch.full((n, (K + 15) // 16 * 16 + 16), 101, dtype=torch.int8, device=DEV)
+        q[:, :K] = torch.randint(-127, 128, (n, K), generator=gen, device=DEV, dtype=torch.int8)
+        rows.append(kernels.Int8Rows(q[:, :K], torch.rand(n, generator=gen, device=DEV)))
+    want, tol = _tail64(kernels.Int8Rows(rows[0].q[None], rows[0].scale[None]), rows[1], None, "bias", None, None, torch.bfloat16)
+    _within(kernels.linear_int8(rows[0], rows[1], tile=tile), want[0], tol[0])
+
+
 @pytest.mark.parametrize("S", [5, 70])
 @pytest.mark.parametrize("epilogue", EPILOGUES)
 @pytest.mark.parametrize("N", [1, 9, 31, 60, 67, 129, 258, 300])
