@@ -11,6 +11,7 @@ import torch
 import torch.nn as nn
 
 from ... import kernels
+from ...core.distributed import parallel_state as ps
 
 
 class Int8Linear(nn.Module):
@@ -65,14 +66,24 @@ def read_rows(linears):
     return True
 
 
-@torch.no_grad()
-def quantize_linears_(module: nn.Module):
-    """Puts an Int8Linear in the place of every torch.nn.Linear below `module` (16-bit, on the GPU); returns module. What has
-    another class (an adapter) stays. Block caches address torch.nn.Linear weights by name: a module whose slices migrate
-    between plans keeps them."""
+def _replace_linears(module):
+    """How many layers below `module` were replaced."""
+    replaced = 0
     for name, child in module.named_children():
         if type(child) is nn.Linear:
             setattr(module, name, Int8Linear.from_linear(child))
+            replaced += 1
         else:
-            quantize_linears_(child)
+            replaced += _replace_linears(child)
+    return replaced
+
+
+@torch.no_grad()
+def quantize_linears_(module: nn.Module):
+    """Puts an Int8Linear in the place of every torch.nn.Linear below `module` (16-bit, on the GPU); returns module. What has
+    another class (an adapter) stays. Steps captured in CUDA graphs before hold the addresses of the 16-bit weights: those of
+    every StepGraphCache are dropped. Block caches address torch.nn.Linear weights by name: a module whose slices migrate
+    between plans keeps them."""
+    if _replace_linears(module) and ps.model_parallel_is_initialized():
+        ps.get_parallel_groups().void_captured_graphs()
     return module

@@ -473,7 +473,6 @@ class ShapedDiT(nn.Module):
         moves between plans, which addresses torch.nn.Linear weights."""
         for blk in list(self.transformer_blocks) + list(self.single_transformer_blocks):
             quantize_linears_(blk)
-        self.__dict__.pop("_step_graphs", None)  # captured with the 16-bit weights
         return self
 
     def register_cache(self):

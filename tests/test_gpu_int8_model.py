@@ -75,3 +75,43 @@ def test_int8_linear_layer_is_the_product_over_its_rows():
         moved = Int8Linear.from_linear(linear).to("cpu").to(DEV)  # the rows keep their places
         assert torch.equal(moved(x), want)
         assert _cosine(want, linear(x)) >= 0.999
+
+
+@pytest.mark.parametrize("through", ["model", "blocks"])
+@torch.no_grad()
+def test_a_pipeline_that_ran_in_16_bits_runs_the_8_bit_layers(through):
+    """The pipeline keeps captured steps of its own."""
+    from hetu_dit_b200 import _C
+    from hetu_dit_b200.config import EngineConfig
+    from hetu_dit_b200.core.distributed import parallel_state as ps
+    from hetu_dit_b200.core.distributed.runtime_state import ModelGeometry, initialize_runtime_state, reset_runtime_state
+    from hetu_dit_b200.core.resource_manager.cache_manager import reset_cache_manager
+    from hetu_dit_b200.model_executor.layers.int8_linear import quantize_linears_
+    from hetu_dit_b200.model_executor.pipelines.pipeline_flux_shaped import FluxShapedPipeline
+    from tests.test_gpu_pipefusion import _tiny_flux
+    _, model, *inputs = _tiny_flux()
+    model, inputs = model.to(DEV), [x.to(DEV) for x in inputs]
+    ps.destroy_model_parallel()
+    reset_cache_manager()
+    rt = initialize_runtime_state(ModelGeometry(4, 64), EngineConfig())
+    rt.set_input_parameters(height=512, width=256, batch_size=1, num_inference_steps=4)
+    try:
+        pipe = FluxShapedPipeline(model, guidance_scale=3.5, grid=(32, 16))
+        steps = lambda: pipe.diffusion_stage(*inputs, 4).clone()  # noqa: E731
+        in_16_bits = steps()
+        assert pipe._graphs.captures == 1 and pipe._graphs.replays == 3
+        if through == "model":
+            model.quantize_linears_()
+        else:
+            quantize_linears_(model.transformer_blocks)
+            quantize_linears_(model.single_transformer_blocks)
+        got = steps()
+        assert pipe._graphs.captures == 2
+        assert torch.equal(steps(), got)  # replays only
+        pipe.use_cuda_graph = False
+        assert torch.equal(steps(), got) and not torch.equal(got, in_16_bits)
+        torch.cuda.synchronize()
+        assert _C.device_status(0, clear=True)[0] == 0
+    finally:
+        reset_runtime_state()
+        reset_cache_manager()

@@ -238,3 +238,23 @@ def test_an_attention_of_its_own_needs_no_projections():
     from hetu_dit_b200.model_executor.models import shaped_dit
     assert not shaped_dit._sees_rows(torch.nn.Identity(), JointAttnProcessor, ("to_q",))
     assert not shaped_dit._sees_rows(shaped_dit._Wrapped(torch.nn.Identity()), JointAttnProcessor, ("to_q",))
+
+
+def test_steps_seen_before_layers_were_replaced_are_not_captured_or_replayed(monkeypatch):
+    """A step cache that lives anywhere (a model's, a pipeline's) forgets what it holds. Its first run of a key is eager, the
+    second one captures, for which it asks the step's inputs for their device: there are none here."""
+    from hetu_dit_b200.model_executor.layers.int8_linear import quantize_linears_
+    from hetu_dit_b200.model_executor.step_graph import StepGraphCache
+    monkeypatch.setattr(kernels, "quantize_rows", lambda w: rows8(*w.shape))
+    cache, runs = StepGraphCache(), []
+    step = lambda: runs.append(1)  # noqa: E731
+    cache.run("step", step)
+    with pytest.raises(StopIteration):
+        cache.run("step", step)
+    net = torch.nn.ModuleList([torch.nn.ModuleList([torch.nn.Linear(8, 16)])])
+    quantize_linears_(net)
+    cache.run("step", step)
+    assert len(runs) == 2
+    quantize_linears_(net)  # nothing is left to replace: what was captured since stays
+    with pytest.raises(StopIteration):
+        cache.run("step", step)
