@@ -1098,6 +1098,8 @@ def linear_int8(x, weight, bias=None, epilogue="bias", residual=None, gate=None,
                 raise ValueError("x must be int8 with a fp32 scale for each row, on one device")
             if (ss % 16 and S != 1) or (sb % 16 and B != 1) or xr.data_ptr() % 16:
                 raise ValueError("x's rows must start on 16-byte boundaries, as quantize_rows() lays them out")
+            if S == 1:
+                ss = sb  # of one row to an entry only the entries' stride counts
             one_pitch = sb == S * ss and scale.is_contiguous()
     if bias is not None and (bias.numel() != n or not bias.is_contiguous() or bias.dtype != dtype or bias.device != dev):
         raise ValueError("bias must be N contiguous elements of x's dtype, on its device")
@@ -1133,7 +1135,7 @@ def linear_int8(x, weight, bias=None, epilogue="bias", residual=None, gate=None,
     elif held:
         if not scale.is_contiguous():
             scale = scale.contiguous()
-        a.a, a.a_scale, a.lda = xr.data_ptr(), scale.data_ptr(), ss if S > 1 else pitch
+        a.a, a.a_scale, a.lda = xr.data_ptr(), scale.data_ptr(), ss if m > 1 else pitch
     else:
         a.x, a.lda, a.x_rows_per_batch, a.x_batch_stride, a.x_row_stride = xr.data_ptr(), pitch, S, sb, ss
         one = own and tile in (0, 5) and (m <= 2 and k <= 65536 or m <= 8 and m * k <= 8192)  # the kernel for a few rows does it all

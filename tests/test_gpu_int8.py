@@ -646,3 +646,20 @@ def test_group_norm_beyond_2_to_31_elements():
     tol = off * (1 + 2.0 ** -8) + 2.0 ** -12 + _half_step(want, torch.bfloat16)  # thousands of terms in a thread
     for at in (0, 1 << 23, x.shape[1] - 2):
         _within(got[:, at:at + 2], want, tol)
+
+
+@pytest.mark.parametrize("B,S", [(4, 1), (9, 1), (140, 1), (1, 9), (3, 50)])
+def test_rows_wider_than_they_have_to_be(B, S):
+    """Rows that a program has laid out itself: the columns of wider ones, one to an entry or several."""
+    from hetu_dit_b200 import kernels
+    gen = _gen(B + S)
+    w = kernels.quantize_rows(_randn(gen, 33, 40, dtype=torch.bfloat16))
+    held = kernels.quantize_rows(_randn(gen, B, S, 40, dtype=torch.bfloat16))
+    want = kernels.linear_int8(held, w)
+    wide = torch.full((B, S, 64), 77, dtype=torch.int8, device=DEV)
+    wide[..., :40] = held.q
+    views = [wide[..., :40]]
+    if S == 1:
+        views.append(wide[:, 0, :40][:, None])  # the same place, another stride of the one row
+    for q in views:
+        assert torch.equal(kernels.linear_int8(kernels.Int8Rows(q, held.scale), w), want)

@@ -258,3 +258,21 @@ def test_steps_seen_before_layers_were_replaced_are_not_captured_or_replayed(mon
     quantize_linears_(net)  # nothing is left to replace: what was captured since stays
     with pytest.raises(StopIteration):
         cache.run("step", step)
+
+
+def _wide_rows(B, S, k, width, unsqueezed=False):
+    """Rows of k in a buffer of `width` bytes to a row; unsqueezed: the rows of a matrix, each an entry of its own."""
+    q = torch.randint(-127, 128, (B, S, width), dtype=torch.int8)[..., :k]
+    if unsqueezed:
+        q = q[:, 0][:, None]
+    return kernels.Int8Rows(q.as_subclass(OnGpu), torch.rand(B, S).as_subclass(OnGpu))
+
+
+@pytest.mark.parametrize("B, S, unsqueezed", [(4, 1, False), (4, 1, True), (1, 4, False), (2, 3, False)])
+def test_rows_wider_than_they_have_to_be_are_addressed_by_their_stride(lib, monkeypatch, B, S, unsqueezed):  # noqa: F811
+    monkeypatch.setattr(kernels, "_cuda_index", lambda device: 0)
+    x = _wide_rows(B, S, 40, 64, unsqueezed)
+    kernels.linear_int8(x, rows8(24, 40), out=gpu_like(B, S, 24))
+    (name, args), = lib.calls
+    a = args[0]._obj
+    assert (name, a.m, a.lda, a.a) == ("hdit_int8_linear", B * S, 64, x.q.data_ptr())
