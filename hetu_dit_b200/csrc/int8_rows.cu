@@ -53,6 +53,7 @@ __global__ void __launch_bounds__(kRowThreads, rows_ctas(NCH, LN, VEC)) int8_row
   const long long first = static_cast<long long>(blockIdx.x) * kTeams + threadIdx.x / TEAM, step = static_cast<long long>(gridDim.x) * kTeams;
   const float inv_dim = 1.f / static_cast<float>(p.dim);
   const int chunks = p.dim / 8;
+  int turn = 0;  // goes on from entry to entry: without the norm no other barrier stands between the last row of one and the first of the next
   for (long long b = blockIdx.y; b < p.batches; b += gridDim.y) {
     const uint16_t* xr = p.x + b * p.x_batch_stride + first * p.x_row_stride;
     const long long row0 = b * p.rows_per_batch;
@@ -85,7 +86,6 @@ __global__ void __launch_bounds__(kRowThreads, rows_ctas(NCH, LN, VEC)) int8_row
       }
       __syncthreads();
     }
-    int turn = 0;
     for (long long r = first; r < p.rows_per_batch; r += step, turn ^= 1) {
       uint4 raw[NCH];
 #pragma unroll

@@ -663,3 +663,19 @@ def test_rows_wider_than_they_have_to_be(B, S):
         views.append(wide[:, 0, :40][:, None])  # the same place, another stride of the one row
     for q in views:
         assert torch.equal(kernels.linear_int8(kernels.Int8Rows(q, held.scale), w), want)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("k", [200, 1032, 1033, 2504, 5000, 20000])
+def test_more_entries_than_a_grid_has_rows_of_ctas(k, dtype):
+    """A CTA goes from one entry to another, with one row of each: windows that move on by eight elements."""
+    from hetu_dit_b200 import kernels
+    B = 65535 + 300
+    long = _randn(_gen(k), 8 * B + k, dtype=dtype)
+    x = long.as_strided((B, 1, k), (8, k, 1))
+    got = kernels.quantize_rows(x)
+    for at in (slice(0, 400), slice(B - 400, B)):
+        q, s = _rows64(x[at])
+        assert torch.equal(got.q[at], q) and torch.equal(got.scale[at], s)
+    again = kernels.quantize_rows(x)
+    assert torch.equal(again.q, got.q) and torch.equal(again.scale, got.scale)
