@@ -504,12 +504,15 @@ int check_gn(const hdit_group_norm_args* a) {
 
 bool off16(const void* p, int64_t a, int64_t b) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0 || a % 8 != 0 || b % 8 != 0; }
 
-template <typename K>
-cudaError_t launch_strips(K kernel, const GnParams& p, long long batch, size_t smem, cudaStream_t st) {
+// of the two launches' kernels: the sums of 8 channels and 512 lanes, the factors of 4096 channels and as many groups
+constexpr int kGnMaxBytes = 64 * 1024;
+
+template <auto kKernel>
+cudaError_t launch_strips(const GnParams& p, long long batch, size_t smem, cudaStream_t st) {
   // static shared memory counts, too
-  const cudaError_t e = smem > 47 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) : cudaSuccess;
+  const cudaError_t e = smem > 47 * 1024 ? allow_shared_memory<kKernel, kGnMaxBytes>() : cudaSuccess;
   if (e != cudaSuccess) return e;
-  return launch_overlapped(kernel, dim3(static_cast<unsigned>(p.strips.strips), static_cast<unsigned>(batch)), dim3(kGnThreads), smem, st, 1, p);
+  return launch_overlapped(kKernel, dim3(static_cast<unsigned>(p.strips.strips), static_cast<unsigned>(batch)), dim3(kGnThreads), smem, st, 1, p);
 }
 
 GnParams params_of(const hdit_group_norm_args* a, bool out_vec) {
@@ -539,24 +542,24 @@ size_t factor_bytes(const GnParams& p) { return static_cast<size_t>(p.channels) 
 template <bool FP16, bool VEC>
 cudaError_t launch_stats(const GnParams& p, long long batch, cudaStream_t st) {
   const size_t smem = static_cast<size_t>(kGnThreads / (p.channels / 8)) * stats_pitch(p.channels) * 2 * sizeof(float);
-  return launch_strips(group_norm_stats_kernel<FP16, VEC>, p, batch, smem, st);
+  return launch_strips<group_norm_stats_kernel<FP16, VEC>>(p, batch, smem, st);
 }
 
 template <bool FP16, bool VEC>
 cudaError_t launch_apply(const GnParams& p, long long batch, cudaStream_t st) {
-  return p.act == HDIT_ACT_SILU ? launch_strips(group_norm_apply_kernel<FP16, true, VEC>, p, batch, factor_bytes(p), st)
-                                : launch_strips(group_norm_apply_kernel<FP16, false, VEC>, p, batch, factor_bytes(p), st);
+  return p.act == HDIT_ACT_SILU ? launch_strips<group_norm_apply_kernel<FP16, true, VEC>>(p, batch, factor_bytes(p), st)
+                                : launch_strips<group_norm_apply_kernel<FP16, false, VEC>>(p, batch, factor_bytes(p), st);
 }
 
 template <bool FP16, bool SILU, bool VEC>
 cudaError_t launch_int8_act(const GnParams& p, long long batch, cudaStream_t st) {
-  auto kernel = p.channels <= 64     ? group_norm_int8_kernel<FP16, SILU, 8, 1, 4, VEC>
-                : p.channels <= 128  ? group_norm_int8_kernel<FP16, SILU, 16, 1, 4, VEC>
-                : p.channels <= 256  ? group_norm_int8_kernel<FP16, SILU, 32, 1, 4, VEC>
-                : p.channels <= 512  ? group_norm_int8_kernel<FP16, SILU, 32, 2, 2, VEC>
-                : p.channels <= 1024 ? group_norm_int8_kernel<FP16, SILU, 32, 4, 1, VEC>
-                                     : group_norm_int8_kernel<FP16, SILU, 128, 4, 1, VEC>;
-  return launch_strips(kernel, p, batch, factor_bytes(p), st);
+  const size_t smem = factor_bytes(p);
+  if (p.channels <= 64) return launch_strips<group_norm_int8_kernel<FP16, SILU, 8, 1, 4, VEC>>(p, batch, smem, st);
+  if (p.channels <= 128) return launch_strips<group_norm_int8_kernel<FP16, SILU, 16, 1, 4, VEC>>(p, batch, smem, st);
+  if (p.channels <= 256) return launch_strips<group_norm_int8_kernel<FP16, SILU, 32, 1, 4, VEC>>(p, batch, smem, st);
+  if (p.channels <= 512) return launch_strips<group_norm_int8_kernel<FP16, SILU, 32, 2, 2, VEC>>(p, batch, smem, st);
+  if (p.channels <= 1024) return launch_strips<group_norm_int8_kernel<FP16, SILU, 32, 4, 1, VEC>>(p, batch, smem, st);
+  return launch_strips<group_norm_int8_kernel<FP16, SILU, 128, 4, 1, VEC>>(p, batch, smem, st);
 }
 
 template <bool FP16, bool VEC>

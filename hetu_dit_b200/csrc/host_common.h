@@ -58,6 +58,20 @@ cudaError_t launch_overlapped(void (*kernel)(KernelArgs...), dim3 grid, dim3 blo
   return err;
 }
 
+// Lets a kernel be launched with up to kBytes of dynamic shared memory. The limit belongs to the kernel on its device, not to a
+// call or a host thread: every call sets the same one, the most that any call takes, so that none lowers it between another
+// thread's set-up and launch.
+template <auto kKernel, int kBytes>
+cudaError_t allow_shared_memory() {
+  static thread_local int last_dev = -1;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || dev == last_dev) return e;
+  e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+  if (e == cudaSuccess) last_dev = dev;
+  return e;
+}
+
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_dependency_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

@@ -25,6 +25,7 @@ constexpr int kFewThreads = 256;
 constexpr int kFewWarps = kFewThreads / 32;
 constexpr int kChunksAhead = 4;
 constexpr int kFewCtas = 4;  // to an SM
+constexpr int kFewMaxBytes = 160 * 1024;  // of rows in shared memory
 
 struct FewParams {
   const uint16_t* x;  // or null: a, a_scale hold the rows
@@ -182,9 +183,9 @@ int few_pitch(long long k) {
 
 template <bool FP16>
 int launch_few(const FewParams& p, cudaStream_t st) {
-  auto kernel = int8_linear_few_kernel<FP16>;
+  constexpr auto kernel = int8_linear_few_kernel<FP16>;
   const int smem = p.M * p.pitch;
-  if (smem > 32 * 1024) HDIT_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  if (smem > 32 * 1024) HDIT_CUDA_OK((allow_shared_memory<kernel, kFewMaxBytes>()));
   const int groups = (p.N + 15) / 16, most = sm_count() * kFewCtas;
   HDIT_CUDA_OK(launch_overlapped(kernel, dim3(static_cast<unsigned>(groups < most ? groups : most)), dim3(kFewThreads), static_cast<size_t>(smem), st, 1, p));
   return HDIT_OK;
@@ -193,7 +194,7 @@ int launch_few(const FewParams& p, cudaStream_t st) {
 }  // namespace
 
 bool int8_linear_few_takes(const hdit_int8_linear_args* a) {
-  return a->m <= kInt8FewRows && a->m * few_pitch(a->k) <= 160 * 1024;
+  return a->m <= kInt8FewRows && a->m * few_pitch(a->k) <= kFewMaxBytes;
 }
 // Rows that take more than 44 KB leave the weights' stream too little of an SM's first-level cache, or room for one CTA only. us, here |
 // in tiles: 3 rows of 8192 -> 3072 12.9 | 16.5, 5 rows (40 KB) 15.4 | 16.4, 6 rows (48 KB) 21.5 | 16.4; 12288 -> 12288, 3 rows (36 KB)

@@ -17,6 +17,8 @@
 namespace hdit {
 namespace {
 
+constexpr int kMaxNormDim = 8192;
+
 struct RowsParams {
   const uint16_t* x;
   const uint16_t* x_end;  // the end of the last row
@@ -209,10 +211,10 @@ dim3 rows_grid(const RowsParams& p, long long teams, long long ctas) {
 
 template <bool FP16, int TEAM, int NCH, bool LN, bool VEC>
 cudaError_t launch_rows(const RowsParams& p, cudaStream_t st) {
-  auto kernel = int8_rows_kernel<FP16, TEAM, NCH, LN, VEC>;
+  constexpr auto kernel = int8_rows_kernel<FP16, TEAM, NCH, LN, VEC>;
   const size_t smem = LN ? static_cast<size_t>(p.dim) * 2 * sizeof(float) : 0;
   if (smem > 47 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    const cudaError_t e = allow_shared_memory<kernel, kMaxNormDim * 2 * static_cast<int>(sizeof(float))>();
     if (e != cudaSuccess) return e;
   }
   return launch_overlapped(kernel, rows_grid(p, kRowThreads / TEAM, rows_ctas(NCH, LN, VEC)), dim3(kRowThreads), smem, st, 1, p);
@@ -293,7 +295,7 @@ extern "C" int hdit_ln_modulate_int8(int32_t dtype, const void* x, const void* s
   using namespace hdit;
   const int rc = check_rows(dtype, x, q, q_scale, rows, dim, rows_per_batch, q_row_stride);
   if (rc != HDIT_OK) return rc;
-  if (dim % 8 != 0 || dim > 8192) return set_error(HDIT_ERR_SHAPE, "row length must be a multiple of 8 and at most 8192");
+  if (dim % 8 != 0 || dim > kMaxNormDim) return set_error(HDIT_ERR_SHAPE, "row length must be a multiple of 8 and at most %d", kMaxNormDim);
   if (rows == 0) return HDIT_OK;
   if (shift == nullptr || scale == nullptr) return set_error(HDIT_ERR_BAD_ARG, "null shift / scale");
   if (((reinterpret_cast<uintptr_t>(shift) | reinterpret_cast<uintptr_t>(scale)) & 1) != 0)

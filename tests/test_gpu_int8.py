@@ -679,3 +679,79 @@ def test_more_entries_than_a_grid_has_rows_of_ctas(k, dtype):
         assert torch.equal(got.q[at], q) and torch.equal(got.scale[at], s)
     again = kernels.quantize_rows(x)
     assert torch.equal(again.q, got.q) and torch.equal(again.scale, got.scale)
+
+
+def _room_calls():
+    """Calls of one kernel that take more and less shared memory than each other, beyond what a launch may have unasked."""
+    from hetu_dit_b200 import kernels
+    gen = _gen(5)
+    dtype = torch.bfloat16
+    calls = {}
+    for name, sizes in (("few rows", (40000, 20000)), ("norm", (8192, 6152)), ("group norm", (4096, 2048)), ("group norm, 8-bit rows", (4096, 2048))):
+        for size in sizes:
+            if name == "few rows":
+                x, w = _randn(gen, 1, 2, size, dtype=dtype), kernels.quantize_rows(_randn(gen, 16, size, dtype=dtype))
+                call = lambda x=x, w=w: kernels.linear_int8(x, w)  # noqa: E731
+            elif name == "norm":
+                x, m = _randn(gen, 1, 3, size, dtype=dtype), _randn(gen, 2, 1, size, dtype=dtype)
+                call = lambda x=x, m=m: kernels.ln_modulate_int8(x, m[0], m[1]).q  # noqa: E731
+            else:
+                x = _randn(gen, 40, 9, 4096, dtype=dtype)  # too many images for a cluster each
+                if name == "group norm":
+                    call = lambda x=x, g=size: kernels.group_norm(x, g)  # noqa: E731
+                else:
+                    call = lambda x=x, g=size: kernels.group_norm_int8(x, g).q  # noqa: E731
+            calls.setdefault(name, []).append(call)
+    return calls
+
+
+@pytest.mark.parametrize("name", ["few rows", "norm", "group norm", "group norm, 8-bit rows"])
+def test_calls_of_two_threads_leave_each_other_their_shared_memory(name):
+    """What a kernel may take belongs to the device, not to the call: the smaller call of one thread must not take the larger
+    one's room between its set-up and its launch."""
+    import threading
+    calls = _room_calls()[name]
+    want = [call() for call in calls]
+    failed, done = [], []
+
+    def work(call, want):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(400):
+                    got = call()
+                torch.cuda.current_stream().synchronize()
+                done.append(torch.equal(got, want))
+        except Exception as e:  # noqa: BLE001
+            failed.append(e)
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=a) for a in list(zip(calls, want)) * 2]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed and done == [True] * 4, failed[:1]
+
+
+@pytest.mark.parametrize("name", ["few rows", "norm", "group norm", "group norm, 8-bit rows"])
+def test_a_larger_call_and_a_smaller_one_in_one_graph(name):
+    calls = _room_calls()[name]
+    want = [call() for call in calls]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = [call() for call in calls]
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("name", ["few rows", "norm", "group norm", "group norm, 8-bit rows"])
+def test_a_smaller_call_leaves_a_kernel_what_a_larger_one_takes(name):
+    from tests.captured_kernels import MOST_DYNAMIC_SHARED, captured_kernels
+    large, small = _room_calls()[name]
+    kernels = captured_kernels(large)
+    assert max(k.shared_bytes for k in kernels) > 48 * 1024
+    small()
+    for k in kernels:
+        assert k.attribute(MOST_DYNAMIC_SHARED) >= k.shared_bytes
