@@ -5,7 +5,8 @@
 //
 // Two launches of one CTA per SM. The first one reads x once: a strip (a CTA) takes every strips-th tile of rows of an image,
 // each thread eight fixed channels, and leaves {mean, sum of squared distances from it} per group and strip. Sums are taken
-// relative to a value of the strip's first row, so that a mean far from zero costs no digits. The second one joins the strips
+// relative to a value of the strip's first row, means relative to the group's pivot, its first value in the image, so that a
+// mean far from zero costs no digits. The second one joins the strips
 // (Chan's formula) and reads x again from its end to its start: what the first launch read last is still in L2. Every CTA joins
 // the strips of its image by itself; with four strips per SM, read eight at a time by a thread, that alone took 3 us.
 // All CTAs work on neighbouring tiles at a time: with one stretch of rows each, 1024 x 1024 x 128 took 148 us (4.8 TB/s of
@@ -48,7 +49,8 @@ struct GnParams {
   uint16_t* out;
   int8_t* q;
   float* q_scale;
-  float2* partial;  // (batch, strips, groups): mean, sum of squared distances from it
+  float2* partial;  // (batch, strips, groups): mean from the pivot, sum of squared distances from the mean
+  uint16_t* pivots;  // (batch, groups)
   long long rows, x_batch_stride, x_row_stride, out_batch_stride, out_row_stride;  // q: out_row_stride only, rows of all images
   Strips strips;
   int channels, groups, act, slab;
@@ -100,9 +102,14 @@ __device__ __forceinline__ void walk_rows(const uint16_t* x, int c, int channels
 
 // Floats from one lane's sums to the next one's: lanes that are summed side by side are in banks of their own (two launches over 64 x 16 8.0 -> 6.5 us; the cluster over 4096 x 512 8.8 -> 7.9)
 __host__ __device__ constexpr int stats_pitch(int channels) { return channels + 4; }
+// of the cluster's sums; the factors take their place
+__host__ __device__ constexpr int sums_bytes(int lanes, int channels) {
+  return lanes * stats_pitch(channels) * 8 > channels * 10 ? lanes * stats_pitch(channels) * 8 : channels * 10;
+}
 
 // Statistics of strip k of an image of `rows` rows of `channels` channels at `x`. A thread passes its eight channels of every lanes-th
-// row to keep(raw, index). smem: [lanes][stats_pitch(channels)] sums, then the same of squares. put(group, {mean, sum of squared distances from it}).
+// row to keep(raw, index). smem: [lanes][stats_pitch(channels)] sums, then the same of squares. put(group, {mean from the pivot, sum of
+// squared distances from the mean}, the pivot's bits).
 template <int THREADS, bool FP16, bool VEC, typename K, typename P>
 __device__ __forceinline__ void strip_stats(const uint16_t* x, long long row_stride, const Strips& strips, int strip, int channels, int per, float* smem, K keep,
                                             P put) {
@@ -158,7 +165,7 @@ __device__ __forceinline__ void strip_stats(const uint16_t* x, long long row_str
     q = sub_sum(q, parts);
     if (ch < channels && part == 0) {  // no other thread reads this channel's first lane
       const float m2 = q - a * a * inv_rows;
-      smem[ch] = int8_unpack2<FP16>(xs[ch]).x + a * inv_rows;
+      smem[ch] = (int8_unpack2<FP16>(xs[ch]).x - int8_unpack2<FP16>(x[ch / per * per]).x) + a * inv_rows;
       smem[lanes * pitch + ch] = m2 > 0.f ? m2 : m2 - m2;  // keeps NaN
     }
   }
@@ -174,7 +181,7 @@ __device__ __forceinline__ void strip_stats(const uint16_t* x, long long row_str
       m2 += smem[lanes * pitch + g * per + k] + n * d * d;
     }
     m2 = sub_sum(m2, n_sub);
-    if (live && sub == 0) put(g, make_float2(mean, m2));
+    if (live && sub == 0) put(g, make_float2(mean, m2), x[g * per]);
   });
 }
 
@@ -185,11 +192,14 @@ __global__ void __launch_bounds__(kGnThreads, 1) group_norm_stats_kernel(const _
   extern __shared__ float smem[];
   float2* out = p.partial + (static_cast<long long>(blockIdx.y) * p.strips.strips + blockIdx.x) * p.groups;
   strip_stats<kGnThreads, FP16, VEC>(p.x + blockIdx.y * p.x_batch_stride, p.x_row_stride, p.strips, static_cast<int>(blockIdx.x), p.channels,
-                                     p.channels / p.groups, smem, [](const uint4&, int) {}, [&](int g, float2 v) { out[g] = v; });
+                                     p.channels / p.groups, smem, [](const uint4&, int) {}, [&](int g, float2 v, uint16_t pivot) {
+                                       out[g] = v;
+                                       if (blockIdx.x == 0) p.pivots[static_cast<long long>(blockIdx.y) * p.groups + g] = pivot;
+                                     });
 }
 
-// {mean, 1 / deviation} of `groups` groups from `strips` strips of an image, `per` channels to a group, into stat[groups].
-// in(strip, group): the strip's {mean, sum of squared distances from it}.
+// {mean from the pivot, 1 / deviation} of `groups` groups from `strips` strips of an image, `per` channels to a group, into
+// stat[groups]. in(strip, group): the strip's {mean from the pivot, sum of squared distances from the mean}.
 template <typename F>
 __device__ __forceinline__ void join_strips(int groups, const Strips& strips, long long rows, int per, float eps, float2* stat, F in) {
   const float inv_total = 1.f / (static_cast<float>(rows) * static_cast<float>(per));
@@ -212,17 +222,19 @@ __device__ __forceinline__ void join_strips(int groups, const Strips& strips, lo
   });
 }
 
-// y = x * a + b with a = weight / deviation and b = bias - mean * a, for each channel in shared memory: `factors` holds a, then b, each first for the lower four channels of every chunk of eight, then for the upper four, so
-// that threads' 16 bytes lie side by side.
-// Against (x - mean) * a + bias this form costs half a unit of 2^-24 of mean * a: a 16-bit x resolves the deviation only while
-// |mean| is below some 2^11 deviations, where that is under 2^-13 of the result's deviation.
-template <bool FP16>
-__device__ __forceinline__ void put_factor(int c, int chunks, float2 stat, float weight, float bias, float4* factors) {
+// y = (x - pivot) * a + b with a = weight / deviation and b = bias - (mean - pivot) * a, for each channel in shared memory: `factors`
+// holds a, then b, each first for the lower four channels of every chunk of eight, then for the upper four, so that threads' 16
+// bytes lie side by side, then -pivot as 16-bit values. No term has the size of the mean: in the form x * a + (bias - mean * a), half
+// a unit of 2^-24 of mean * a was off, which at a constant image of 500 with an eps of 1e-6 is 0.03. The pivot is one of the group's
+// n values, no more than sqrt(n) deviations from the mean.
+__device__ __forceinline__ void put_factor(int c, int chunks, float2 stat, float weight, float bias, uint16_t pivot, float4* factors) {
   const float a = stat.y * weight;
   float* to = reinterpret_cast<float*>(factors) + (c >> 3) * 4 + ((c >> 2) & 1) * chunks * 4 + (c & 3);
   to[0] = a;
   to[8 * chunks] = fmaf(-stat.x, a, bias);
+  reinterpret_cast<uint16_t*>(factors + 4 * chunks)[c] = pivot ^ 0x8000u;
 }
+__host__ __device__ constexpr int factor_bytes(int channels) { return channels * 10; }
 template <bool FP16>
 __device__ __forceinline__ float gn_weight(const GnParams& p, int c) { return p.weight != nullptr ? int8_unpack2<FP16>(p.weight[c]).x : 1.f; }
 template <bool FP16>
@@ -232,7 +244,8 @@ __device__ __forceinline__ float gn_bias(const GnParams& p, int c) { return p.bi
 template <bool FP16>
 __device__ __forceinline__ void group_norm_factors(const GnParams& p, float4* factors) {
   const int per = p.channels / p.groups;
-  float2* stat = reinterpret_cast<float2*>(factors + p.channels / 2);
+  float2* stat = reinterpret_cast<float2*>(factors + factor_bytes(p.channels) / 16);
+  const uint16_t* pivots = p.pivots + static_cast<long long>(blockIdx.y) * p.groups;
   const float2* in = p.partial + static_cast<long long>(blockIdx.y) * p.strips.strips * p.groups;
   float weight = 1.f, bias = 0.f;  // on their way while the strips are joined
   if (threadIdx.x < p.channels) {
@@ -241,9 +254,9 @@ __device__ __forceinline__ void group_norm_factors(const GnParams& p, float4* fa
   }
   join_strips(p.groups, p.strips, p.rows, per, p.eps, stat, [&](int k, int g) { return in[static_cast<long long>(k) * p.groups + g]; });
   __syncthreads();
-  if (threadIdx.x < p.channels) put_factor<FP16>(threadIdx.x, p.channels / 8, stat[threadIdx.x / per], weight, bias, factors);
+  if (threadIdx.x < p.channels) put_factor(threadIdx.x, p.channels / 8, stat[threadIdx.x / per], weight, bias, pivots[threadIdx.x / per], factors);
   for (int c = threadIdx.x + kGnThreads; c < p.channels; c += kGnThreads)
-    put_factor<FP16>(c, p.channels / 8, stat[c / per], gn_weight<FP16>(p, c), gn_bias<FP16>(p, c), factors);
+    put_factor(c, p.channels / 8, stat[c / per], gn_weight<FP16>(p, c), gn_bias<FP16>(p, c), pivots[c / per], factors);
   __syncthreads();
 }
 
@@ -267,12 +280,12 @@ __device__ __forceinline__ uint32_t gn_pack(float lo, float hi) {
 
 // Eight channels of a row, normalised, to dst.
 template <bool FP16, bool SILU, bool VEC>
-__device__ __forceinline__ void apply8(const uint4& raw, const float (&a)[8], const float (&b)[8], uint16_t* dst) {
+__device__ __forceinline__ void apply8(const uint4& raw, const float (&a)[8], const float (&b)[8], const uint4& minus_pivot, uint16_t* dst) {
   uint4 y = raw;
   uint32_t* u = reinterpret_cast<uint32_t*>(&y);
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    const float2 v = int8_unpack2<FP16>(u[k]);
+    const float2 v = add2(int8_unpack2<FP16>(u[k]), int8_unpack2<FP16>(reinterpret_cast<const uint32_t*>(&minus_pivot)[k]));
     float y0 = fmaf(v.x, a[2 * k], b[2 * k]), y1 = fmaf(v.y, a[2 * k + 1], b[2 * k + 1]);
     if constexpr (SILU) y0 = silu(y0), y1 = silu(y1);
     u[k] = gn_pack<FP16>(y0, y1);
@@ -284,7 +297,8 @@ __device__ __forceinline__ void apply8(const uint4& raw, const float (&a)[8], co
     for (int k = 0; k < 8; ++k) dst[k] = static_cast<uint16_t>(u[k / 2] >> (16 * (k & 1)));
   }
 }
-__device__ __forceinline__ void read_factors(const float4* factors, int chunks, int chunk, float (&a)[8], float (&b)[8]) {
+__device__ __forceinline__ void read_factors(const float4* factors, int chunks, int chunk, float (&a)[8], float (&b)[8], uint4& minus_pivot) {
+  minus_pivot = *reinterpret_cast<const uint4*>(factors + 4 * chunks + chunk);
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     *reinterpret_cast<float4*>(a + 4 * h) = factors[h * chunks + chunk];
@@ -303,13 +317,14 @@ __global__ void __launch_bounds__(kGnThreads, 1) group_norm_apply_kernel(const _
   group_norm_factors<FP16>(p, factors);
   if (lane >= lanes) return;
   float a[8], b[8];
-  read_factors(factors, chunks, chunk, a, b);
+  uint4 minus_pivot;
+  read_factors(factors, chunks, chunk, a, b, minus_pivot);
   // the strip's rows from the last to the first
   const int strip = static_cast<int>(blockIdx.x), count = p.strips.rows_of_lane(strip, lane);
   const long long step = p.strips.step(), last = p.strips.first(strip, lane) + (count - 1) * step, out_step = step * p.out_row_stride;
   uint16_t* out = p.out + blockIdx.y * p.out_batch_stride + last * p.out_row_stride + c;
   walk_rows<VEC>(p.x + blockIdx.y * p.x_batch_stride + last * p.x_row_stride, c, p.channels, count, -step * p.x_row_stride,
-                 [&](const uint4& raw, int i) { apply8<FP16, SILU, VEC>(raw, a, b, out - i * out_step); });
+                 [&](const uint4& raw, int i) { apply8<FP16, SILU, VEC>(raw, a, b, minus_pivot, out - i * out_step); });
 }
 
 // A row in 8 bits, held by a team as NCH chunks of eight channels a thread.
@@ -324,10 +339,12 @@ __device__ __forceinline__ void row_to_int8(const GnParams& p, const Team<TEAM, 
     const int c = c0 + k * TEAM * 8;
     if (c >= p.channels) continue;
     const uint32_t* u = reinterpret_cast<const uint32_t*>(&raw[k]);
+    const uint4 minus_pivot = *reinterpret_cast<const uint4*>(factors + 4 * chunks + (c >> 3));
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float4 av = factors[(i >> 1) * chunks + (c >> 3)], bv = factors[(2 + (i >> 1)) * chunks + (c >> 3)];
-      y[k][i] = fma2(int8_unpack2<FP16>(u[i]), i & 1 ? make_float2(av.z, av.w) : make_float2(av.x, av.y), i & 1 ? make_float2(bv.z, bv.w) : make_float2(bv.x, bv.y));
+      const float2 v = add2(int8_unpack2<FP16>(u[i]), int8_unpack2<FP16>(reinterpret_cast<const uint32_t*>(&minus_pivot)[i]));
+      y[k][i] = fma2(v, i & 1 ? make_float2(av.z, av.w) : make_float2(av.x, av.y), i & 1 ? make_float2(bv.z, bv.w) : make_float2(bv.x, bv.y));
       if constexpr (SILU) y[k][i] = make_float2(silu(y[k][i].x), silu(y[k][i].y));
       top = max_magnitude(max_magnitude(top, y[k][i].x), y[k][i].y);
     }
@@ -384,7 +401,8 @@ __global__ void __launch_bounds__(kGnThreads, 1) group_norm_int8_kernel(const __
 // One launch for what fits the shared memory of a few SMs: a cluster of CTAs takes a slab of channels (whole groups) of an
 // image, each CTA a strip of its rows, which stay in its shared memory between the two passes; the CTAs read each other's
 // statistics there. p.strips: a strip is a CTA; p.slab: channels of a slab. Shared memory: the rows, the sums (then the
-// factors), the strip's statistics, the groups' statistics.
+// factors), the strip's statistics, the groups' statistics, their pivots: `out` may be x, so nothing of x is read when the cluster
+// has met.
 template <bool FP16, bool SILU, bool VEC, bool INT8>
 __global__ void __launch_bounds__(cluster_threads(INT8), INT8 ? 1 : 2) group_norm_cluster_kernel(const __grid_constant__ GnParams p) {
   grid_dependency_release();
@@ -399,8 +417,9 @@ __global__ void __launch_bounds__(cluster_threads(INT8), INT8 ? 1 : 2) group_nor
   const int rank = static_cast<int>(blockIdx.x);
   uint4* held = reinterpret_cast<uint4*>(smem4);  // [tiles * lanes][chunks]
   float4* factors = smem4 + p.strips.tiles_of(0) * lanes * chunks;
-  float2* strip = reinterpret_cast<float2*>(factors + lanes * stats_pitch(p.slab) / 2);
+  float2* strip = reinterpret_cast<float2*>(factors + sums_bytes(lanes, p.slab) / 16);
   float2* stat = strip + groups;
+  uint16_t* pivots = reinterpret_cast<uint16_t*>(stat + groups);
   float weight = 1.f, bias = 0.f;  // on their way while the statistics are made
   if (threadIdx.x < p.slab) {
     weight = gn_weight<FP16>(p, slab0 + threadIdx.x);
@@ -408,7 +427,11 @@ __global__ void __launch_bounds__(cluster_threads(INT8), INT8 ? 1 : 2) group_nor
   }
   strip_stats<kThreads, FP16, VEC>(
       p.x + blockIdx.z * p.x_batch_stride + slab0, p.x_row_stride, p.strips, rank, p.slab, per, reinterpret_cast<float*>(factors),
-      [&](const uint4& raw, int at) { held[(at * lanes + lane) * chunks + chunk] = raw; }, [&](int g, float2 v) { strip[g] = v; });
+      [&](const uint4& raw, int at) { held[(at * lanes + lane) * chunks + chunk] = raw; },
+      [&](int g, float2 v, uint16_t pivot) {
+        strip[g] = v;
+        pivots[g] = pivot;
+      });
   __syncthreads();
   cluster_sync_all();
   join_strips(groups, p.strips, p.rows, per, p.eps, stat, [&](int k, int g) {
@@ -418,9 +441,9 @@ __global__ void __launch_bounds__(cluster_threads(INT8), INT8 ? 1 : 2) group_nor
   });
   __syncthreads();
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // this CTA has read the others' statistics
-  if (threadIdx.x < p.slab) put_factor<FP16>(threadIdx.x, chunks, stat[threadIdx.x / per], weight, bias, factors);
+  if (threadIdx.x < p.slab) put_factor(threadIdx.x, chunks, stat[threadIdx.x / per], weight, bias, pivots[threadIdx.x / per], factors);
   for (int c = threadIdx.x + kThreads; c < p.slab; c += kThreads)
-    put_factor<FP16>(c, chunks, stat[c / per], gn_weight<FP16>(p, slab0 + c), gn_bias<FP16>(p, slab0 + c), factors);
+    put_factor(c, chunks, stat[c / per], gn_weight<FP16>(p, slab0 + c), gn_bias<FP16>(p, slab0 + c), pivots[c / per], factors);
   __syncthreads();
   if constexpr (INT8) {
     const Team<32, kThreads> team{red};
@@ -435,11 +458,12 @@ __global__ void __launch_bounds__(cluster_threads(INT8), INT8 ? 1 : 2) group_nor
     }
   } else if (lane < lanes) {
     float a[8], b[8];
-    read_factors(factors, chunks, chunk, a, b);
+    uint4 minus_pivot;
+    read_factors(factors, chunks, chunk, a, b, minus_pivot);
     const int count = p.strips.rows_of_lane(rank, lane);
     uint16_t* out = p.out + blockIdx.z * p.out_batch_stride + p.strips.first(rank, lane) * p.out_row_stride + slab0 + chunk * 8;
     const long long out_step = p.strips.step() * p.out_row_stride;
-    for (int at = 0; at < count; ++at) apply8<FP16, SILU, VEC>(held[(at * lanes + lane) * chunks + chunk], a, b, out + at * out_step);
+    for (int at = 0; at < count; ++at) apply8<FP16, SILU, VEC>(held[(at * lanes + lane) * chunks + chunk], a, b, minus_pivot, out + at * out_step);
   }
   __syncwarp();
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // the others have read this CTA's
@@ -476,7 +500,7 @@ bool cluster_of(long long batch, long long rows, int channels, int groups, bool 
     const long long clusters = batch * (channels / slab), lanes = cluster_threads(int8) / (slab / 8);
     const long long tiles = ((rows + lanes - 1) / lanes + kClusterCtas - 1) / kClusterCtas;
     if (rows <= lanes * (kClusterCtas - 1)) continue;  // each CTA has rows
-    const long long held = tiles * lanes * slab * 2, smem = held + lanes * stats_pitch(slab) * 8 + slab / per * 16;
+    const long long held = tiles * lanes * slab * 2, smem = held + sums_bytes(static_cast<int>(lanes), slab) + slab / per * 18;
     // So many clusters of this size are on the GPU at a time; a second wave costs more than a second launch. 8-bit rows need all
     // channels of a pixel in one CTA, which leaves few CTAs: with 82 KB each, two images of 32 x 32 x 640 took 15 us, in two
     // launches 9.9; and a warp has a row, so many rows take long however short they are: 384 x 256 7.3 us against 7.6 in two
@@ -504,8 +528,8 @@ int check_gn(const hdit_group_norm_args* a) {
 
 bool off16(const void* p, int64_t a, int64_t b) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0 || a % 8 != 0 || b % 8 != 0; }
 
-// of the two launches' kernels: the sums of 8 channels and 512 lanes, the factors of 4096 channels and as many groups
-constexpr int kGnMaxBytes = 64 * 1024;
+// of the two launches' kernels: the factors of 4096 channels and the statistics of as many groups
+constexpr int kGnMaxBytes = factor_bytes(kMaxChannels) + kMaxChannels * static_cast<int>(sizeof(float2));
 
 template <auto kKernel>
 cudaError_t launch_strips(const GnParams& p, long long batch, size_t smem, cudaStream_t st) {
@@ -537,7 +561,7 @@ GnParams params_of(const hdit_group_norm_args* a, bool out_vec) {
   return p;
 }
 
-size_t factor_bytes(const GnParams& p) { return static_cast<size_t>(p.channels) * 2 * sizeof(float) + static_cast<size_t>(p.groups) * sizeof(float2); }
+size_t apply_bytes(const GnParams& p) { return factor_bytes(p.channels) + static_cast<size_t>(p.groups) * sizeof(float2); }
 
 template <bool FP16, bool VEC>
 cudaError_t launch_stats(const GnParams& p, long long batch, cudaStream_t st) {
@@ -547,13 +571,13 @@ cudaError_t launch_stats(const GnParams& p, long long batch, cudaStream_t st) {
 
 template <bool FP16, bool VEC>
 cudaError_t launch_apply(const GnParams& p, long long batch, cudaStream_t st) {
-  return p.act == HDIT_ACT_SILU ? launch_strips<group_norm_apply_kernel<FP16, true, VEC>>(p, batch, factor_bytes(p), st)
-                                : launch_strips<group_norm_apply_kernel<FP16, false, VEC>>(p, batch, factor_bytes(p), st);
+  return p.act == HDIT_ACT_SILU ? launch_strips<group_norm_apply_kernel<FP16, true, VEC>>(p, batch, apply_bytes(p), st)
+                                : launch_strips<group_norm_apply_kernel<FP16, false, VEC>>(p, batch, apply_bytes(p), st);
 }
 
 template <bool FP16, bool SILU, bool VEC>
 cudaError_t launch_int8_act(const GnParams& p, long long batch, cudaStream_t st) {
-  const size_t smem = factor_bytes(p);
+  const size_t smem = apply_bytes(p);
   if (p.channels <= 64) return launch_strips<group_norm_int8_kernel<FP16, SILU, 8, 1, 4, VEC>>(p, batch, smem, st);
   if (p.channels <= 128) return launch_strips<group_norm_int8_kernel<FP16, SILU, 16, 1, 4, VEC>>(p, batch, smem, st);
   if (p.channels <= 256) return launch_strips<group_norm_int8_kernel<FP16, SILU, 32, 1, 4, VEC>>(p, batch, smem, st);
@@ -596,6 +620,7 @@ int run_group_norm(const hdit_group_norm_args* a, bool int8) {
   }
   if (a->scratch == nullptr || (reinterpret_cast<uintptr_t>(a->scratch) & 7) != 0) return set_error(HDIT_ERR_BAD_ARG, "scratch is null or not 8-byte aligned");
   p.strips = make_strips(a->rows, strips_of(a->batch, a->rows, p.channels), kGnThreads / (p.channels / 8));
+  p.pivots = reinterpret_cast<uint16_t*>(p.partial + a->batch * p.strips.strips * a->groups);
   HDIT_CUDA_OK((HDIT_GN_OF(launch_stats, fp16, p.vec)(p, a->batch, st)));
   if (int8) HDIT_CUDA_OK((HDIT_GN_OF(launch_int8, fp16, p.vec)(p, a->batch, st)));
   else HDIT_CUDA_OK((HDIT_GN_OF(launch_apply, fp16, p.vec)(p, a->batch, st)));
@@ -611,7 +636,7 @@ extern "C" int64_t hdit_group_norm_scratch(int64_t batch, int64_t rows, int64_t 
   if (batch <= 0 || rows <= 0 || rows > 0x7fffffffLL || channels <= 0 || groups <= 0 || channels % 8 != 0 || channels > kMaxChannels || channels % groups != 0)
     return 0;
   if (cluster_of(batch, rows, static_cast<int>(channels), static_cast<int>(groups), int8_rows != 0, &c)) return 0;
-  return batch * strips_of(batch, rows, static_cast<int>(channels)) * groups * static_cast<int64_t>(sizeof(float2));
+  return batch * groups * (strips_of(batch, rows, static_cast<int>(channels)) * static_cast<int64_t>(sizeof(float2)) + 2);
 }
 
 extern "C" int hdit_group_norm(const hdit_group_norm_args* a) {

@@ -755,3 +755,34 @@ def test_a_smaller_call_leaves_a_kernel_what_a_larger_one_takes(name):
     small()
     for k in kernels:
         assert k.attribute(MOST_DYNAMIC_SHARED) >= k.shared_bytes
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("value", [3.0, 50.0, -500.0, 5000.0])
+@pytest.mark.parametrize("shape", [(2, 50, 64), (1, 3000, 64), (40, 700, 64), (1, 40000, 16)])
+def test_group_norm_of_flat_groups(shape, value, dtype):
+    """Groups whose variance is nothing, or little beside eps: a step of x counts 1 / sqrt(eps), and so does an error of the
+    mean. All but one group are constant; that one differs in one place by the type's step.
+
+    The bound is _gn64()'s without a term of the mean's size: x - pivot is rounded (u of it, below |z| + D deviations), a has three
+    roundings and multiplies x - pivot and mean - pivot alike, b is rounded (u of D w and |b|), the result as well."""
+    from hetu_dit_b200 import kernels
+    B, S, C = shape
+    gen, u = _gen(S), 2.0 ** -24
+    x = torch.full(shape, value, device=DEV, dtype=dtype)
+    x[B - 1, S // 2, C - 3] += torch.finfo(dtype).eps * 2 ** math.floor(math.log2(abs(value)))
+    w, b = _randn(gen, C, dtype=dtype), _randn(gen, C, dtype=dtype)
+    X = x.double().view(B, S, 8, C // 8)
+    z = (X - X.mean((1, 3), keepdim=True)) / torch.sqrt(X.var((1, 3), correction=0, keepdim=True) + 1e-6)
+    D = (z.abs().amax((1, 3), keepdim=True) + 1).expand(X.shape).reshape(shape)
+    z, w64, b64 = z.reshape(shape), w.double(), b.double()
+    want = z * w64 + b64
+    off = w64.abs() * 320 * u * (D + z.abs() * D ** 2) + 3 * u * (2 * w64.abs() * (z.abs() + D) + want.abs() + b64.abs())
+    got = kernels.group_norm(x, 8, w, b)
+    _within(got, want, off * (1 + torch.finfo(dtype).eps) + _half_step(want, dtype))
+    inplace = x.clone()
+    assert torch.equal(kernels.group_norm(inplace, 8, w, b, out=inplace), got)
+    got8 = kernels.group_norm_int8(x, 8, w, b)
+    s = got8.scale.double()
+    _within(s, want.abs().amax(-1) / 127, off.amax(-1) / 127 + 2.0 ** -23 * s)
+    _within(got8.q.double() * s[..., None], want, off + s[..., None] * (0.5 + 127 * 2.0 ** -22))
