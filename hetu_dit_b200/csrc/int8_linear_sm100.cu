@@ -210,7 +210,9 @@ __device__ __forceinline__ void int8_tile_coords(const Int8Params& p, int tile, 
   m_t = m0 + (r - n_t * rows);
 }
 
-template <int BN, bool PAIR, bool FP16, int EPI>
+// PLAIN_RESIDUAL: no bulk copy can move the residual. A kernel of its own: its pieces in registers cost the other one, at 256 columns
+// with 96 registers a thread, 76 bytes of spills.
+template <int BN, bool PAIR, bool FP16, int EPI, bool PLAIN_RESIDUAL>
 __global__ void __launch_bounds__(Int8Cfg<BN, PAIR, EPI>::kThreads, 1) int8_linear_kernel(const __grid_constant__ Int8Params p) {
   using C = Int8Cfg<BN, PAIR, EPI>;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -363,6 +365,7 @@ __global__ void __launch_bounds__(Int8Cfg<BN, PAIR, EPI>::kThreads, 1) int8_line
   } else {
     // ------------------------------------------------------------------ epilogue
     constexpr bool kGated = EPI == HDIT_GEMM_BIAS_GATE_RESIDUAL;
+    constexpr bool kTmaResidual = kGated && !PLAIN_RESIDUAL;
     const int quarter = warp & 3;  // the TMEM lanes this warp may read: [32 * quarter, 32 * quarter + 32)
     const int team = (warp - 2) >> 2;
     uint8_t* const staging = staging_base + (warp - 2) * (C::kBufs * kPieceBytes);
@@ -415,8 +418,7 @@ __global__ void __launch_bounds__(Int8Cfg<BN, PAIR, EPI>::kThreads, 1) int8_line
     bool ok = true;
     if (unit < total_tiles) {
       fetch(unit);
-      if constexpr (kGated)
-        if (p.tma_residual) issue_residual(row0, tile_col, 0);
+      if constexpr (kTmaResidual) issue_residual(row0, tile_col, 0);
     }
     for (int tile = unit; tile < total_tiles; tile += n_units, ++local) {
       const uint32_t acc = local & 1, use = local >> 1;
@@ -433,24 +435,22 @@ __global__ void __launch_bounds__(Int8Cfg<BN, PAIR, EPI>::kThreads, 1) int8_line
       team_sync();
       if (!ok) continue;  // after a failure: the team's other warps still meet the barriers
       if (tile + n_units < total_tiles) fetch(tile + n_units);
-      if constexpr (kGated) {
-        if (!p.tma_residual) {
-          // both pieces, into buffers that the tile before has left, while its sums are on their way
-          static_assert(C::kTeamPieces == 2 && C::kBufs == 2, "a buffer for each piece of a tile");
-          RaggedPiece v[2];
-          auto piece_at = [&](int c, auto f) {
-            if (my_row0 < p.M && my_col + c * 32 < p.N)
-              f(p.residual + my_row0 * p.ldr + my_col + c * 32, min(32, p.M - my_row0), min(32, p.N - my_col - c * 32));
-          };
+      if constexpr (PLAIN_RESIDUAL) {
+        // both pieces, into buffers that the tile before has left, while its sums are on their way
+        static_assert(C::kTeamPieces == 2 && C::kBufs == 2, "a buffer for each piece of a tile");
+        RaggedPiece v[2];
+        auto piece_at = [&](int c, auto f) {
+          if (my_row0 < p.M && my_col + c * 32 < p.N)
+            f(p.residual + my_row0 * p.ldr + my_col + c * 32, min(32, p.M - my_row0), min(32, p.N - my_col - c * 32));
+        };
 #pragma unroll
-          for (int c = 0; c < 2; ++c) piece_at(c, [&](const uint16_t* g, int rows, int cols) { ragged_load(v[c], g, p.ldr, rows, cols, lane); });
-          if (lane == 0) tma_store_wait_read<0>();
-          __syncwarp();
+        for (int c = 0; c < 2; ++c) piece_at(c, [&](const uint16_t* g, int rows, int cols) { ragged_load(v[c], g, p.ldr, rows, cols, lane); });
+        if (lane == 0) tma_store_wait_read<0>();
+        __syncwarp();
 #pragma unroll
-          for (int c = 0; c < 2; ++c)
-            piece_at(c, [&](const uint16_t* g, int rows, int cols) { ragged_stage(v[c], staging + c * kPieceBytes, g, p.ldr, rows, cols, lane); });
-          __syncwarp();
-        }
+        for (int c = 0; c < 2; ++c)
+          piece_at(c, [&](const uint16_t* g, int rows, int cols) { ragged_stage(v[c], staging + c * kPieceBytes, g, p.ldr, rows, cols, lane); });
+        __syncwarp();
       }
       if (!__all_sync(0xffffffffu, mbar_wait_bounded(&acc_full[acc], use & 1, abort_flag, kSpinLimit))) {
         if (lane == 0) report_failure(p.status, abort_flag, HDIT_ERR_PEER_TIMEOUT, Q_EPI_ACC_FULL, static_cast<int>(local));
@@ -467,25 +467,23 @@ __global__ void __launch_bounds__(Int8Cfg<BN, PAIR, EPI>::kThreads, 1) int8_line
         const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + acc * C::kAccCols + team * C::kTeamCols + at;
         uint32_t r[32];
         tmem_ld32(taddr, r);
-        if constexpr (kGated) {
-          if (p.tma_residual) {
-            // the next piece's residual, into the buffer that the previous piece's result has left
-            fence_proxy_async_smem();  // where it left by plain loads
-            if (lane == 0) tma_store_wait_read<0>();
-            __syncwarp();
-            if (c + 1 < C::kTeamPieces) issue_residual(my_row0, col0 + 32, buf ^ 1);
-            else if (tile + n_units < total_tiles) issue_residual(row0, tile_col, buf ^ 1);
-            if (in) {
-              if (!__all_sync(0xffffffffu, mbar_wait_bounded(&res_full[buf], (res_phase >> buf) & 1, abort_flag, kSpinLimit))) {
-                if (lane == 0) report_failure(p.status, abort_flag, HDIT_ERR_PEER_TIMEOUT, Q_EPI_RESIDUAL, static_cast<int>(piece));
-                ok = false;
-                break;
-              }
-              res_phase ^= 1u << buf;
-              res_pending &= ~(1u << buf);
+        if constexpr (kTmaResidual) {
+          // the next piece's residual, into the buffer that the previous piece's result has left
+          fence_proxy_async_smem();  // where it left by plain loads
+          if (lane == 0) tma_store_wait_read<0>();
+          __syncwarp();
+          if (c + 1 < C::kTeamPieces) issue_residual(my_row0, col0 + 32, buf ^ 1);
+          else if (tile + n_units < total_tiles) issue_residual(row0, tile_col, buf ^ 1);
+          if (in) {
+            if (!__all_sync(0xffffffffu, mbar_wait_bounded(&res_full[buf], (res_phase >> buf) & 1, abort_flag, kSpinLimit))) {
+              if (lane == 0) report_failure(p.status, abort_flag, HDIT_ERR_PEER_TIMEOUT, Q_EPI_RESIDUAL, static_cast<int>(piece));
+              ok = false;
+              break;
             }
+            res_phase ^= 1u << buf;
+            res_pending &= ~(1u << buf);
           }
-        } else {
+        } else if constexpr (!kGated) {
           if (lane == 0) tma_store_wait_read<C::kBufs - 1>();  // the buffer's last result has left
           __syncwarp();
         }
@@ -569,7 +567,7 @@ __global__ void __launch_bounds__(Int8Cfg<BN, PAIR, EPI>::kThreads, 1) int8_line
     }
     // copies in flight must have left or landed before the CTA's shared memory is given back
     if (lane == 0) tma_store_wait_all();
-    if constexpr (kGated) {
+    if constexpr (kTmaResidual) {
       volatile int never = 0;
       for (uint32_t buf = 0; buf < 2; ++buf)
         if ((res_pending >> buf) & 1) mbar_wait_bounded(&res_full[buf], (res_phase >> buf) & 1, &never, kSpinLimit);
@@ -619,17 +617,11 @@ int encode_pieces(CUtensorMap* map, const void* ptr, long long rows, long long n
   return HDIT_OK;
 }
 
-template <int BN, bool PAIR, bool FP16, int EPI>
+template <int BN, bool PAIR, bool FP16, int EPI, bool PLAIN_RESIDUAL = false>
 int launch_int8(Int8Params& p, const hdit_int8_linear_args* a) {
   using C = Int8Cfg<BN, PAIR, EPI>;
-  auto kernel = int8_linear_kernel<BN, PAIR, FP16, EPI>;
-  static thread_local int last_dev = -1;  // the attribute is per device
-  int dev = 0;
-  HDIT_CUDA_OK(cudaGetDevice(&dev));
-  if (dev != last_dev) {
-    HDIT_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes));
-    last_dev = dev;
-  }
+  constexpr auto kernel = int8_linear_kernel<BN, PAIR, FP16, EPI, PLAIN_RESIDUAL>;
+  HDIT_CUDA_OK((allow_shared_memory<kernel, C::kSmemBytes>()));
   // Boxes of rows that lie outside cost more than rows: 16 x 6144 -> 9216 took 22.9 us with boxes of 128 rows, 15.0 with 16; 128 rows take 15.8.
   const int a_rows = a->m < 128 ? static_cast<int>((a->m + 7) / 8 * 8) : 128;
   p.a_bytes = static_cast<uint32_t>(a_rows * kTileKBytes);
@@ -662,7 +654,9 @@ int launch_int8_of(Int8Params& p, const hdit_int8_linear_args* a) {
   switch (a->epilogue) {
     case HDIT_GEMM_BIAS: return fp16 ? launch_int8<BN, PAIR, true, 0>(p, a) : launch_int8<BN, PAIR, false, 0>(p, a);
     case HDIT_GEMM_BIAS_GELU_TANH: return fp16 ? launch_int8<BN, PAIR, true, 1>(p, a) : launch_int8<BN, PAIR, false, 1>(p, a);
-    default: return fp16 ? launch_int8<BN, PAIR, true, 2>(p, a) : launch_int8<BN, PAIR, false, 2>(p, a);
+    default:
+      if (!p.tma_residual) return fp16 ? launch_int8<BN, PAIR, true, 2, true>(p, a) : launch_int8<BN, PAIR, false, 2, true>(p, a);
+      return fp16 ? launch_int8<BN, PAIR, true, 2>(p, a) : launch_int8<BN, PAIR, false, 2>(p, a);
   }
 }
 

@@ -786,3 +786,17 @@ def test_group_norm_of_flat_groups(shape, value, dtype):
     s = got8.scale.double()
     _within(s, want.abs().amax(-1) / 127, off.amax(-1) / 127 + 2.0 ** -23 * s)
     _within(got8.q.double() * s[..., None], want, off + s[..., None] * (0.5 + 127 * 2.0 ** -22))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("epilogue", ["bias", "gelu_tanh", "gate_residual"])
+@pytest.mark.parametrize("tile", [1, 2, 3, 4])
+def test_aligned_products_keep_their_values_in_registers(tile, epilogue, dtype):
+    """A few bytes of local memory for what a failed wait reports, no spilled values beside them."""
+    from hetu_dit_b200 import kernels
+    from tests.captured_kernels import LOCAL_BYTES, captured_kernels
+    x, w, b, res, gate = _layer(1, 300, 512, 264, dtype, 4)
+    x8 = kernels.quantize_rows(x)
+    rest = (res, gate) if epilogue == "gate_residual" else (None, None)
+    (kernel,) = captured_kernels(lambda: kernels.linear_int8(x8, w, b, epilogue, *rest, tile=tile))
+    assert kernel.attribute(LOCAL_BYTES) <= 16
