@@ -54,17 +54,21 @@ struct GnParams {
   long long rows, x_batch_stride, x_row_stride, out_batch_stride, out_row_stride;  // q: out_row_stride only, rows of all images
   Strips strips;
   int channels, groups, act, slab;
-  float eps;
+  float eps, inv_per;  // 1 / channels of a group
   bool vec;
 };
 
+// Group of a channel (below 4096: the product is off by less than the half that is added). Integer divisions one after the other
+// between two barriers cost more than the sums there.
+__device__ __forceinline__ int group_of(int channel, float inv_per) { return static_cast<int>((static_cast<float>(channel) + 0.5f) * inv_per); }
+
 // Calls f(group, sub, n_sub) in groups of n_sub consecutive threads of a warp, the same number of times in all threads.
-template <typename F>
+template <int THREADS, typename F>
 __device__ __forceinline__ void for_groups(int groups, F f) {
-  int n_sub = 32;
-  while (n_sub > 1 && groups * n_sub > static_cast<int>(blockDim.x)) n_sub >>= 1;
-  const int at_once = static_cast<int>(blockDim.x) / n_sub;
-  for (int g0 = 0; g0 < groups; g0 += at_once) f(g0 + static_cast<int>(threadIdx.x) / n_sub, static_cast<int>(threadIdx.x) % n_sub, n_sub);
+  int shift = 5;
+  while (shift > 0 && groups << shift > THREADS) --shift;
+  const int sub = static_cast<int>(threadIdx.x) & ((1 << shift) - 1);
+  for (int g0 = 0; g0 < groups; g0 += THREADS >> shift) f(g0 + (static_cast<int>(threadIdx.x) >> shift), sub, 1 << shift);
 }
 __device__ __forceinline__ float sub_sum(float v, int n_sub) {
   for (int o = n_sub >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -72,9 +76,9 @@ __device__ __forceinline__ float sub_sum(float v, int n_sub) {
 }
 
 // Walks `count` rows of a thread, `step` elements apart: use(values of the row's eight channels, index). Groups of kAhead rows
-// are on their way while the group before is used.
-template <bool VEC, typename F>
-__device__ __forceinline__ void walk_rows(const uint16_t* x, int c, int channels, int count, long long step, F use) {
+// are on their way while the group before is used; meanwhile() is called when the first ones are.
+template <bool VEC, typename M, typename F>
+__device__ __forceinline__ void walk_rows(const uint16_t* x, int c, int channels, int count, long long step, M meanwhile, F use) {
   uint4 next[kAhead];
   const int full = count / kAhead;
   auto fetch = [&](int n) {
@@ -84,6 +88,7 @@ __device__ __forceinline__ void walk_rows(const uint16_t* x, int c, int channels
     x += kAhead * step;
   };
   fetch(full > 0 ? kAhead : count);
+  meanwhile();
   int at = 0;
   for (int f = 0; f < full; ++f) {
     uint4 raw[kAhead];
@@ -104,42 +109,46 @@ __device__ __forceinline__ void walk_rows(const uint16_t* x, int c, int channels
 __host__ __device__ constexpr int stats_pitch(int channels) { return channels + 4; }
 // of the cluster's sums; the factors take their place
 __host__ __device__ constexpr int sums_bytes(int lanes, int channels) {
-  return lanes * stats_pitch(channels) * 8 > channels * 10 ? lanes * stats_pitch(channels) * 8 : channels * 10;
+  return lanes * stats_pitch(channels) * 8 > channels * 12 ? lanes * stats_pitch(channels) * 8 : channels * 12;
 }
 
 // Statistics of strip k of an image of `rows` rows of `channels` channels at `x`. A thread passes its eight channels of every lanes-th
-// row to keep(raw, index). smem: [lanes][stats_pitch(channels)] sums, then the same of squares. put(group, {mean from the pivot, sum of
-// squared distances from the mean}, the pivot's bits).
+// row to keep(raw, index). smem: [lanes][stats_pitch(channels)] sums, then the same of squares. row0: the image's first row, which has
+// the groups' pivots, is left there. put(group, {mean from the pivot, sum of squared distances from the mean}).
 template <int THREADS, bool FP16, bool VEC, typename K, typename P>
-__device__ __forceinline__ void strip_stats(const uint16_t* x, long long row_stride, const Strips& strips, int strip, int channels, int per, float* smem, K keep,
-                                            P put) {
+__device__ __forceinline__ void strip_stats(const uint16_t* x, long long row_stride, const Strips& strips, int strip, int channels, int per, float inv_per, float* smem,
+                                            uint16_t* row0, K keep, P put) {
   const int chunks = channels / 8;
   const int lanes = strips.lanes, pitch = stats_pitch(channels);  // rows at a time
   const int lane = threadIdx.x / chunks, c = (threadIdx.x - lane * chunks) * 8;
   const uint16_t* xs = x + static_cast<long long>(strip) * lanes * row_stride;  // the strip's first row
   if (lane < lanes) {
-    float s[8], ss[8], pivot[8];
+    float s[8], ss[8], first_row[8];
+    uint4 image_row;
     const uint4 first = int8_load8(xs, c, channels, VEC);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float2 v = int8_unpack2<FP16>(reinterpret_cast<const uint32_t*>(&first)[i]);
-      pivot[2 * i] = v.x;
-      pivot[2 * i + 1] = v.y;
+      first_row[2 * i] = v.x;
+      first_row[2 * i + 1] = v.y;
       s[2 * i] = s[2 * i + 1] = ss[2 * i] = ss[2 * i + 1] = 0.f;
     }
-    walk_rows<VEC>(x + strips.first(strip, lane) * row_stride, c, channels, strips.rows_of_lane(strip, lane), strips.step() * row_stride, [&](const uint4& raw, int at) {
+    walk_rows<VEC>(x + strips.first(strip, lane) * row_stride, c, channels, strips.rows_of_lane(strip, lane), strips.step() * row_stride, [&] {
+      if (lane == 0) image_row = int8_load8(x, c, channels, VEC);
+    }, [&](const uint4& raw, int at) {
       keep(raw, at);
       const uint32_t* u = reinterpret_cast<const uint32_t*>(&raw);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float2 v = int8_unpack2<FP16>(u[i]);
-        const float d0 = v.x - pivot[2 * i], d1 = v.y - pivot[2 * i + 1];
+        const float d0 = v.x - first_row[2 * i], d1 = v.y - first_row[2 * i + 1];
         s[2 * i] += d0;
         ss[2 * i] = fmaf(d0, d0, ss[2 * i]);
         s[2 * i + 1] += d1;
         ss[2 * i + 1] = fmaf(d1, d1, ss[2 * i + 1]);
       }
     });
+    if (lane == 0) *reinterpret_cast<uint4*>(row0 + c) = image_row;
     float4* to = reinterpret_cast<float4*>(smem + lane * pitch + c);
     to[0] = make_float4(s[0], s[1], s[2], s[3]);
     to[1] = make_float4(s[4], s[5], s[6], s[7]);
@@ -148,13 +157,14 @@ __device__ __forceinline__ void strip_stats(const uint16_t* x, long long row_str
     to[1] = make_float4(ss[4], ss[5], ss[6], ss[7]);
   }
   __syncthreads();
-  // Over the lanes: `parts` neighbouring lanes of a warp to a channel. Then per channel, in the first lane's places: the mean,
-  // and the sum of squared distances from it.
-  int parts = 1;
-  while (parts < 32 && parts < lanes && parts * 2 * channels <= THREADS) parts *= 2;
+  // Over the lanes: `parts` neighbouring lanes of a warp to a channel. Then per channel, in the first lane's places: the mean from the
+  // group's pivot, and the sum of squared distances from the mean.
+  int shift = 0;
+  while (shift < 5 && 1 << shift < lanes && 2 * channels << shift <= THREADS) ++shift;
+  const int parts = 1 << shift, part = static_cast<int>(threadIdx.x) & (parts - 1);
   const float n = static_cast<float>(strips.rows_of(strip)), inv_rows = 1.f / n;
-  for (int ch0 = 0; ch0 < channels; ch0 += THREADS / parts) {
-    const int ch = ch0 + static_cast<int>(threadIdx.x) / parts, part = static_cast<int>(threadIdx.x) % parts;
+  for (int ch0 = 0; ch0 < channels; ch0 += THREADS >> shift) {
+    const int ch = ch0 + (static_cast<int>(threadIdx.x) >> shift);
     float a = 0.f, q = 0.f;
     if (ch < channels)
       for (int l = part; l < lanes; l += parts) {
@@ -165,13 +175,12 @@ __device__ __forceinline__ void strip_stats(const uint16_t* x, long long row_str
     q = sub_sum(q, parts);
     if (ch < channels && part == 0) {  // no other thread reads this channel's first lane
       const float m2 = q - a * a * inv_rows;
-      smem[ch] = (int8_unpack2<FP16>(xs[ch]).x - int8_unpack2<FP16>(x[ch / per * per]).x) + a * inv_rows;
+      smem[ch] = (int8_unpack2<FP16>(xs[ch]).x - int8_unpack2<FP16>(row0[group_of(ch, inv_per) * per]).x) + a * inv_rows;
       smem[lanes * pitch + ch] = m2 > 0.f ? m2 : m2 - m2;  // keeps NaN
     }
   }
   __syncthreads();
-  const float inv_per = 1.f / static_cast<float>(per);
-  for_groups(channels / per, [&](int g, int sub, int n_sub) {
+  for_groups<THREADS>(channels / per, [&](int g, int sub, int n_sub) {
     const bool live = g * per < channels;
     float mean = 0.f, m2 = 0.f;
     for (int k = sub; live && k < per; k += n_sub) mean += smem[g * per + k];
@@ -181,7 +190,7 @@ __device__ __forceinline__ void strip_stats(const uint16_t* x, long long row_str
       m2 += smem[lanes * pitch + g * per + k] + n * d * d;
     }
     m2 = sub_sum(m2, n_sub);
-    if (live && sub == 0) put(g, make_float2(mean, m2), x[g * per]);
+    if (live && sub == 0) put(g, make_float2(mean, m2));
   });
 }
 
@@ -189,21 +198,23 @@ template <bool FP16, bool VEC>
 __global__ void __launch_bounds__(kGnThreads, 1) group_norm_stats_kernel(const __grid_constant__ GnParams p) {
   grid_dependency_release();
   grid_dependency_wait();
-  extern __shared__ float smem[];
+  extern __shared__ __align__(16) float smem[];
+  const int per = p.channels / p.groups;
+  uint16_t* row0 = reinterpret_cast<uint16_t*>(smem + p.strips.lanes * stats_pitch(p.channels) * 2);
   float2* out = p.partial + (static_cast<long long>(blockIdx.y) * p.strips.strips + blockIdx.x) * p.groups;
-  strip_stats<kGnThreads, FP16, VEC>(p.x + blockIdx.y * p.x_batch_stride, p.x_row_stride, p.strips, static_cast<int>(blockIdx.x), p.channels,
-                                     p.channels / p.groups, smem, [](const uint4&, int) {}, [&](int g, float2 v, uint16_t pivot) {
+  strip_stats<kGnThreads, FP16, VEC>(p.x + blockIdx.y * p.x_batch_stride, p.x_row_stride, p.strips, static_cast<int>(blockIdx.x), p.channels, per, p.inv_per, smem,
+                                     row0, [](const uint4&, int) {}, [&](int g, float2 v) {
                                        out[g] = v;
-                                       if (blockIdx.x == 0) p.pivots[static_cast<long long>(blockIdx.y) * p.groups + g] = pivot;
+                                       if (blockIdx.x == 0) p.pivots[static_cast<long long>(blockIdx.y) * p.groups + g] = row0[g * per];
                                      });
 }
 
 // {mean from the pivot, 1 / deviation} of `groups` groups from `strips` strips of an image, `per` channels to a group, into
 // stat[groups]. in(strip, group): the strip's {mean from the pivot, sum of squared distances from the mean}.
-template <typename F>
+template <int THREADS, typename F>
 __device__ __forceinline__ void join_strips(int groups, const Strips& strips, long long rows, int per, float eps, float2* stat, F in) {
   const float inv_total = 1.f / (static_cast<float>(rows) * static_cast<float>(per));
-  for_groups(groups, [&](int g, int sub, int n_sub) {
+  for_groups<THREADS>(groups, [&](int g, int sub, int n_sub) {
     const bool live = g < groups;
     const float base = live ? in(0, g).x : 0.f;
     float a = 0.f, q = 0.f;
@@ -222,19 +233,21 @@ __device__ __forceinline__ void join_strips(int groups, const Strips& strips, lo
   });
 }
 
-// y = (x - pivot) * a + b with a = weight / deviation and b = bias - (mean - pivot) * a, for each channel in shared memory: `factors`
-// holds a, then b, each first for the lower four channels of every chunk of eight, then for the upper four, so that threads' 16
-// bytes lie side by side, then -pivot as 16-bit values. No term has the size of the mean: in the form x * a + (bias - mean * a), half
-// a unit of 2^-24 of mean * a was off, which at a constant image of 500 with an eps of 1e-6 is 0.03. The pivot is one of the group's
-// n values, no more than sqrt(n) deviations from the mean.
-__device__ __forceinline__ void put_factor(int c, int chunks, float2 stat, float weight, float bias, uint16_t pivot, float4* factors) {
+// y = (x * a + b) + rest with a = weight / deviation and b + rest = bias - mean * a, for each channel in shared memory: `factors` holds
+// a, b, rest, each first for the lower four channels of every chunk of eight, then for the upper four, so that threads' 16 bytes
+// lie side by side. b alone would be off by half a unit of 2^-24 of mean * a, which at a constant image of 500 with an eps of 1e-6 is
+// 0.03; `rest` is what its roundings lose (of the product by an FMA, of the sum by Knuth's two-sum). stat: {mean - pivot, 1 / deviation}.
+__device__ __forceinline__ void put_factor(int c, int chunks, float2 stat, float weight, float bias, float pivot, float4* factors) {
   const float a = stat.y * weight;
+  const float near = fmaf(-stat.x, a, bias), far = __fmul_rn(pivot, a);
+  const float b = __fsub_rn(near, far), taken = __fsub_rn(b, near);
+  const float rest = __fsub_rn(__fsub_rn(__fsub_rn(near, __fsub_rn(b, taken)), __fadd_rn(far, taken)), fmaf(pivot, a, -far));
   float* to = reinterpret_cast<float*>(factors) + (c >> 3) * 4 + ((c >> 2) & 1) * chunks * 4 + (c & 3);
   to[0] = a;
-  to[8 * chunks] = fmaf(-stat.x, a, bias);
-  reinterpret_cast<uint16_t*>(factors + 4 * chunks)[c] = pivot ^ 0x8000u;
+  to[8 * chunks] = b;
+  to[16 * chunks] = isinf(b) ? 0.f : rest;  // a bias without a number: the difference of two of it would be none
 }
-__host__ __device__ constexpr int factor_bytes(int channels) { return channels * 10; }
+__host__ __device__ constexpr int factor_bytes(int channels) { return channels * 12; }
 template <bool FP16>
 __device__ __forceinline__ float gn_weight(const GnParams& p, int c) { return p.weight != nullptr ? int8_unpack2<FP16>(p.weight[c]).x : 1.f; }
 template <bool FP16>
@@ -248,15 +261,20 @@ __device__ __forceinline__ void group_norm_factors(const GnParams& p, float4* fa
   const uint16_t* pivots = p.pivots + static_cast<long long>(blockIdx.y) * p.groups;
   const float2* in = p.partial + static_cast<long long>(blockIdx.y) * p.strips.strips * p.groups;
   float weight = 1.f, bias = 0.f;  // on their way while the strips are joined
+  float pivot = 0.f;
+  const int own = group_of(threadIdx.x, p.inv_per);
   if (threadIdx.x < p.channels) {
     weight = gn_weight<FP16>(p, threadIdx.x);
     bias = gn_bias<FP16>(p, threadIdx.x);
+    pivot = int8_unpack2<FP16>(pivots[own]).x;
   }
-  join_strips(p.groups, p.strips, p.rows, per, p.eps, stat, [&](int k, int g) { return in[static_cast<long long>(k) * p.groups + g]; });
+  join_strips<kGnThreads>(p.groups, p.strips, p.rows, per, p.eps, stat, [&](int k, int g) { return in[static_cast<long long>(k) * p.groups + g]; });
   __syncthreads();
-  if (threadIdx.x < p.channels) put_factor(threadIdx.x, p.channels / 8, stat[threadIdx.x / per], weight, bias, pivots[threadIdx.x / per], factors);
-  for (int c = threadIdx.x + kGnThreads; c < p.channels; c += kGnThreads)
-    put_factor(c, p.channels / 8, stat[c / per], gn_weight<FP16>(p, c), gn_bias<FP16>(p, c), pivots[c / per], factors);
+  if (threadIdx.x < p.channels) put_factor(threadIdx.x, p.channels / 8, stat[own], weight, bias, pivot, factors);
+  for (int c = threadIdx.x + kGnThreads; c < p.channels; c += kGnThreads) {
+    const int g = group_of(c, p.inv_per);
+    put_factor(c, p.channels / 8, stat[g], gn_weight<FP16>(p, c), gn_bias<FP16>(p, c), int8_unpack2<FP16>(pivots[g]).x, factors);
+  }
   __syncthreads();
 }
 
@@ -280,13 +298,13 @@ __device__ __forceinline__ uint32_t gn_pack(float lo, float hi) {
 
 // Eight channels of a row, normalised, to dst.
 template <bool FP16, bool SILU, bool VEC>
-__device__ __forceinline__ void apply8(const uint4& raw, const float (&a)[8], const float (&b)[8], const uint4& minus_pivot, uint16_t* dst) {
+__device__ __forceinline__ void apply8(const uint4& raw, const float (&a)[8], const float (&b)[8], const float (&rest)[8], uint16_t* dst) {
   uint4 y = raw;
   uint32_t* u = reinterpret_cast<uint32_t*>(&y);
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    const float2 v = add2(int8_unpack2<FP16>(u[k]), int8_unpack2<FP16>(reinterpret_cast<const uint32_t*>(&minus_pivot)[k]));
-    float y0 = fmaf(v.x, a[2 * k], b[2 * k]), y1 = fmaf(v.y, a[2 * k + 1], b[2 * k + 1]);
+    const float2 v = int8_unpack2<FP16>(u[k]);
+    float y0 = fmaf(v.x, a[2 * k], b[2 * k]) + rest[2 * k], y1 = fmaf(v.y, a[2 * k + 1], b[2 * k + 1]) + rest[2 * k + 1];
     if constexpr (SILU) y0 = silu(y0), y1 = silu(y1);
     u[k] = gn_pack<FP16>(y0, y1);
   }
@@ -297,12 +315,12 @@ __device__ __forceinline__ void apply8(const uint4& raw, const float (&a)[8], co
     for (int k = 0; k < 8; ++k) dst[k] = static_cast<uint16_t>(u[k / 2] >> (16 * (k & 1)));
   }
 }
-__device__ __forceinline__ void read_factors(const float4* factors, int chunks, int chunk, float (&a)[8], float (&b)[8], uint4& minus_pivot) {
-  minus_pivot = *reinterpret_cast<const uint4*>(factors + 4 * chunks + chunk);
+__device__ __forceinline__ void read_factors(const float4* factors, int chunks, int chunk, float (&a)[8], float (&b)[8], float (&rest)[8]) {
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     *reinterpret_cast<float4*>(a + 4 * h) = factors[h * chunks + chunk];
     *reinterpret_cast<float4*>(b + 4 * h) = factors[(2 + h) * chunks + chunk];
+    *reinterpret_cast<float4*>(rest + 4 * h) = factors[(4 + h) * chunks + chunk];
   }
 }
 
@@ -316,15 +334,14 @@ __global__ void __launch_bounds__(kGnThreads, 1) group_norm_apply_kernel(const _
   const int lane = threadIdx.x / chunks, chunk = threadIdx.x - lane * chunks, c = chunk * 8;
   group_norm_factors<FP16>(p, factors);
   if (lane >= lanes) return;
-  float a[8], b[8];
-  uint4 minus_pivot;
-  read_factors(factors, chunks, chunk, a, b, minus_pivot);
+  float a[8], b[8], rest[8];
+  read_factors(factors, chunks, chunk, a, b, rest);
   // the strip's rows from the last to the first
   const int strip = static_cast<int>(blockIdx.x), count = p.strips.rows_of_lane(strip, lane);
   const long long step = p.strips.step(), last = p.strips.first(strip, lane) + (count - 1) * step, out_step = step * p.out_row_stride;
   uint16_t* out = p.out + blockIdx.y * p.out_batch_stride + last * p.out_row_stride + c;
-  walk_rows<VEC>(p.x + blockIdx.y * p.x_batch_stride + last * p.x_row_stride, c, p.channels, count, -step * p.x_row_stride,
-                 [&](const uint4& raw, int i) { apply8<FP16, SILU, VEC>(raw, a, b, minus_pivot, out - i * out_step); });
+  walk_rows<VEC>(p.x + blockIdx.y * p.x_batch_stride + last * p.x_row_stride, c, p.channels, count, -step * p.x_row_stride, [] {},
+                 [&](const uint4& raw, int i) { apply8<FP16, SILU, VEC>(raw, a, b, rest, out - i * out_step); });
 }
 
 // A row in 8 bits, held by a team as NCH chunks of eight channels a thread.
@@ -339,12 +356,12 @@ __device__ __forceinline__ void row_to_int8(const GnParams& p, const Team<TEAM, 
     const int c = c0 + k * TEAM * 8;
     if (c >= p.channels) continue;
     const uint32_t* u = reinterpret_cast<const uint32_t*>(&raw[k]);
-    const uint4 minus_pivot = *reinterpret_cast<const uint4*>(factors + 4 * chunks + (c >> 3));
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float4 av = factors[(i >> 1) * chunks + (c >> 3)], bv = factors[(2 + (i >> 1)) * chunks + (c >> 3)];
-      const float2 v = add2(int8_unpack2<FP16>(u[i]), int8_unpack2<FP16>(reinterpret_cast<const uint32_t*>(&minus_pivot)[i]));
-      y[k][i] = fma2(v, i & 1 ? make_float2(av.z, av.w) : make_float2(av.x, av.y), i & 1 ? make_float2(bv.z, bv.w) : make_float2(bv.x, bv.y));
+      const int at = (i >> 1) * chunks + (c >> 3);
+      const float4 av = factors[at], bv = factors[2 * chunks + at], rv = factors[4 * chunks + at];
+      const float2 v = fma2(int8_unpack2<FP16>(u[i]), i & 1 ? make_float2(av.z, av.w) : make_float2(av.x, av.y), i & 1 ? make_float2(bv.z, bv.w) : make_float2(bv.x, bv.y));
+      y[k][i] = add2(v, i & 1 ? make_float2(rv.z, rv.w) : make_float2(rv.x, rv.y));
       if constexpr (SILU) y[k][i] = make_float2(silu(y[k][i].x), silu(y[k][i].y));
       top = max_magnitude(max_magnitude(top, y[k][i].x), y[k][i].y);
     }
@@ -401,8 +418,8 @@ __global__ void __launch_bounds__(kGnThreads, 1) group_norm_int8_kernel(const __
 // One launch for what fits the shared memory of a few SMs: a cluster of CTAs takes a slab of channels (whole groups) of an
 // image, each CTA a strip of its rows, which stay in its shared memory between the two passes; the CTAs read each other's
 // statistics there. p.strips: a strip is a CTA; p.slab: channels of a slab. Shared memory: the rows, the sums (then the
-// factors), the strip's statistics, the groups' statistics, their pivots: `out` may be x, so nothing of x is read when the cluster
-// has met.
+// factors), the strip's statistics, the groups' statistics. The image's first row, with the pivots, stays in between: `out` may be
+// x, so nothing of x is read when the cluster has met.
 template <bool FP16, bool SILU, bool VEC, bool INT8>
 __global__ void __launch_bounds__(cluster_threads(INT8), INT8 ? 1 : 2) group_norm_cluster_kernel(const __grid_constant__ GnParams p) {
   grid_dependency_release();
@@ -417,33 +434,33 @@ __global__ void __launch_bounds__(cluster_threads(INT8), INT8 ? 1 : 2) group_nor
   const int rank = static_cast<int>(blockIdx.x);
   uint4* held = reinterpret_cast<uint4*>(smem4);  // [tiles * lanes][chunks]
   float4* factors = smem4 + p.strips.tiles_of(0) * lanes * chunks;
-  float2* strip = reinterpret_cast<float2*>(factors + sums_bytes(lanes, p.slab) / 16);
+  uint16_t* row0 = reinterpret_cast<uint16_t*>(factors + sums_bytes(lanes, p.slab) / 16);
+  float2* strip = reinterpret_cast<float2*>(row0 + p.slab);
   float2* stat = strip + groups;
-  uint16_t* pivots = reinterpret_cast<uint16_t*>(stat + groups);
   float weight = 1.f, bias = 0.f;  // on their way while the statistics are made
   if (threadIdx.x < p.slab) {
     weight = gn_weight<FP16>(p, slab0 + threadIdx.x);
     bias = gn_bias<FP16>(p, slab0 + threadIdx.x);
   }
   strip_stats<kThreads, FP16, VEC>(
-      p.x + blockIdx.z * p.x_batch_stride + slab0, p.x_row_stride, p.strips, rank, p.slab, per, reinterpret_cast<float*>(factors),
+      p.x + blockIdx.z * p.x_batch_stride + slab0, p.x_row_stride, p.strips, rank, p.slab, per, p.inv_per, reinterpret_cast<float*>(factors), row0,
       [&](const uint4& raw, int at) { held[(at * lanes + lane) * chunks + chunk] = raw; },
-      [&](int g, float2 v, uint16_t pivot) {
-        strip[g] = v;
-        pivots[g] = pivot;
-      });
+      [&](int g, float2 v) { strip[g] = v; });
   __syncthreads();
   cluster_sync_all();
-  join_strips(groups, p.strips, p.rows, per, p.eps, stat, [&](int k, int g) {
+  join_strips<kThreads>(groups, p.strips, p.rows, per, p.eps, stat, [&](int k, int g) {
     float2 v;
     asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(map_to_cta(strip + g, static_cast<uint32_t>(k))) : "memory");
     return v;
   });
   __syncthreads();
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // this CTA has read the others' statistics
-  if (threadIdx.x < p.slab) put_factor(threadIdx.x, chunks, stat[threadIdx.x / per], weight, bias, pivots[threadIdx.x / per], factors);
-  for (int c = threadIdx.x + kThreads; c < p.slab; c += kThreads)
-    put_factor(c, chunks, stat[c / per], gn_weight<FP16>(p, slab0 + c), gn_bias<FP16>(p, slab0 + c), pivots[c / per], factors);
+  auto put = [&](int c, float w, float b) {
+    const int g = group_of(c, p.inv_per);
+    put_factor(c, chunks, stat[g], w, b, int8_unpack2<FP16>(row0[g * per]).x, factors);
+  };
+  if (threadIdx.x < p.slab) put(threadIdx.x, weight, bias);
+  for (int c = threadIdx.x + kThreads; c < p.slab; c += kThreads) put(c, gn_weight<FP16>(p, slab0 + c), gn_bias<FP16>(p, slab0 + c));
   __syncthreads();
   if constexpr (INT8) {
     const Team<32, kThreads> team{red};
@@ -457,13 +474,12 @@ __global__ void __launch_bounds__(cluster_threads(INT8), INT8 ? 1 : 2) group_nor
       row_to_int8<FP16, SILU, 32, 4, kThreads>(p, team, 0, raw, factors, c0, blockIdx.z * p.rows + row, true);
     }
   } else if (lane < lanes) {
-    float a[8], b[8];
-    uint4 minus_pivot;
-    read_factors(factors, chunks, chunk, a, b, minus_pivot);
+    float a[8], b[8], rest[8];
+    read_factors(factors, chunks, chunk, a, b, rest);
     const int count = p.strips.rows_of_lane(rank, lane);
     uint16_t* out = p.out + blockIdx.z * p.out_batch_stride + p.strips.first(rank, lane) * p.out_row_stride + slab0 + chunk * 8;
     const long long out_step = p.strips.step() * p.out_row_stride;
-    for (int at = 0; at < count; ++at) apply8<FP16, SILU, VEC>(held[(at * lanes + lane) * chunks + chunk], a, b, minus_pivot, out + at * out_step);
+    for (int at = 0; at < count; ++at) apply8<FP16, SILU, VEC>(held[(at * lanes + lane) * chunks + chunk], a, b, rest, out + at * out_step);
   }
   __syncwarp();
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // the others have read this CTA's
@@ -500,7 +516,7 @@ bool cluster_of(long long batch, long long rows, int channels, int groups, bool 
     const long long clusters = batch * (channels / slab), lanes = cluster_threads(int8) / (slab / 8);
     const long long tiles = ((rows + lanes - 1) / lanes + kClusterCtas - 1) / kClusterCtas;
     if (rows <= lanes * (kClusterCtas - 1)) continue;  // each CTA has rows
-    const long long held = tiles * lanes * slab * 2, smem = held + sums_bytes(static_cast<int>(lanes), slab) + slab / per * 18;
+    const long long held = tiles * lanes * slab * 2, smem = held + sums_bytes(static_cast<int>(lanes), slab) + slab * 2 + slab / per * 16;
     // So many clusters of this size are on the GPU at a time; a second wave costs more than a second launch. 8-bit rows need all
     // channels of a pixel in one CTA, which leaves few CTAs: with 82 KB each, two images of 32 x 32 x 640 took 15 us, in two
     // launches 9.9; and a warp has a row, so many rows take long however short they are: 384 x 256 7.3 us against 7.6 in two
@@ -557,6 +573,7 @@ GnParams params_of(const hdit_group_norm_args* a, bool out_vec) {
   p.groups = static_cast<int>(a->groups);
   p.act = a->act;
   p.eps = a->eps;
+  p.inv_per = static_cast<float>(a->groups) / static_cast<float>(a->channels);
   p.vec = out_vec && !off16(a->x, a->x_batch_stride, a->x_row_stride);
   return p;
 }
@@ -565,7 +582,7 @@ size_t apply_bytes(const GnParams& p) { return factor_bytes(p.channels) + static
 
 template <bool FP16, bool VEC>
 cudaError_t launch_stats(const GnParams& p, long long batch, cudaStream_t st) {
-  const size_t smem = static_cast<size_t>(kGnThreads / (p.channels / 8)) * stats_pitch(p.channels) * 2 * sizeof(float);
+  const size_t smem = static_cast<size_t>(kGnThreads / (p.channels / 8)) * stats_pitch(p.channels) * 2 * sizeof(float) + p.channels * sizeof(uint16_t);
   return launch_strips<group_norm_stats_kernel<FP16, VEC>>(p, batch, smem, st);
 }
 
