@@ -10,9 +10,10 @@
 //
 // us, this kernel | 128 x 128 tiles, 8-bit rows: 9216 x 1536, 1 row 4.4 | 7.8, 8 rows 6.2 | 7.6, 16 rows 9.1 | 7.6 (as two column
 // tiles); 18432 x 3072, 1 row 12.4 | 16.2, 8 rows 16.1 | 16.0: taken for up to eight rows. 16-bit rows are brought into 8 bits by every
-// CTA for itself where there are one or two, or at most 8192 elements: a launch less, 3 us on the host. us on the device, so |
-// after quantize_rows: 9216 x 1536, 2 rows 5.9 | 6.2, 4 rows 7.5 | 6.9, 8 rows 9.3 | 8.0; 2048 x 2048, 4 rows 5.5 | 6.3, 8 rows
-// 7.4 | 7.0; 500 x 200, 8 rows 3.2 | 4.2; 1536 x 6144, 2 rows 7.6 | 8.0, 6 rows 16.6 | 11.2.
+// CTA for itself where there are one or two, or where the first pass over a row is one turn of its warps and no SM has two CTAs
+// that do it: a launch less, 3 us on the host. us in a graph, so | after quantize_rows: 9216 x 1536, 2 rows 5.4 | 5.6; 2048 x 2048, 4
+// rows 5.5 | 6.3; 1024 x 1024, 8 rows 4.4 | 5.3; 2368 x 512, 8 rows 3.6 | 4.5; 256 x 768, 8 rows 4.5 | 4.6. Not: 9216 x 1536, 4 rows
+// 6.7 | 6.3; 9216 x 768, 8 rows 6.9 | 5.7; 6144 x 256, 8 rows 4.8 | 4.2 (many CTAs); 512 x 1536, 5 rows 5.3 | 4.9 (two turns).
 #include "gemm_common.cuh"
 #include "host_common.h"
 #include "int8_linear.h"
@@ -202,7 +203,7 @@ bool int8_linear_few_takes(const hdit_int8_linear_args* a) {
 bool int8_linear_few_pays(const hdit_int8_linear_args* a) { return a->m <= 2 || a->m * few_pitch(a->k) <= 44 * 1024; }
 // Not where the result may take x's place (x = residual = out): a CTA would write what another one has yet to read.
 bool int8_linear_few_quantizes(const hdit_int8_linear_args* a) {
-  if (a->m > 2 && a->m * a->k > 8192) return false;
+  if (a->m > 2 && (a->k > (a->m > 4 ? 1024 : 2048) || a->n > 16 * 148)) return false;  // 1024 elements: four loads of a warp's lanes
   const int64_t per = a->x_rows_per_batch < a->m ? a->x_rows_per_batch : a->m, entries = (a->m + per - 1) / per;
   const uintptr_t x0 = reinterpret_cast<uintptr_t>(a->x), x1 = x0 + 2 * ((entries - 1) * a->x_batch_stride + (per - 1) * a->x_row_stride + a->k);
   const uintptr_t o0 = reinterpret_cast<uintptr_t>(a->out), o1 = o0 + 2 * ((a->m - 1) * a->ldo + a->n);

@@ -1046,6 +1046,12 @@ def ln_modulate_int8(x, shift, scale, eps=1e-6):
     return out
 
 
+def _overlap(a, b):
+    """Whether the memory between two tensors' first and last elements has a part in common."""
+    (a0, a1), (b0, b1) = ((t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))) for t in (a, b))
+    return a0 < b1 and b0 < a1
+
+
 _TAILS = {"bias": _C.GEMM_BIAS, "gelu_tanh": _C.GEMM_BIAS_GELU_TANH, "gate_residual": _C.GEMM_BIAS_GATE_RESIDUAL}
 
 
@@ -1138,9 +1144,10 @@ def linear_int8(x, weight, bias=None, epilogue="bias", residual=None, gate=None,
         a.a, a.a_scale, a.lda = xr.data_ptr(), scale.data_ptr(), ss if m > 1 else pitch
     else:
         a.x, a.lda, a.x_rows_per_batch, a.x_batch_stride, a.x_row_stride = xr.data_ptr(), pitch, S, sb, ss
-        one = own and tile in (0, 5) and (m <= 2 and k <= 65536 or m <= 8 and m * k <= 8192)  # the kernel for a few rows does it all
+        # the kernel for a few rows does it all (int8_linear_few_quantizes() in csrc/int8_linear_few.cu)
+        one = tile in (0, 5) and (own or not _overlap(x, out)) and (m <= 2 or m <= 8 and k <= (1024 if m > 4 else 2048) and n <= 2368)
         launches = 1 if one else 2
-        if not one or m > 2:  # the rows in 8 bits, their scales behind them: scratch of the call
+        if not (one and own and m <= 2 and k <= 65536):  # the rows in 8 bits, their scales behind them: scratch of the call
             scratch = torch.empty(m * (pitch + 4), dtype=torch.int8, device=dev)
             a.a = a.a_scale = scratch.data_ptr()
             a.a_scale += m * pitch

@@ -800,3 +800,23 @@ def test_aligned_products_keep_their_values_in_registers(tile, epilogue, dtype):
     rest = (res, gate) if epilogue == "gate_residual" else (None, None)
     (kernel,) = captured_kernels(lambda: kernels.linear_int8(x8, w, b, epilogue, *rest, tile=tile))
     assert kernel.attribute(LOCAL_BYTES) <= 16
+
+
+@pytest.mark.parametrize("m,k,n,held,placed,count", [
+    (1, 1536, 9216, False, False, 1), (2, 1536, 9216, False, True, 1), (2, 70000, 32, False, False, 1), (4, 2048, 2048, False, False, 1),
+    (8, 1024, 2368, False, True, 1), (4, 1536, 9216, False, False, 2), (8, 768, 9216, False, False, 2), (5, 1536, 512, False, False, 2),
+    (8, 256, 2369, False, False, 2), (9, 64, 64, False, False, 2), (8, 512, 512, True, False, 1), (300, 512, 512, False, True, 2)])
+def test_launches_of_a_few_rows(m, k, n, held, placed, count):
+    """In a graph a launch more costs less than rows brought into 8 bits by several CTAs of an SM, or in several turns. What is
+    counted is what is launched."""
+    from hetu_dit_b200 import kernels
+    from tests.captured_kernels import captured_kernels
+    gen = _gen(m)
+    x, w = _randn(gen, 1, m, k, dtype=torch.bfloat16), kernels.quantize_rows(_randn(gen, n, k, dtype=torch.bfloat16))
+    x = kernels.quantize_rows(x) if held else x
+    out = torch.empty(1, m, n, dtype=torch.bfloat16, device=DEV) if placed else None
+    call = lambda: kernels.linear_int8(x, w, out=out)  # noqa: E731
+    assert len(captured_kernels(call)) == count
+    before = kernels.launch_count()
+    call()
+    assert kernels.launch_count() - before == count
