@@ -86,13 +86,17 @@ def _qkv(attn, streams, rope):
             return outs
     outs = []
     for x, projs, (wq, wk), ranges in streams:
-        if read_rows(projs) and torch.is_tensor(x):
-            x = kernels.quantize_rows(x)  # once for all three
+        x = _rows_once(x, projs)
         q, k, v = (_heads(p(x), attn) for p in projs)
         for lo, hi, rotate, row0, seq_start in ranges:
             _norm_rope(attn, q[:, lo:hi], k[:, lo:hi], wq, wk, rope if rotate else None, row0, seq_start)
         outs.append([q, k, v])
     return outs
+
+
+def _rows_once(x, projs):
+    """x as 8-bit rows where all its readers are 8-bit layers: made once for all three, not by each."""
+    return kernels.quantize_rows(x) if torch.is_tensor(x) and read_rows(projs) else x
 
 
 def _prologue_range(lo, hi, wq, wk, rope, row0):
@@ -165,8 +169,10 @@ class JointAttnProcessor:
         B, S_img, _ = hidden_states.shape
         S_txt = encoder_hidden_states.shape[1]
         t0, i0 = (0, S_txt) if attn.text_first else (S_img, 0)
+        img_projs, txt_projs = (attn.to_q, attn.to_k, attn.to_v), (attn.add_q_proj, attn.add_k_proj, attn.add_v_proj)
+        hidden_states, encoder_hidden_states = _rows_once(hidden_states, img_projs), _rows_once(encoder_hidden_states, txt_projs)
         bufs = []
-        for img_p, txt_p in ((attn.to_q, attn.add_q_proj), (attn.to_k, attn.add_k_proj), (attn.to_v, attn.add_v_proj)):
+        for img_p, txt_p in zip(img_projs, txt_projs):
             buf = torch.empty((B, S_txt + S_img, attn.heads * attn.head_dim), dtype=hidden_states.dtype,
                               device=hidden_states.device)
             _project_into(buf, i0, hidden_states, img_p)
@@ -255,7 +261,9 @@ class SingleAttnProcessor:
         rope_txt = rope if attn.rope_on_text else None
         sp = ps.get_sequence_parallel_world_size()
         if text_offset is not None and sp > 1:
-            q, k, v = (_heads(p(hidden_states), attn) for p in (attn.to_q, attn.to_k, attn.to_v))
+            projs = (attn.to_q, attn.to_k, attn.to_v)
+            hidden_states = _rows_once(hidden_states, projs)
+            q, k, v = (_heads(p(hidden_states), attn) for p in projs)
             text_rows = int(text_total) if attn.rope_on_text else 0
             ranges = [_prologue_range(t_lo, t_hi, attn.norm_q, attn.norm_k, rope_txt, text_offset),
                       _prologue_range(i_lo, i_hi, attn.norm_q, attn.norm_k, rope, text_rows + token_offset)]

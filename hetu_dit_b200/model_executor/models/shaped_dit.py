@@ -243,9 +243,9 @@ class _Branch:
 
 
 def _sees_rows(attn, processor, projections, *others):
-    """Whether a wrapped attention layer on one GPU may be given its input as Int8Rows: its projections (by name) and whatever
-    else reads the input are 8-bit layers, and nothing else sees it."""
-    if ps.get_sequence_parallel_world_size() != 1 or not kernels.is_plain(attn, _Wrapped):
+    """Whether a wrapped attention layer may be given its input as Int8Rows: its projections (by name) and whatever else reads
+    the input are 8-bit layers, and nothing else sees it."""
+    if not kernels.is_plain(attn, _Wrapped):
         return False
     inner = attn.module
     return kernels.is_plain(inner, Attention) and type(inner.processor) is processor and \

@@ -276,3 +276,63 @@ def test_rows_wider_than_they_have_to_be_are_addressed_by_their_stride(lib, monk
     (name, args), = lib.calls
     a = args[0]._obj
     assert (name, a.m, a.lda, a.a) == ("hdit_int8_linear", B * S, 64, x.q.data_ptr())
+
+
+def _tiny_attention(joint, monkeypatch):
+    from hetu_dit_b200.core.distributed import parallel_state as ps
+    from hetu_dit_b200.model_executor.layers import int8_linear
+    from hetu_dit_b200.model_executor.models import shaped_dit
+    from tests.test_gpu_model import tiny_shape
+    shape, _ = tiny_shape("flux")
+    attn = shaped_dit.Attention(shape, joint=joint, out_proj=joint)
+    made, products = [], []
+
+    def quantize_rows(x):
+        made.append(x)
+        return rows8(*x.shape)
+
+    def linear_int8(x, weight, bias=None, epilogue="bias", residual=None, gate=None, out=None):
+        products.append(x)
+        return torch.zeros(*x.shape[:-1], weight.shape[0], dtype=x.dtype) if out is None else out
+
+    monkeypatch.setattr(kernels, "quantize_rows", quantize_rows)
+    monkeypatch.setattr(kernels, "linear_int8", linear_int8)
+    monkeypatch.setattr(ps, "get_sequence_parallel_world_size", lambda: 2)
+    monkeypatch.setattr(attn.processor._ops, "get", lambda cls: lambda key, q, k, v, **kw: q)
+    int8_linear.quantize_linears_(attn)
+    made.clear()
+    return shape, attn, made, products
+
+
+@pytest.mark.parametrize("rows_given", [False, True])
+def test_sharded_streams_are_quantised_once_for_their_projections(monkeypatch, rows_given):
+    """Under sequence parallelism the projections write into the shards' buffers one by one: all of a stream read one set of rows."""
+    shape, attn, made, products = _tiny_attention(True, monkeypatch)
+    make = rows8 if rows_given else lambda *s: torch.zeros(*s).bfloat16()
+    img, txt = make(1, 12, shape.hidden), make(1, 4, shape.hidden)
+    with torch.no_grad():
+        attn(img, txt, text_len=8, token_offset=12, text_offset=4)
+    assert made[:2] == [] if rows_given else made[0] is img and made[1] is txt
+    assert len(made) == (0 if rows_given else 2) and len(products) == 8
+    assert [type(x) for x in products] == [kernels.Int8Rows] * 6 + [torch.Tensor] * 2  # the projections, then the outputs' 16-bit input
+    assert len({id(x) for x in products[:6]}) == 2
+
+
+@pytest.mark.parametrize("rows_given", [False, True])
+def test_a_sharded_single_stream_is_quantised_once_for_its_projections(monkeypatch, rows_given):
+    shape, attn, made, products = _tiny_attention(False, monkeypatch)
+    x = (rows8 if rows_given else lambda *s: torch.zeros(*s).bfloat16())(1, 16, shape.hidden)
+    with torch.no_grad():
+        attn(x, text_len=4, token_offset=12, text_offset=4, text_total=8)
+    assert len(made) == (0 if rows_given else 1) and len(products) == 3 and len({id(p) for p in products}) == 1
+    assert type(products[0]) is kernels.Int8Rows
+
+
+def test_norms_write_rows_under_sequence_parallelism_too(monkeypatch):
+    from hetu_dit_b200.core.distributed import parallel_state as ps
+    from hetu_dit_b200.model_executor.layers.attention_processor import SingleAttnProcessor
+    from hetu_dit_b200.model_executor.models import shaped_dit
+    shape, attn, _, _ = _tiny_attention(False, monkeypatch)
+    assert ps.get_sequence_parallel_world_size() == 2
+    assert shaped_dit._sees_rows(shaped_dit._Wrapped(attn), SingleAttnProcessor, ("to_q", "to_k", "to_v"))
+    assert not shaped_dit._sees_rows(shaped_dit._Wrapped(attn), SingleAttnProcessor, ("to_q", "to_k", "to_v"), torch.nn.Linear(2, 2))
