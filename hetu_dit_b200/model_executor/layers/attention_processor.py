@@ -22,7 +22,7 @@ from ...core.distributed import parallel_state as ps
 from ...core.parallel import (hetuDiTFluxLongContextAttention, hetuDiTJointLongContextAttention,
                               hetuDiTLongContextAttention)
 from ...core.resource_manager.cache_manager import get_cache_manager
-from .int8_linear import Int8Linear, read_rows
+from .int8_linear import Int8Linear, read_rows, refuse_gradients
 
 
 def _heads(x, attn):
@@ -96,7 +96,10 @@ def _qkv(attn, streams, rope):
 
 def _rows_once(x, projs):
     """x as 8-bit rows where all its readers are 8-bit layers: made once for all three, not by each."""
-    return kernels.quantize_rows(x) if torch.is_tensor(x) and read_rows(projs) else x
+    if not torch.is_tensor(x) or not read_rows(projs):
+        return x
+    refuse_gradients(x)
+    return kernels.quantize_rows(x)
 
 
 def _prologue_range(lo, hi, wq, wk, rope, row0):
@@ -112,7 +115,7 @@ def _project_into(buf, row0, x, linear):
     """buf[:, row0:row0 + S] = linear(x) without a temporary when the rows are one contiguous block."""
     B, S, _ = x.shape
     if kernels.is_plain(linear, Int8Linear):
-        kernels.linear_int8(x, linear.rows, linear.bias, out=buf[:, row0:row0 + S])
+        linear.with_tail(x, "bias", out=buf[:, row0:row0 + S])
     elif B == 1 and not torch.is_grad_enabled() and not isinstance(linear, Int8Linear):
         torch.addmm(linear.bias, x[0], linear.weight.t(), out=buf[0, row0:row0 + S])
     else:

@@ -14,8 +14,15 @@ from ... import kernels
 from ...core.distributed import parallel_state as ps
 
 
+def refuse_gradients(*tensors):
+    """Raises where a gradient is recorded for one of the tensors (None and Int8Rows among them): the result would have none."""
+    if torch.is_grad_enabled() and any(getattr(t, "requires_grad", False) for t in tensors):
+        raise RuntimeError("8-bit linear layers have no gradients: run them under torch.no_grad() or on tensors that require none")
+
+
 class Int8Linear(nn.Module):
-    """x @ weight.T + bias with the weight in 8 bits, in place of a torch.nn.Linear. x: a 16-bit tensor, or kernels.Int8Rows."""
+    """x @ weight.T + bias with the weight in 8 bits, in place of a torch.nn.Linear. x: a 16-bit tensor that no gradient is
+    recorded for, or kernels.Int8Rows."""
 
     def __init__(self, weight: kernels.Int8Rows, bias=None):
         super().__init__()
@@ -47,10 +54,12 @@ class Int8Linear(nn.Module):
         return self
 
     def forward(self, x):
+        refuse_gradients(x)
         return kernels.linear_int8(x, self.rows, self.bias)
 
     def with_tail(self, x, epilogue, residual=None, gate=None, out=None):
-        """kernels.linear_tail() of this layer in one launch (two with 16-bit x)."""
+        """kernels.linear_tail() of this layer, or the layer alone ("bias"), in one launch (two with 16-bit x)."""
+        refuse_gradients(x, residual, gate)
         return kernels.linear_int8(x, self.rows, self.bias, epilogue, residual=residual, gate=gate, out=out)
 
     def extra_repr(self):

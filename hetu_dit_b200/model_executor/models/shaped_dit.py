@@ -469,11 +469,12 @@ class ShapedDiT(nn.Module):
 
     def quantize_linears_(self):
         """Brings the weights of the blocks' linear layers, adaLN among them, into 8 bits (layers.int8_linear): 16-bit model on
-        the GPU, inference only. The embedders and the output layer stay as they are. Not for a model whose blocks a block cache
-        moves between plans, which addresses torch.nn.Linear weights."""
+        the GPU, inference only: no parameter of the model asks for a gradient from then on. The embedders and the output layer
+        stay as they are. Not for a model whose blocks a block cache moves between plans, which addresses torch.nn.Linear
+        weights."""
         for blk in list(self.transformer_blocks) + list(self.single_transformer_blocks):
             quantize_linears_(blk)
-        return self
+        return self.requires_grad_(False)
 
     def register_cache(self):
         """One stale-KV entry per attention layer: the plain cache when the plan has no sequence

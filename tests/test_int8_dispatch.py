@@ -336,3 +336,39 @@ def test_norms_write_rows_under_sequence_parallelism_too(monkeypatch):
     assert ps.get_sequence_parallel_world_size() == 2
     assert shaped_dit._sees_rows(shaped_dit._Wrapped(attn), SingleAttnProcessor, ("to_q", "to_k", "to_v"))
     assert not shaped_dit._sees_rows(shaped_dit._Wrapped(attn), SingleAttnProcessor, ("to_q", "to_k", "to_v"), torch.nn.Linear(2, 2))
+
+
+def test_an_8_bit_layer_refuses_a_gradient(monkeypatch):
+    from hetu_dit_b200.model_executor.layers.attention_processor import _project_into
+    from hetu_dit_b200.model_executor.layers.int8_linear import Int8Linear
+    layer = Int8Linear(rows8(24, 40), torch.zeros(24).bfloat16())
+    monkeypatch.setattr(kernels, "linear_int8", lambda x, w, b=None, epilogue="bias", residual=None, gate=None, out=None: gpu_like(*x.shape[:-1], 24))
+    x, res, gate = gpu_like(1, 5, 40), gpu_like(1, 5, 24), gpu_like(1, 24)
+    grad = [t.detach().clone().requires_grad_() for t in (x, res, gate)]
+    calls = (lambda: layer(grad[0]), lambda: kernels.linear_tail(layer, grad[0], "gelu_tanh"),
+             lambda: kernels.linear_tail(layer, x, "gate_residual", residual=grad[1], gate=gate),
+             lambda: kernels.linear_tail(layer, x, "gate_residual", residual=res, gate=grad[2]),
+             lambda: _project_into(torch.zeros(1, 9, 24).bfloat16(), 0, grad[0], layer))
+    for call in calls:
+        with pytest.raises(RuntimeError, match="no gradients"):
+            call()
+    with torch.no_grad():
+        for call in calls:
+            call()
+    layer(x), layer(rows8(1, 5, 40)), kernels.linear_tail(layer, x, "gate_residual", residual=res, gate=gate)
+
+
+def test_rows_of_an_input_that_asks_for_a_gradient_are_refused(monkeypatch):
+    shape, attn, made, _ = _tiny_attention(False, monkeypatch)
+    x = torch.zeros(1, 16, shape.hidden).bfloat16().requires_grad_()
+    with pytest.raises(RuntimeError, match="no gradients"):
+        attn(x, text_len=4, token_offset=12, text_offset=4, text_total=8)
+
+
+def test_a_model_in_8_bits_asks_for_no_gradients(monkeypatch):
+    from hetu_dit_b200.model_executor.models.shaped_dit import ShapedDiT
+    from tests.test_gpu_model import tiny_shape
+    monkeypatch.setattr(kernels, "quantize_rows", lambda w: rows8(*w.shape))
+    model = ShapedDiT(tiny_shape("sd3")[0])
+    assert any(p.requires_grad for p in model.parameters())
+    assert model.quantize_linears_() is model and not any(p.requires_grad for p in model.parameters())
