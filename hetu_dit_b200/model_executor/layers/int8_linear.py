@@ -75,24 +75,24 @@ def read_rows(linears):
     return True
 
 
-def _replace_linears(module):
-    """How many layers below `module` were replaced."""
-    replaced = 0
-    for name, child in module.named_children():
-        if type(child) is nn.Linear:
-            setattr(module, name, Int8Linear.from_linear(child))
-            replaced += 1
-        else:
-            replaced += _replace_linears(child)
-    return replaced
+def _places(module):
+    """(parent, name) of every torch.nn.Linear below `module`."""
+    return [(parent, name) for parent in module.modules() for name, child in parent._modules.items() if type(child) is nn.Linear]
 
 
 @torch.no_grad()
 def quantize_linears_(module: nn.Module):
     """Puts an Int8Linear in the place of every torch.nn.Linear below `module` (16-bit, on the GPU); returns module. What has
-    another class (an adapter) stays. Steps captured in CUDA graphs before hold the addresses of the 16-bit weights: those of
-    every StepGraphCache are dropped. Block caches address torch.nn.Linear weights by name: a module whose slices migrate
-    between plans keeps them."""
-    if _replace_linears(module) and ps.model_parallel_is_initialized():
-        ps.get_parallel_groups().void_captured_graphs()
+    another class (an adapter) stays. A layer that cannot be brought into 8 bits (another type, another device) raises before any
+    is replaced. Steps captured in CUDA graphs before hold the addresses of the 16-bit weights: those of every StepGraphCache are
+    dropped. Block caches address torch.nn.Linear weights by name: a module whose slices migrate between plans keeps them."""
+    places = _places(module)
+    for parent, name in places:
+        kernels.quantize_rows(parent._modules[name].weight.detach()[:0])  # all that it asks of a weight, and nothing launched
+    try:
+        for parent, name in places:  # one by one: its 16-bit weight goes before the next one's 8-bit copy comes
+            setattr(parent, name, Int8Linear.from_linear(parent._modules[name]))
+    finally:
+        if places and ps.model_parallel_is_initialized():
+            ps.get_parallel_groups().void_captured_graphs()
     return module

@@ -372,3 +372,22 @@ def test_a_model_in_8_bits_asks_for_no_gradients(monkeypatch):
     model = ShapedDiT(tiny_shape("sd3")[0])
     assert any(p.requires_grad for p in model.parameters())
     assert model.quantize_linears_() is model and not any(p.requires_grad for p in model.parameters())
+
+
+def test_a_layer_that_cannot_be_in_8_bits_leaves_the_module_as_it_was(lib, monkeypatch):  # noqa: F811
+    """The first layers could be converted; the last one has another type, or lies on the host."""
+    from hetu_dit_b200.model_executor.layers.int8_linear import quantize_linears_
+    monkeypatch.setattr(kernels, "_cuda_index", lambda device: 0)
+
+    def linear(dtype, on_gpu):
+        layer = torch.nn.Linear(16, 8, dtype=dtype)
+        weight = layer.weight.detach()
+        layer.weight = torch.nn.Parameter(weight.as_subclass(OnGpu) if on_gpu else weight)
+        return layer
+
+    for last in (linear(torch.float32, True), linear(torch.bfloat16, False)):
+        net = torch.nn.ModuleList([linear(torch.bfloat16, True), torch.nn.ModuleList([linear(torch.bfloat16, True)]), last])
+        with pytest.raises((TypeError, RuntimeError)):
+            quantize_linears_(net)
+        assert sum(type(m) is torch.nn.Linear for m in net.modules()) == 3
+    assert lib.calls == []
