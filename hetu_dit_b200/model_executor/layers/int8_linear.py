@@ -75,15 +75,23 @@ def read_rows(linears):
     return True
 
 
+def _replaceable(layer):
+    """Whether a layer is a torch.nn.Linear that nothing was put on: a hook, a forward() or a weight of a class of its own would go
+    with the layer."""
+    own = layer.__dict__
+    return type(layer) is nn.Linear and type(layer.weight) is nn.Parameter and "forward" not in own and \
+        not (own["_forward_hooks"] or own["_forward_pre_hooks"] or own["_backward_hooks"] or own["_backward_pre_hooks"])
+
+
 def _places(module):
-    """(parent, name) of every torch.nn.Linear below `module`."""
-    return [(parent, name) for parent in module.modules() for name, child in parent._modules.items() if type(child) is nn.Linear]
+    """(parent, name) of every layer below `module` that is to be replaced."""
+    return [(parent, name) for parent in module.modules() for name, child in parent._modules.items() if child is not None and _replaceable(child)]
 
 
 @torch.no_grad()
 def quantize_linears_(module: nn.Module):
     """Puts an Int8Linear in the place of every torch.nn.Linear below `module` (16-bit, on the GPU); returns module. What has
-    another class (an adapter) stays. A layer that cannot be brought into 8 bits (another type, another device) raises before any
+    another class (an adapter), and a layer with a hook, a forward() or a weight of a class of its own, stays. A layer that cannot be brought into 8 bits (another type, another device) raises before any
     is replaced. Steps captured in CUDA graphs before hold the addresses of the 16-bit weights: those of every StepGraphCache are
     dropped. Block caches address torch.nn.Linear weights by name: a module whose slices migrate between plans keeps them."""
     places = _places(module)

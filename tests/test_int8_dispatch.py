@@ -378,16 +378,39 @@ def test_a_layer_that_cannot_be_in_8_bits_leaves_the_module_as_it_was(lib, monke
     """The first layers could be converted; the last one has another type, or lies on the host."""
     from hetu_dit_b200.model_executor.layers.int8_linear import quantize_linears_
     monkeypatch.setattr(kernels, "_cuda_index", lambda device: 0)
+    on_host = torch.nn.Linear(24, 8, dtype=torch.bfloat16)
 
-    def linear(dtype, on_gpu):
-        layer = torch.nn.Linear(16, 8, dtype=dtype)
-        weight = layer.weight.detach()
-        layer.weight = torch.nn.Parameter(weight.as_subclass(OnGpu) if on_gpu else weight)
-        return layer
+    def require_cuda(*tensors):
+        if any(t.shape == on_host.weight.shape or t.shape == (0, 24) for t in tensors):
+            raise RuntimeError("no CPU path")
 
-    for last in (linear(torch.float32, True), linear(torch.bfloat16, False)):
-        net = torch.nn.ModuleList([linear(torch.bfloat16, True), torch.nn.ModuleList([linear(torch.bfloat16, True)]), last])
+    monkeypatch.setattr(kernels, "_require_cuda", require_cuda)
+    for last in (torch.nn.Linear(16, 8), on_host):
+        net = torch.nn.ModuleList([torch.nn.Linear(16, 8, dtype=torch.bfloat16),
+                                   torch.nn.ModuleList([torch.nn.Linear(16, 8, dtype=torch.bfloat16)]), last])
         with pytest.raises((TypeError, RuntimeError)):
             quantize_linears_(net)
         assert sum(type(m) is torch.nn.Linear for m in net.modules()) == 3
     assert lib.calls == []
+
+
+def test_a_layer_that_something_was_put_on_stays(monkeypatch):
+    from hetu_dit_b200.model_executor.layers import int8_linear
+    from tests.test_host_dispatch import _hook, _other_weight, _own_forward, _pre_hook
+    monkeypatch.setattr(kernels, "quantize_rows", lambda w: rows8(*w.shape))
+    changes = [_hook, _pre_hook, _own_forward, _other_weight, lambda layer: layer.register_full_backward_hook(lambda m, a, b: None),
+               lambda layer: torch.nn.utils.parametrizations.weight_norm(layer)]
+    net = torch.nn.ModuleList([torch.nn.Linear(8, 8) for _ in changes] + [torch.nn.Linear(8, 8), None])
+    for change, layer in zip(changes, net):
+        change(layer)
+    kept = list(net)[:len(changes)]
+    int8_linear.quantize_linears_(net)
+    assert all(a is b for a, b in zip(net, kept)) and type(net[len(changes)]) is int8_linear.Int8Linear
+    # what waits for the calls of all modules waits for the 8-bit layer's, too
+    net = torch.nn.ModuleList([torch.nn.Linear(8, 8)])
+    handle = torch.nn.modules.module.register_module_forward_hook(lambda m, a, y: None)
+    try:
+        int8_linear.quantize_linears_(net)
+    finally:
+        handle.remove()
+    assert type(net[0]) is int8_linear.Int8Linear
