@@ -20,6 +20,20 @@ def refuse_gradients(*tensors):
         raise RuntimeError("8-bit linear layers have no gradients: run them under torch.no_grad() or on tensors that require none")
 
 
+def _whole_rows(q):
+    """The rows (n, k) with what lies behind each up to the next 16-byte boundary, so that a copy of them keeps the rows on such
+    boundaries: the same memory, or a copy where the rows are not on such boundaries or the memory ends before the last one's."""
+    n, k = q.shape
+    width = (k + 15) & ~15
+    pitch = q.stride(0) if n > 1 else width
+    if pitch % 16 == 0 and pitch >= width and q.data_ptr() % 16 == 0 and \
+            q.storage_offset() + (n - 1) * pitch + width <= q.untyped_storage().nbytes():
+        return q.as_strided((n, width), (pitch, 1))
+    whole = q.new_zeros(n, width)
+    whole[:, :k] = q
+    return whole
+
+
 class Int8Linear(nn.Module):
     """x @ weight.T + bias with the weight in 8 bits, in place of a torch.nn.Linear. x: a 16-bit tensor that no gradient is
     recorded for, or kernels.Int8Rows."""
@@ -27,10 +41,7 @@ class Int8Linear(nn.Module):
     def __init__(self, weight: kernels.Int8Rows, bias=None):
         super().__init__()
         self.out_features, self.in_features = weight.shape
-        pitch = weight.q.stride(0) if self.out_features > 1 else (self.in_features + 15) & ~15
-        # the whole rows, padding included: a copy of them keeps the rows on 16-byte boundaries
-        self.register_buffer("weight_q", weight.q if pitch == self.in_features else
-                             weight.q.as_strided((self.out_features, pitch), (pitch, 1)))
+        self.register_buffer("weight_q", _whole_rows(weight.q))
         self.register_buffer("weight_scale", weight.scale)
         self.register_buffer("bias", None if bias is None else bias.detach().clone())
         self.dtype = weight.dtype

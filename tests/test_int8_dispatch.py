@@ -414,3 +414,20 @@ def test_a_layer_that_something_was_put_on_stays(monkeypatch):
     finally:
         handle.remove()
     assert type(net[0]) is int8_linear.Int8Linear
+
+
+@pytest.mark.parametrize("n,k,width,first", [(5, 40, 96, 48), (5, 40, 96, 0), (5, 40, 48, 0), (1, 40, 40, 0), (1, 40, 64, 16), (5, 32, 96, 64), (5, 40, 88, 48),
+                                             (5, 40, 88, 0), (5, 32, 40, 8)])
+def test_an_8_bit_layer_of_rows_that_a_program_has_laid_out(n, k, width, first):
+    """Columns of wider rows; the last ones end where the memory ends."""
+    from hetu_dit_b200.model_executor.layers.int8_linear import Int8Linear
+    buf = torch.randint(-127, 128, (n, width), dtype=torch.int8)
+    q = buf[:, first:first + k]
+    layer = Int8Linear(kernels.Int8Rows(q, torch.rand(n)))
+    assert layer.weight_q.stride(0) % 16 == 0 and layer.weight_q.data_ptr() % 16 == 0
+    for copied in (layer, Int8Linear(kernels.Int8Rows(torch.zeros(n, k, dtype=torch.int8), torch.zeros(n)))):
+        copied.load_state_dict(layer.state_dict())
+        rows = copied.rows
+        assert torch.equal(rows.q, q) and rows.shape == (n, k) and torch.equal(rows.scale, layer.weight_scale)
+    moved = layer.weight_q.clone()  # as a copy to another device lays it out
+    assert moved.stride(0) % 16 == 0 and torch.equal(moved[:, :k], q)
