@@ -660,6 +660,11 @@ extern "C" int hdit_group_norm(const hdit_group_norm_args* a) {
   using namespace hdit;
   const int rc = check_gn(a);
   if (rc != HDIT_OK || a->batch == 0 || a->rows == 0) return rc;
+  // rows one after the other, and images one after the other or their rows in turn
+  const int64_t row = a->out_row_stride, image = a->out_batch_stride;
+  const bool rows_apart = a->rows == 1 || row >= a->channels;
+  const bool images_apart = a->batch == 1 || image >= (a->rows - 1) * row + a->channels || (image >= a->channels && row >= (a->batch - 1) * image + a->channels);
+  if (!rows_apart || !images_apart) return set_error(HDIT_ERR_SHAPE, "rows of out overlap");
   return run_group_norm(a, false);
 }
 

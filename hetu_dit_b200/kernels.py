@@ -1123,7 +1123,9 @@ def linear_int8(x, weight, bias=None, epilogue="bias", residual=None, gate=None,
     else:
         if out.shape != (B, S, n) or out.dtype != dtype or out.device != dev or (out.stride(2) != 1 and n != 1):
             raise ValueError("out does not match (B, S, N), x's dtype or its device")
-        so = out.stride(1)
+        so, sb_out = out.stride(1), out.stride(0)
+        if B > 1 and S > 0 and not (sb_out >= (S - 1) * so + n or (sb_out >= n and so >= (B - 1) * sb_out + n)):
+            raise ValueError("rows of out overlap")
     if B > 1 and not (one_pitch and _even_rows(out) and (not gated or _even_rows(residual))):
         for b in range(B):  # a slice of the rows of every entry: one launch per entry
             xb = Int8Rows(x.q[b:b + 1], x.scale[b:b + 1], dtype) if held else x[b:b + 1]

@@ -600,7 +600,7 @@ HDIT_API int hdit_int8_linear(const hdit_int8_linear_args* args);
  * GroupNorm over channels-last images, then an activation:
  *   out[b, r, c] = act((x[b, r, c] - mean[b, g]) / sqrt(var[b, g] + eps) * weight[c] + bias[c]),  g = c / (channels / groups)
  * with mean and biased variance over the rows r (pixels) and channels of group g, fp32 arithmetic, 16-bit storage. x and out are
- * (batch, rows, channels) with contiguous channels, any batch and row strides (elements); channels a multiple of 8 and of
+ * (batch, rows, channels) with contiguous channels, any batch and row strides (elements) that keep the rows of out apart; channels a multiple of 8 and of
  * groups, at most 4096; weight and bias `channels` elements each or NULL (1 and 0). scratch: hdit_group_norm_scratch() bytes
  * (0: none is needed), 8-byte aligned, of which nothing has to be kept before or after the call; calls that may overlap need one each. `out` may be x.
  * hdit_group_norm_int8 writes each row (all channels of a pixel) as an 8-bit row instead: out is int8, rows of all images in

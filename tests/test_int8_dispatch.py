@@ -431,3 +431,24 @@ def test_an_8_bit_layer_of_rows_that_a_program_has_laid_out(n, k, width, first):
         assert torch.equal(rows.q, q) and rows.shape == (n, k) and torch.equal(rows.scale, layer.weight_scale)
     moved = layer.weight_q.clone()  # as a copy to another device lays it out
     assert moved.stride(0) % 16 == 0 and torch.equal(moved[:, :k], q)
+
+
+def test_a_result_whose_rows_overlap_is_refused(lib, monkeypatch):  # noqa: F811
+    monkeypatch.setattr(kernels, "_cuda_index", lambda device: 0)
+    kw = dict(x=gpu_like(3, 40, 32), residual=gpu_like(3, 40, 24), gate=gpu_like(3, 24))
+    for out in (gpu_like(1, 40, 24).expand(3, 40, 24), gpu_like(80, 24).as_strided((3, 40, 24), (20 * 24, 24, 1))):
+        with pytest.raises(ValueError, match="overlap"):
+            _linear(out=out, **kw)
+    assert lib.calls == []
+    _linear(out=gpu_like(40, 3, 24).transpose(0, 1), **kw)  # the entries' rows in turn
+    assert [c[0] for c in lib.calls] == ["hdit_int8_linear"] * 3
+
+
+def test_the_library_refuses_an_image_whose_rows_overlap():
+    a = _C.GroupNormArgs()
+    for name, v in dict(dtype=0, act=0, x=4096, out=4096, batch=3, rows=4, channels=64, groups=8, x_row_stride=64, out_batch_stride=256,
+                        out_row_stride=64, eps=1e-6).items():
+        setattr(a, name, v)
+    for row, image in ((0, 256), (63, 256), (64, 0), (64, 255), (128, 64), (-64, 256), (64, -256)):
+        a.out_row_stride, a.out_batch_stride = row, image
+        assert _C.lib().hdit_group_norm(ctypes.byref(a)) == _C.HDIT_ERR_SHAPE, (row, image)
