@@ -1052,6 +1052,12 @@ def _overlap(a, b):
     return a0 < b1 and b0 < a1
 
 
+def _few_rows_fit(m, k):
+    """Whether the kernel for a few rows has room for them (int8_linear_few_takes() in csrc/int8_linear_few.cu)."""
+    pitch = (k + 63) & ~63
+    return m * (pitch if pitch % 128 else pitch + 64) <= 160 << 10
+
+
 _TAILS = {"bias": _C.GEMM_BIAS, "gelu_tanh": _C.GEMM_BIAS_GELU_TANH, "gate_residual": _C.GEMM_BIAS_GATE_RESIDUAL}
 
 
@@ -1147,7 +1153,8 @@ def linear_int8(x, weight, bias=None, epilogue="bias", residual=None, gate=None,
     else:
         a.x, a.lda, a.x_rows_per_batch, a.x_batch_stride, a.x_row_stride = xr.data_ptr(), pitch, S, sb, ss
         # the kernel for a few rows does it all (int8_linear_few_quantizes() in csrc/int8_linear_few.cu)
-        one = tile in (0, 5) and (own or not _overlap(x, out)) and (m <= 2 or m <= 8 and k <= (1024 if m > 4 else 2048) and n <= 2368)
+        one = tile in (0, 5) and (m <= 2 and (k <= 65536 or _few_rows_fit(m, k)) or m <= 8 and k <= (1024 if m > 4 else 2048) and n <= 2368) \
+            and (own or not _overlap(x, out))
         launches = 1 if one else 2
         if not (one and own and m <= 2 and k <= 65536):  # the rows in 8 bits, their scales behind them: scratch of the call
             scratch = torch.empty(m * (pitch + 4), dtype=torch.int8, device=dev)

@@ -805,7 +805,7 @@ def test_aligned_products_keep_their_values_in_registers(tile, epilogue, dtype):
 @pytest.mark.parametrize("m,k,n,held,placed,count", [
     (1, 1536, 9216, False, False, 1), (2, 1536, 9216, False, True, 1), (2, 70000, 32, False, False, 1), (4, 2048, 2048, False, False, 1),
     (8, 1024, 2368, False, True, 1), (4, 1536, 9216, False, False, 2), (8, 768, 9216, False, False, 2), (5, 1536, 512, False, False, 2),
-    (8, 256, 2369, False, False, 2), (9, 64, 64, False, False, 2), (8, 512, 512, True, False, 1), (300, 512, 512, False, True, 2)])
+    (8, 256, 2369, False, False, 2), (9, 64, 64, False, False, 2), (1, 131072, 16, False, False, 1), (2, 81856, 16, False, False, 1), (2, 81857, 16, False, False, 2), (8, 512, 512, True, False, 1), (300, 512, 512, False, True, 2)])
 def test_launches_of_a_few_rows(m, k, n, held, placed, count):
     """In a graph a launch more costs less than rows brought into 8 bits by several CTAs of an SM, or in several turns. What is
     counted is what is launched."""
