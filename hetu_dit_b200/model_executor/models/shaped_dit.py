@@ -472,8 +472,7 @@ class ShapedDiT(nn.Module):
         the GPU, inference only: no parameter of the model asks for a gradient from then on. The embedders and the output layer
         stay as they are. Not for a model whose blocks a block cache moves between plans, which addresses torch.nn.Linear
         weights."""
-        for blk in list(self.transformer_blocks) + list(self.single_transformer_blocks):
-            quantize_linears_(blk)
+        quantize_linears_(nn.ModuleList([self.transformer_blocks, self.single_transformer_blocks]))  # all blocks' layers or none
         return self.requires_grad_(False)
 
     def register_cache(self):

@@ -452,3 +452,21 @@ def test_the_library_refuses_an_image_whose_rows_overlap():
     for row, image in ((0, 256), (63, 256), (64, 0), (64, 255), (128, 64), (-64, 256), (64, -256)):
         a.out_row_stride, a.out_batch_stride = row, image
         assert _C.lib().hdit_group_norm(ctypes.byref(a)) == _C.HDIT_ERR_SHAPE, (row, image)
+
+
+def test_a_layer_that_cannot_be_in_8_bits_leaves_all_blocks_as_they_were(monkeypatch):
+    from hetu_dit_b200.model_executor.models.shaped_dit import ShapedDiT
+    from tests.test_gpu_model import tiny_shape
+
+    def quantize_rows(w):
+        if w.dtype == torch.float64:
+            raise TypeError("unsupported dtype")
+        return rows8(*w.shape)
+
+    monkeypatch.setattr(kernels, "quantize_rows", quantize_rows)
+    model = ShapedDiT(tiny_shape("flux")[0])
+    layers = sum(type(m) is torch.nn.Linear for m in model.modules())
+    model.single_transformer_blocks[-1].proj_out.double()
+    with pytest.raises(TypeError):
+        model.quantize_linears_()
+    assert sum(type(m) is torch.nn.Linear for m in model.modules()) == layers and any(p.requires_grad for p in model.parameters())
