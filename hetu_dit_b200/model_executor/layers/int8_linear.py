@@ -102,9 +102,10 @@ def _places(module):
 @torch.no_grad()
 def quantize_linears_(module: nn.Module):
     """Puts an Int8Linear in the place of every torch.nn.Linear below `module` (16-bit, on the GPU); returns module. What has
-    another class (an adapter), and a layer with a hook, a forward() or a weight of a class of its own, stays. A layer that cannot be brought into 8 bits (another type, another device) raises before any
-    is replaced. Steps captured in CUDA graphs before hold the addresses of the 16-bit weights: those of every StepGraphCache are
-    dropped. Block caches address torch.nn.Linear weights by name: a module whose slices migrate between plans keeps them."""
+    another class (an adapter), and a layer with a hook, a forward() or a weight of a class of its own, stays. A layer that
+    cannot be brought into 8 bits (another type, another device) raises before any is replaced. Steps captured in CUDA graphs
+    before hold the addresses of the 16-bit weights: those of every StepGraphCache are dropped. Block caches address
+    torch.nn.Linear weights by name: a module whose slices migrate between plans keeps them."""
     places = _places(module)
     for parent, name in places:
         kernels.quantize_rows(parent._modules[name].weight.detach()[:0])  # all that it asks of a weight, and nothing launched
